@@ -308,6 +308,91 @@ int32_t sl_op_head(sl_engine* e, const uint16_t* h_rows_f16, int32_t M, uint16_t
 /* final-norm'ed rows -> logits (may be NULL) and greedy tokens (may be NULL). */
 int32_t sl_op_lm_head(sl_engine* e, const uint16_t* normed_f16, int32_t M, uint16_t* out_logits_f16, int32_t* out_tokens);
 
+/* ---- a KV cache held in 4 bits, and what a step does with it (NO COUNTERPART IN THE REFERENCE, whose caches are fp16) ----
+ * All pointers are device pointers unless marked host; every call enqueues on cuda_stream, whose device must be current, and
+ * returns without synchronising.  Nothing is allocated.  Rows and heads are addressed by strides in halves (multiples of 8) from
+ * 16-byte aligned pointers; a head's dims are contiguous.
+ *
+ * Layout.  A page of one layer is [kv_heads][page_size / 16][18 * head_dim] bytes: blocks of 16 positions of one head.  Block: K codes
+ * (8 * head_dim bytes), V codes, K scales and biases (head_dim bytes), V scales and biases.  A position's codes are head_dim / 2 bytes,
+ * low nibble first; the 16-byte piece at byte o of a code region stands at o ^ (16 * (o / 128 mod 8)).  Scales and biases: per 64 dims
+ * 16 fp16 scales, then 16 fp16 biases.  An element is worth fp16(code * scale + bias), the scheme of the 4-bit weights; a 64-dim group
+ * that an infinity or a NaN went into reads back as NaN. */
+typedef struct sl_kv4_cache {
+    void* data;              /* 16-byte aligned */
+    int64_t page_stride;     /* bytes from a page to the next: sl_kv4_page_bytes() or more (several layers in one page), a multiple of 16 */
+    int32_t pages;
+    int32_t page_size;       /* positions, a multiple of 16 */
+    int32_t kv_heads;
+    int32_t head_dim;        /* 64, 128 or 256 */
+} sl_kv4_cache;
+/* Bytes of one page of one layer, or SL_ERR_INVALID. */
+int64_t sl_kv4_page_bytes(int32_t kv_heads, int32_t head_dim, int32_t page_size);
+
+/* Page tables, slot map, positions and row offsets of a step from the requests' lengths.  Request b has lens[b] positions cached and
+ * new_rows[b] rows to come; new_rows[b] < 0: it has ended, its pages go back onto the stack of free pages.  Then the tables of the others
+ * grow to ceil((lens + new_rows) / page_size) pages, request by request from the top of the stack.
+ * status: [0] pages short, [1] requests whose length is negative or longer than a table row (and 1 more when the stack has no room
+ * for what returns), [2] rows beyond max_rows.  Unless all three are 0 nothing is planned: tables, stack and lengths stay, q_start is 0
+ * throughout, every slot -1.  kv_len may be lens and free_count_out may be free_count; nothing else may overlap. */
+typedef struct sl_kv_plan {
+    const int32_t* lens; const int32_t* new_rows;            /* [batch] */
+    int32_t batch, page_size;
+    int32_t* table; int64_t table_stride; int32_t table_width;   /* [batch][table_width] pages, rows table_stride apart: grown in place */
+    int32_t* free_pages; int32_t free_capacity;              /* the stack of free pages; its top is at free_count - 1 */
+    const int32_t* free_count;                               /* [1] */
+    int32_t* kv_len;                                         /* out [batch]: lens + new_rows, 0 of an ended request */
+    int32_t* q_start;                                        /* out [batch + 1]: first row of each request */
+    int64_t* slots; int32_t* pos; int32_t max_rows;          /* out [max_rows]: page * page_size + offset and position of each row; -1, 0 behind the last */
+    int32_t* free_count_out;                                 /* out [1] */
+    int32_t* status;                                         /* out [3] */
+} sl_kv_plan;
+int32_t sl_op_kv_plan_device(const sl_kv_plan* plan, void* cuda_stream);
+
+/* Query and key norm, rotation, and the rows' K and V into the cache.  For every head x of a row: y = rope(x * rsqrt(mean(x^2) + eps) * w);
+ * queries go to q_out (which may be q), keys are rounded to fp16 and quantised at the row's slot, values as they are.  Rotation: dims d and
+ * d + rope_dims / 2 of the first rope_dims by the angle pos[axis_of[d]][row] * rope_theta^(-2 d / rope_dims).
+ * A row whose slot is not one of the cache's is padding: nothing of it is written.  The slots of a call must differ. */
+typedef struct sl_kv4_append {
+    const uint16_t *q, *k, *v;                               /* fp16; q NULL: no queries; k and v NULL: queries alone (slots may be NULL then) */
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+    uint16_t* q_out; int64_t q_out_row, q_out_head;
+    int32_t rows, q_heads;
+    const uint16_t *q_norm, *k_norm; float eps;              /* fp16 [head_dim], NULL: no norm */
+    const int32_t* pos; int64_t pos_axis; int32_t axes;      /* [axes][rows], axes pos_axis apart */
+    int32_t rope_dims; float rope_theta;                     /* 0 (no rotation) or a multiple of 16 up to head_dim; theta >= 1 */
+    const uint8_t* axis_of;                                  /* host [rope_dims / 2]: the position axis of each frequency; NULL: axis 0 */
+    const int64_t* slots;                                    /* [rows] */
+} sl_kv4_append;
+int32_t sl_op_kv4_append_device(const sl_kv4_cache* cache, const sl_kv4_append* rows, void* cuda_stream);
+
+/* K and V at given slots as fp16 [rows][kv_heads][head_dim]; rows whose slot is not one of the cache's are left as they were. */
+typedef struct sl_kv4_read {
+    const int64_t* slots; int32_t rows;
+    uint16_t *k, *v; int64_t k_row, k_head, v_row, v_head;
+} sl_kv4_read;
+int32_t sl_op_kv4_read_device(const sl_kv4_cache* cache, const sl_kv4_read* rows, void* cuda_stream);
+
+/* out = softmax(scale * q K^T) V [* sigmoid(gate)] for the rows q_start[b] .. q_start[b + 1] - 1 of every request b over its positions
+ * 0 .. kv_len[b] - 1; query head h reads kv head h / (q_heads / kv_heads), at most 128 of them one kv head.  causal: row i of a request's n
+ * sees the first kv_len - n + i + 1 positions.  A row that sees none is zero; table entries that are no page of the cache hold no keys; rows of
+ * no request, and rows of a request behind its first max_q, are left as they were.
+ * workspace: 16-byte aligned, sl_kv4_attention_workspace() bytes (the same arguments), any contents; calls that may run at the same
+ * time need one each. */
+typedef struct sl_kv4_attention {
+    const uint16_t* q; int64_t q_row, q_head;
+    const uint16_t* gate; int64_t gate_row, gate_head;       /* NULL: no gate */
+    uint16_t* out; int64_t out_row, out_head;                /* may be q */
+    int32_t rows, q_heads;                                   /* rows of q, gate and out */
+    const int32_t *q_start, *kv_len; int32_t batch;
+    int32_t max_q;                                           /* most rows of a request */
+    const int32_t* table; int64_t table_stride; int32_t table_width;
+    int32_t causal; float scale;
+    void* workspace; uint64_t workspace_bytes;
+} sl_kv4_attention;
+int64_t sl_kv4_attention_workspace(int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t batch, int32_t max_q, int32_t rows);
+int32_t sl_op_kv4_attention_device(const sl_kv4_cache* cache, const sl_kv4_attention* call, void* cuda_stream);
+
 /* ---- synthetic data helpers (same generator as the engine's weights) ---- */
 int32_t sl_synth_tokens(uint64_t seed, const char* name, int64_t n, int32_t vocab, int32_t* out);
 int32_t sl_synth_f16(uint64_t seed, const char* name, int64_t n, float mean, float std, uint16_t* out_f16);

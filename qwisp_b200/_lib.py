@@ -47,6 +47,42 @@ class SlSnap(C.Structure):
     _fields_ = [("kv_len", C.c_int32), ("parity", C.c_int32), ("valid", C.c_int32), ("calls", C.c_int32)]
 
 
+class SlKv4Cache(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("page_stride", C.c_int64),
+                ("pages", C.c_int32), ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class SlKvPlan(C.Structure):
+    _fields_ = [("lens", C.c_void_p), ("new_rows", C.c_void_p), ("batch", C.c_int32), ("page_size", C.c_int32),
+                ("table", C.c_void_p), ("table_stride", C.c_int64), ("table_width", C.c_int32),
+                ("free_pages", C.c_void_p), ("free_capacity", C.c_int32), ("free_count", C.c_void_p),
+                ("kv_len", C.c_void_p), ("q_start", C.c_void_p), ("slots", C.c_void_p), ("pos", C.c_void_p), ("max_rows", C.c_int32),
+                ("free_count_out", C.c_void_p), ("status", C.c_void_p)]
+
+
+class SlKv4Append(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("q_row", C.c_int64), ("q_head", C.c_int64), ("k_row", C.c_int64), ("k_head", C.c_int64), ("v_row", C.c_int64), ("v_head", C.c_int64),
+                ("q_out", C.c_void_p), ("q_out_row", C.c_int64), ("q_out_head", C.c_int64), ("rows", C.c_int32), ("q_heads", C.c_int32),
+                ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("eps", C.c_float),
+                ("pos", C.c_void_p), ("pos_axis", C.c_int64), ("axes", C.c_int32), ("rope_dims", C.c_int32), ("rope_theta", C.c_float),
+                ("axis_of", C.c_char_p), ("slots", C.c_void_p)]
+
+
+class SlKv4Read(C.Structure):
+    _fields_ = [("slots", C.c_void_p), ("rows", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("k_row", C.c_int64), ("k_head", C.c_int64), ("v_row", C.c_int64), ("v_head", C.c_int64)]
+
+
+class SlKv4Attention(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("q_row", C.c_int64), ("q_head", C.c_int64),
+                ("gate", C.c_void_p), ("gate_row", C.c_int64), ("gate_head", C.c_int64),
+                ("out", C.c_void_p), ("out_row", C.c_int64), ("out_head", C.c_int64), ("rows", C.c_int32), ("q_heads", C.c_int32),
+                ("q_start", C.c_void_p), ("kv_len", C.c_void_p), ("batch", C.c_int32), ("max_q", C.c_int32),
+                ("table", C.c_void_p), ("table_stride", C.c_int64), ("table_width", C.c_int32), ("causal", C.c_int32), ("scale", C.c_float),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
 # every symbol include/seedless_b200.h declares: name -> (restype, argtypes)
 _VP, _I32, _I64, _U64, _F = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64, C.c_float
 SYMBOLS = {
@@ -103,6 +139,12 @@ SYMBOLS = {
     "sl_op_read_kv": (_I32, [_VP, _I32, _I32, _I32, _VP, _VP]),
     "sl_op_layer": (_I32, [_VP, _I32, _VP, _I32, _I32, _VP]),
     "sl_op_head": (_I32, [_VP, _VP, _I32, _VP, _VP]),
+    "sl_kv4_page_bytes": (_I64, [_I32, _I32, _I32]),
+    "sl_op_kv_plan_device": (_I32, [C.POINTER(SlKvPlan), _VP]),
+    "sl_op_kv4_append_device": (_I32, [C.POINTER(SlKv4Cache), C.POINTER(SlKv4Append), _VP]),
+    "sl_op_kv4_read_device": (_I32, [C.POINTER(SlKv4Cache), C.POINTER(SlKv4Read), _VP]),
+    "sl_kv4_attention_workspace": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32]),
+    "sl_op_kv4_attention_device": (_I32, [C.POINTER(SlKv4Cache), C.POINTER(SlKv4Attention), _VP]),
     "sl_synth_tokens": (_I32, [_U64, C.c_char_p, _I64, _I32, _VP]),
     "sl_synth_f16": (_I32, [_U64, C.c_char_p, _I64, _F, _F, _VP]),
 }

@@ -160,16 +160,6 @@ int32_t guard(sl_engine* e) {
     return SL_OK;
 }
 
-// (a device once found stays: asking the driver again is 0.26 us of the 8 that a single-operator call takes)
-bool device_ok() {
-    static std::atomic<bool> found{false};
-    if (found.load(std::memory_order_relaxed)) return true;
-    int n = 0;
-    if (cudaGetDeviceCount(&n) != cudaSuccess || n <= 0) { cudaGetLastError(); return false; }
-    found.store(true, std::memory_order_relaxed);
-    return true;
-}
-
 template <typename T>
 int32_t dalloc(sl_engine* e, T** out, size_t count) {
     void* p = nullptr;

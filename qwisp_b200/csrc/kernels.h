@@ -197,6 +197,7 @@ struct StepEndArgs {
 };
 
 int sm_count();
+bool device_ok();                          // is there a CUDA device?
 // ---- the one-kernel decode step (step_persistent.cu) ----
 struct PsGeom {
     int G;                                  // CTAs (one per multiprocessor)

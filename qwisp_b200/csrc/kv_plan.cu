@@ -1,0 +1,168 @@
+// kv_plan.cu -- page tables, slot map, positions and row offsets of a step, on the device, from the requests' lengths.
+//
+// Request b has lens[b] positions cached and news[b] rows to come (negative: it has ended and gives its pages back).  With
+// have = ceil(lens / P) and need = ceil((lens + news) / P) its table grows by need - have pages, taken from the top of the stack of
+// free pages; the rows' offsets, the pages returned and the pages taken are prefix sums over the requests, so the result does not
+// depend on the order in which threads run.  All of it or nothing: where pages, table columns or rows are short, the tables and the
+// stack stay as they are and the status says what was short.
+//
+// A few hundred requests are bound by latency alone (three dependent loads and the launch), so one CTA does everything: sums, pages and,
+// up to PLAN_ROWS of them, the rows.  More rows get a kernel of their own over the whole device.
+#include "kv4.cuh"
+
+namespace sl {
+
+constexpr int PLAN_T = 1024;             // threads, and requests of a chunk
+constexpr int PLAN_ROWS = 8192;
+
+struct PlanSums { long long rows; int back, grown, bad; };
+struct PlanOne { long long len; int rows, have, need; bool ended, bad; };
+
+__device__ __forceinline__ PlanOne plan_one(const KvPlanArgs& a, int b) {
+    PlanOne r{0, 0, 0, 0, false, false};
+    if (b >= a.batch) return r;
+    const int len = a.lens[b], n = a.news[b];
+    r.len = len; r.ended = n < 0; r.rows = n < 0 ? 0 : n;
+    const long long have = (r.len + a.page_size - 1) / a.page_size, need = (r.len + r.rows + a.page_size - 1) / a.page_size;
+    r.bad = len < 0 || need > a.table_width || r.len + r.rows > 0x7fffffffll;
+    if (r.bad) r.rows = 0;
+    else { r.have = (int)have; r.need = r.ended ? 0 : (int)need; }
+    return r;
+}
+// inclusive sums over the CTA of two values; all threads call it
+__device__ __forceinline__ void plan_scan(int& x, int& y, int (*ws)[32]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, x, d), v = __shfl_up_sync(0xffffffffu, y, d);
+        if (lane >= d) { x += u; y += v; }
+    }
+    if (lane == 31) { ws[0][warp] = x; ws[1][warp] = y; }
+    __syncthreads();
+    if (warp == 0) {
+        int u = ws[0][lane], v = ws[1][lane];
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int p = __shfl_up_sync(0xffffffffu, u, d), q = __shfl_up_sync(0xffffffffu, v, d);
+            if (lane >= d) { u += p; v += q; }
+        }
+        ws[0][lane] = u; ws[1][lane] = v;
+    }
+    __syncthreads();
+    if (warp) { x += ws[0][warp - 1]; y += ws[1][warp - 1]; }
+    __syncthreads();
+}
+// the last i of [0, n) with start[i] <= v (start[0] <= v)
+__device__ __forceinline__ int plan_find(const int* start, int n, int v) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (start[mid] <= v) lo = mid; else hi = mid - 1; }
+    return lo;
+}
+__device__ __forceinline__ void plan_row(const KvPlanArgs& a, int r, int total) {
+    int64_t slot = -1; int pos = 0;
+    if (r < total) {
+        const int b = plan_find(a.q_start, a.batch, r);       // (requests without rows share the next one's offset: the last is meant)
+        pos = a.kv_len[b] - (a.q_start[b + 1] - r);
+        slot = (int64_t)a.table[(int64_t)b * a.table_stride + pos / a.page_size] * a.page_size + pos % a.page_size;
+    }
+    a.slots[r] = slot; a.pos[r] = pos;
+}
+
+__global__ void __launch_bounds__(PLAN_T) k_kv_plan(KvPlanArgs a, int rows_here) {
+    __shared__ int ws[2][32], s_back[PLAN_T], s_grown[PLAN_T], s_have[PLAN_T];
+    __shared__ unsigned long long s_rows;
+    __shared__ int s_tot[3];
+    const int tid = threadIdx.x;
+    if (tid == 0) { s_rows = 0; s_tot[0] = s_tot[1] = s_tot[2] = 0; }
+    __syncthreads();
+    // ---- what the whole step needs
+    const int F = *a.free_count;
+    PlanOne mine = plan_one(a, tid);
+    {
+        long long rows = 0, back = 0, grown = 0; int bad = 0;
+        for (int b = tid; b < a.batch; b += PLAN_T) {
+            const PlanOne r = b == tid ? mine : plan_one(a, b);
+            rows += r.rows; bad += r.bad;
+            if (r.ended) back += r.have; else grown += r.need - r.have;
+        }
+        // (pages and requests number below 2^31 in all: what a table of int32 pages can hold)
+        atomicAdd(&s_rows, (unsigned long long)rows);
+        if (back) atomicAdd(&s_tot[0], (int)back);
+        if (grown) atomicAdd(&s_tot[1], (int)grown);
+        if (bad) atomicAdd(&s_tot[2], bad);
+    }
+    __syncthreads();
+    const long long rows = (long long)s_rows;
+    const int back = s_tot[0], grown = s_tot[1];
+    const bool stack_bad = F < 0 || (long long)F + back > a.free_cap;
+    const long long top = (long long)F + back;
+    const int bad = s_tot[2] + (stack_bad ? 1 : 0);
+    const long long shrt = stack_bad || grown <= top ? 0 : grown - top, over = rows > a.max_rows ? rows - a.max_rows : 0;
+    const bool fine = !bad && !shrt && !over;
+    if (tid == 0) {
+        a.status[0] = (int)shrt; a.status[1] = bad; a.status[2] = (int)(over > 0x7fffffffll ? 0x7fffffffll : over);
+        *a.free_count_out = fine ? (int)(top - grown) : F;
+        a.q_start[a.batch] = fine ? (int)rows : 0;
+    }
+    if (!fine) {
+        for (int b = tid; b < a.batch; b += PLAN_T) { const int len = a.lens[b]; a.q_start[b] = 0; a.kv_len[b] = len; }
+        for (int r = tid; rows_here && r < a.max_rows; r += PLAN_T) { a.slots[r] = -1; a.pos[r] = 0; }
+        return;
+    }
+    // ---- pages of ended requests onto the stack
+    if (back) {
+        int base = F;
+        for (int b0 = 0; b0 < a.batch; b0 += PLAN_T) {
+            const PlanOne r = b0 ? plan_one(a, b0 + tid) : mine;
+            int x = r.ended ? r.have : 0, y = 0;
+            const int own = x;
+            plan_scan(x, y, ws);
+            s_back[tid] = x - own;
+            __syncthreads();
+            const int n = ws[0][31];
+            for (int i = tid; i < n; i += PLAN_T) {
+                const int j = plan_find(s_back, PLAN_T, i);
+                a.free_pages[base + i] = a.table[(int64_t)(b0 + j) * a.table_stride + i - s_back[j]];
+            }
+            base += n;
+            __syncthreads();
+        }
+    }
+    // ---- row offsets, new lengths, pages off the stack
+    int row0 = 0, taken = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += PLAN_T) {
+        const PlanOne r = b0 ? plan_one(a, b0 + tid) : mine;
+        const int own = r.ended ? 0 : r.need - r.have;
+        int x = r.rows, y = own;
+        plan_scan(x, y, ws);
+        s_grown[tid] = y - own; s_have[tid] = r.have;
+        if (b0 + tid < a.batch) {
+            a.q_start[b0 + tid] = row0 + x - r.rows;
+            a.kv_len[b0 + tid] = r.ended ? 0 : (int)r.len + r.rows;           // (may be the array of lengths: its reader was this thread)
+        }
+        __syncthreads();
+        const int n = ws[1][31];
+        for (int i = tid; i < n; i += PLAN_T) {
+            const int j = plan_find(s_grown, PLAN_T, i);
+            a.table[(int64_t)(b0 + j) * a.table_stride + s_have[j] + i - s_grown[j]] = a.free_pages[top - 1 - taken - i];
+        }
+        row0 += ws[0][31]; taken += n;
+        __syncthreads();
+    }
+    if (rows_here) for (int r = tid; r < a.max_rows; r += PLAN_T) plan_row(a, r, (int)rows);
+}
+__global__ void __launch_bounds__(256) k_kv_plan_rows(KvPlanArgs a) {
+    pdl_wait();
+    const int r = blockIdx.x * 256 + threadIdx.x;
+    if (r < a.max_rows) plan_row(a, r, a.q_start[a.batch]);
+}
+
+int launch_kv_plan(const KvPlanArgs& a, cudaStream_t st) {
+    const bool here = a.max_rows <= PLAN_ROWS;
+    int rc = 0;
+    profile_launch("k_kv_plan", st, [&] { return rc = launch_pdl(false, k_kv_plan, dim3(1), PLAN_T, 0, st, a, here ? 1 : 0); });
+    if (rc == 0 && !here) profile_launch("k_kv_plan_rows", st, [&] { return rc = launch_pdl(false, k_kv_plan_rows, dim3((unsigned)((a.max_rows + 255) / 256)), 256, 0, st, a); });
+    return rc;
+}
+
+}  // namespace sl
