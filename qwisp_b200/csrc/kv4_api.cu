@@ -95,7 +95,9 @@ int32_t sl_op_kv4_attention_device(const sl_kv4_cache* cache, const sl_kv4_atten
     if (!p->q || !p->out || !p->q_start || !p->workspace || ((uintptr_t)p->workspace & 15)) return SL_ERR_INVALID;
     if (p->batch && (!p->kv_len || (!p->table && p->table_width) || p->table_stride < p->table_width)) return SL_ERR_INVALID;
     if (!aligned(p->q, p->q_row, p->q_head) || !aligned(p->out, p->out_row, p->out_head) || (p->gate && !aligned(p->gate, p->gate_row, p->gate_head))) return SL_ERR_INVALID;
-    if (p->q_heads / c.KV > 128 || p->batch > 65535 || (int64_t)p->table_width * c.page_size > 0x7fffffffll - 65536) return SL_ERR_CAPACITY;
+    // (positions and key blocks are counted in 31 bits)
+    const int64_t span = (int64_t)p->table_width * c.page_size;
+    if (p->q_heads / c.KV > 128 || p->batch > 4096 || span > 0x7fffffffll - 65536 || (span / KV4_B + 1) * p->batch * c.KV > 0x7fffffffll - 65536) return SL_ERR_CAPACITY;
     if (!device_ok()) return SL_ERR_NO_DEVICE;
     if (p->rows == 0 || p->batch == 0) return SL_OK;
     if (p->workspace_bytes < kv4_attn_workspace(c.D, p->q_heads / c.KV, c.KV, p->batch, p->max_q, p->rows)) return SL_ERR_CAPACITY;

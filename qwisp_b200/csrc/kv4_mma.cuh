@@ -1,0 +1,45 @@
+// kv4_mma.cuh -- pieces of the attention kernels over the cache held in 4 bits.
+#pragma once
+#include "common.cuh"
+#include <atomic>
+
+namespace sl {
+
+__device__ __forceinline__ void kv4_cp16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void kv4_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void kv4_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void kv4_ldsm(uint32_t r[4], uint32_t p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
+}
+__device__ __forceinline__ void kv4_ldsm_t(uint32_t r[4], uint32_t p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
+}
+__device__ __forceinline__ void kv4_mma(float c[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// an 8 x 8 matrix of halves, two of a row a lane, transposed
+__device__ __forceinline__ uint32_t kv4_transpose(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ float kv4_exp2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+__device__ __forceinline__ uint32_t kv4_pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ __half2 kv4_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+__device__ __forceinline__ uint32_t kv4_u(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+// Eight codes of a word -> halves code * s + b in pairs (0, 4), (1, 5), (2, 6), (3, 7).  A code in the low bits of a half whose exponent says
+// 1024 is 1024 + code, four bits further up under an exponent of 64 it is 64 + code: one masking instruction a pair, an exact
+// subtraction and one multiply-add with one rounding.
+__device__ __forceinline__ void kv4_expand(uint32_t w, __half2 s, __half2 b, uint32_t o[4]) {
+    const __half2 k1024 = kv4_h2(0x64006400u), k64 = kv4_h2(0x54005400u);
+    const uint32_t v = w >> 8;
+    o[0] = kv4_u(__hfma2(__hsub2(kv4_h2((w & 0x000f000fu) | 0x64006400u), k1024), s, b));
+    o[1] = kv4_u(__hfma2(__hsub2(kv4_h2((w & 0x00f000f0u) | 0x54005400u), k64), s, b));
+    o[2] = kv4_u(__hfma2(__hsub2(kv4_h2((v & 0x000f000fu) | 0x64006400u), k1024), s, b));
+    o[3] = kv4_u(__hfma2(__hsub2(kv4_h2((v & 0x00f000f0u) | 0x54005400u), k64), s, b));
+}
+
+}  // namespace sl

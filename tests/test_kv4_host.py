@@ -82,6 +82,8 @@ def test_attention_refusals(kw):
 def test_sizes_beyond_the_kernels_are_refused():
     assert call("sl_op_kv4_attention_device", cache(), attention(q_heads=2 * 129)) == CAPACITY
     assert call("sl_op_kv4_attention_device", cache(), attention(table_width=1 << 25, table_stride=1 << 25)) == CAPACITY      # positions past 31 bits
+    assert call("sl_op_kv4_attention_device", cache(), attention(batch=4097)) == CAPACITY
+    assert call("sl_op_kv4_attention_device", cache(), attention(batch=4096, table_width=1 << 17, table_stride=1 << 17)) == CAPACITY      # key blocks
     assert call("sl_op_kv_plan_device", plan(batch=1 << 16, table_width=1 << 16, table_stride=1 << 16)) == CAPACITY
     assert _lib.lib().sl_kv4_attention_workspace(2 * 129, 2, 128, 1, 1, 1) == CAPACITY
     for args in ((7, 2, 128, 1, 1, 1), (8, 0, 128, 1, 1, 1), (8, 2, 96, 1, 1, 1), (8, 2, 128, -1, 1, 1), (8, 2, 128, 1, 0, 1), (8, 2, 128, 1, 1, -1)):
