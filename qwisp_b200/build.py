@@ -7,7 +7,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 SO = os.path.join(HERE, "libseedless_b200.so")
 SOURCES = ["synth.cu", "kernels.cu", "step_persistent.cu", "ep_exchange.cu", "rows_kernels.cu", "gdn_rows.cu", "state_io.cu", "attn_prefill.cu", "sampler.cu", "gemm_tc.cu", "engine.cu",
-           "kv_plan.cu", "kv4_rows.cu", "kv4_attn.cu", "kv4_api.cu"]
+           "kv_plan.cu", "kv4_rows.cu", "kv4_attn.cu", "kv4_prompt.cu", "kv4_api.cu"]
 HEADERS = ["common.cuh", "gemv.cuh", "mixer_math.cuh", "route.cuh", "kernels.h", "kv4.cuh", "kv4_mma.cuh", os.path.join("..", "..", "include", "seedless_b200.h")]
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-lineinfo",

@@ -1,0 +1,391 @@
+// kv4_prompt.cu -- attention of many query rows of a request over the cache held in 4 bits (kv4.cuh), on the 5th-generation tensor cores.
+//
+// A CTA takes NQ tiles of 128 rows (tokens x query heads of one kv head, so that the codes are expanded once for all of a kv head's
+// query heads) and walks the keys 64 at a time.  Warps have roles and meet only at mbarriers:
+//   mma       1 warp: S = Q K^T (queries as the A operand in tensor memory, keys in shared memory) and O += P V (weights in tensor memory
+//             where the scores were, values in shared memory), D + 64 NQ columns of f32 in tensor memory;
+//   expand    4 or 8 warps: a block of 16 keys or half of one each, codes from global memory a tile ahead, to fp16 (one multiply-add a pair), into 128-byte
+//             swizzled tiles: rows of 64 dims, K-major for the scores and, the same bytes, MN-major for the values.  A word expands to its dims
+//             in the order 0 4 1 5 2 6 3 7; the queries are loaded and the outputs stored in that order;
+//   softmax   4 warps a tile, a thread a row: scores in, running maximum and sum in registers, weights out.  The maximum is raised (and the
+//             outputs rescaled) only when a score exceeds it by 2^6; the weights are carried times 2^8, so that fp16 holds them from 2^-32 of the
+//             largest on.
+// NQ = 2 (D 64, 128): while the rows of one tile go through softmax, the tensor cores work for the other.  NQ = 1 (D 256, where the outputs
+// take half of tensor memory): the scores of the next 64 keys are ready before the weights of these are.
+#include "kv4.cuh"
+#include "kv4_mma.cuh"
+
+namespace sl {
+
+constexpr int KP_M = 128, KP_N = 64, KP_ST = 3;
+template <int D> constexpr int kp_nq = D == 256 ? 1 : 2;
+template <int D> constexpr int kp_exp = D == 256 ? 8 : 4;                     // expanding warps: 13 warps in all, 128 registers a thread
+template <int D> constexpr int kp_threads = (1 + kp_exp<D> + 4 * kp_nq<D>) * 32;
+template <int D> constexpr int kp_tile = KP_N * D * 2;                        // bytes of a tile of keys or values
+// (more than half of a multiprocessor's: a second CTA would wait for the first one's tensor memory)
+template <int D> constexpr size_t kp_smem = ((size_t)2 * KP_ST * kp_tile<D> > 120 * 1024 ? (size_t)2 * KP_ST * kp_tile<D> : 120 * 1024) + 1024;
+constexpr int KP_LIMIT = 1 << 22;                                            // polls of a wait (up to 4 us each)
+constexpr float KP_UP = 8.0f, KP_SLACK = 6.0f;
+
+__device__ __forceinline__ uint64_t kp_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {      // version 1, 128-byte swizzle
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// D (tensor memory) (+)= A (tensor memory) B (shared memory)
+__device__ __forceinline__ void kp_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void kp_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void kp_ld32(uint32_t t, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                   "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+                   "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]) : "r"(t) : "memory");
+}
+__device__ __forceinline__ void kp_st32(uint32_t t, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+                 ::"r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+                   "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+                   "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+__device__ __forceinline__ void kp_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void kp_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void kp_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void kp_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void kp_arrive(uint64_t* b) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory"); }
+__device__ __forceinline__ bool kp_elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// Bounded wait of a whole warp.  The first that runs out raises the CTA's abort word, and every later one gives up soon; a role then leaves
+// its loop (nothing in the CTA waits for it unboundedly) and the rows come out as NaN.
+__device__ __forceinline__ bool kp_wait(uint64_t* b, uint32_t parity, volatile int* abort_word) {
+    bool ok = mbar_try_wait(b, parity);
+    for (int i = 0; !ok && i < KP_LIMIT; ++i) {
+        ok = mbar_try_wait(b, parity);
+        if ((i & 255) == 255 && *abort_word) break;
+    }
+    if (!ok) *abort_word = 1;
+    return __all_sync(0xffffffffu, ok);
+}
+
+struct KpSeq { int q0, rows, n, keys; };
+
+template <int D>
+__global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4AttnArgs a, int least, uint32_t q_and, uint32_t q_xor) {
+    constexpr int NQ = kp_nq<D>, TILE = kp_tile<D>, NT = kp_threads<D>, W = NT / 32, SW0 = 4;      // softmax warps start at SW0
+    constexpr uint32_t S0 = NQ * D, Q0 = S0 + 2 * KP_N;                       // columns of tensor memory: outputs, scores, queries
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    __shared__ __align__(8) uint64_t k_full[KP_ST], k_free[KP_ST], v_full[KP_ST], v_free[KP_ST], s_full[2], p_full[2], q_full, o_done;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort, s_b, s_tile, s_sum[W];
+    __shared__ __align__(4) uint8_t s_have[8][4];                             // whether a tile's blocks of 16 keys exist (softmax is up to four tiles behind)
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const int tokens = KP_M / a.G, per_cta = tokens * NQ, head = blockIdx.y;
+    // ---- which request, and which of its tiles: the longest of a request first
+    if (tid == 0) { s_b = -1; s_abort = 0; }
+    __syncthreads();
+    for (int b0 = 0, base = 0; b0 < a.batch; b0 += NT) {
+        const int b = b0 + tid;
+        int x = 0;
+        if (b < a.batch) {
+            const int q0 = a.q_start[b], rows = min(min(a.q_start[b + 1] - q0, a.max_q), a.rows - q0);
+            if (q0 >= 0 && rows > least / a.G) x = (rows + per_cta - 1) / per_cta;
+        }
+        const int own = x;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) { const int u = __shfl_up_sync(0xffffffffu, x, d); if (lane >= d) x += u; }
+        if (lane == 31) s_sum[warp] = x;
+        __syncthreads();
+        int all = 0;
+        x += base;
+        for (int w = 0; w < W; ++w) { if (w < warp) x += s_sum[w]; all += s_sum[w]; }
+        if ((int)blockIdx.x < x && (int)blockIdx.x >= x - own) { s_b = b; s_tile = x - 1 - (int)blockIdx.x; }
+        base += all;
+        __syncthreads();
+        if (s_b >= 0) break;
+    }
+    const int b = s_b;
+    if (b < 0) return;
+    KpSeq sq;
+    sq.q0 = a.q_start[b]; sq.n = a.q_start[b + 1] - sq.q0; sq.rows = min(min(sq.n, a.max_q), a.rows - sq.q0);
+    sq.keys = min(max(a.kv_len[b], 0), a.table_width * c.page_size);
+    const int t0 = s_tile * per_cta;                                          // first token
+    const int nq = NQ == 1 || t0 + tokens >= sq.rows ? 1 : 2;                 // tiles that have rows
+    const int last = min(t0 + per_cta, sq.rows) - 1;
+    const int span = a.causal ? min(sq.keys, max(0, sq.keys - sq.n + last + 1)) : sq.keys;
+    const int tiles = (span + KP_N - 1) / KP_N;
+    if (tid == 0) {
+        for (int i = 0; i < KP_ST; ++i) { mbar_init(&k_full[i], kp_exp<D>); mbar_init(&v_full[i], kp_exp<D>); mbar_init(&k_free[i], 1); mbar_init(&v_free[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
+        mbar_init(&q_full, 4 * nq); mbar_init(&o_done, 1);
+        mbar_fence_init();
+    }
+    if (warp == 0) {
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    kp_before();
+    __syncthreads();
+    kp_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0), smem0 = smem_u32(smem);
+    bool ok = true;
+    if (warp == 0) {
+        // ------------------------------------------------------------ mma
+        if (tiles > 0) {
+            constexpr uint32_t ID_S = (1u << 4) | ((uint32_t)(KP_N >> 3) << 17) | ((uint32_t)(KP_M >> 4) << 24);                  // f32 += f16 x f16, K-major B
+            constexpr uint32_t ID_O = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(KP_M >> 4) << 24);       // MN-major B
+            const uint64_t dk = kp_desc(smem0, 16, 1024), dv = kp_desc(smem0 + KP_ST * TILE, KP_N * 128, 1024);
+            auto scores = [&](int q, int j) {                                 // S of tile q, keys 64 j ..
+                const int st = j % KP_ST, slot = NQ == 2 ? q : j & 1;
+                if (kp_elect()) {
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i)
+                        kp_mma(tmem + S0 + slot * KP_N, tmem + Q0 + q * (D / 2) + i * 8, dk + (uint32_t)(st * (TILE >> 4) + (i >> 2) * (KP_N * 128 >> 4) + (i & 3) * 2), ID_S, i > 0);
+                    kp_commit(&s_full[slot]);
+                    if (q == nq - 1) kp_commit(&k_free[st]);
+                }
+                __syncwarp();
+            };
+            ok = kp_wait(&q_full, 0, &s_abort) && kp_wait(&k_full[0], 0, &s_abort);
+            kp_after();
+            if (ok) for (int q = 0; q < nq; ++q) scores(q, 0);
+            for (int j = 0; j < tiles && ok; ++j) {
+                const bool more = j + 1 < tiles;
+                if (more) ok = kp_wait(&k_full[(j + 1) % KP_ST], (uint32_t)((j + 1) / KP_ST & 1), &s_abort) && ok;
+                kp_after();
+                if (NQ == 1 && more && ok) scores(0, j + 1);
+                ok = ok && kp_wait(&v_full[j % KP_ST], (uint32_t)(j / KP_ST & 1), &s_abort);
+                for (int q = 0; q < nq && ok; ++q) {
+                    const int slot = NQ == 2 ? q : j & 1;
+                    ok = kp_wait(&p_full[slot], (uint32_t)((NQ == 2 ? j : j >> 1) & 1), &s_abort);
+                    if (!ok) break;
+                    kp_after();
+                    if (kp_elect()) {
+#pragma unroll
+                        for (int i = 0; i < KP_N / 16; ++i)
+                            kp_mma(tmem + q * D, tmem + S0 + slot * KP_N + i * 8, dv + (uint32_t)((j % KP_ST) * (TILE >> 4) + i * (2048 >> 4)), ID_O, j > 0 || i > 0);
+                        if (q == nq - 1) { kp_commit(&v_free[j % KP_ST]); if (NQ == 1 || !more) kp_commit(&o_done); }
+                    }
+                    __syncwarp();
+                    if (NQ == 2 && more) scores(q, j + 1);
+                }
+            }
+        }
+    } else if (warp < SW0 || warp >= SW0 + 4 * NQ) {
+        // ------------------------------------------------------------ expand: keys PER e .. of every tile
+        constexpr int PER = KP_N / kp_exp<D>, LPC = 32 / PER, LD = (D / 32) * PER / 32;      // keys of a warp; 16-byte pieces a lane
+        static_assert(LD * 32 == (D / 32) * PER && PER * LPC == 32, "");
+        const int e = warp < SW0 ? warp - 1 : warp - (SW0 + 4 * NQ) + SW0 - 1, key = (lane & 7) + (PER == 16 ? lane & 8 : 0), ch0 = PER == 16 ? lane >> 4 : lane >> 3;
+        const int page_blocks = c.page_size / KV4_B, at = PER == 16 ? key : (e & 1) * 8 + key;            // position in its block of 16
+        const int* table = a.table + (int64_t)b * a.table_stride;
+        struct Raw { uint4 code[2][LD]; __half s[2][LD], b[2][LD]; bool have; };
+        auto fetch = [&](int j, Raw& r) {
+            const int blk = j * 4 + e * PER / KV4_B, pg = blk / page_blocks;
+            int page = -1;
+            if (j < tiles && blk * KV4_B < sq.keys) page = table[pg];
+            r.have = page >= 0 && page < c.pages;
+            const unsigned char* p = r.have ? kv4_block(c, page, head, blk - pg * page_blocks) : nullptr;
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+                for (int i = 0; i < LD; ++i) {
+                    r.code[v][i] = make_uint4(0, 0, 0, 0); r.s[v][i] = __ushort_as_half(0); r.b[v][i] = __ushort_as_half(0);
+                    const int ch = ch0 + LPC * i;
+                    if (p && blk * KV4_B + at < sq.keys) {                    // (what lies behind the keys stays zero)
+                        r.code[v][i] = *reinterpret_cast<const uint4*>(p + v * 8 * D + kv4_swz((uint32_t)(at * (D / 2) + ch * 16)));
+                        const __half* sb = reinterpret_cast<const __half*>(p + (16 + v) * D) + (ch >> 1) * 32 + at;
+                        r.s[v][i] = sb[0]; r.b[v][i] = sb[16];
+                    }
+                }
+        };
+        auto store = [&](const Raw& r, int v, uint32_t tile) {                // row of 64 dims: 128 bytes, its 16-byte pieces XORed with the key
+#pragma unroll
+            for (int i = 0; i < LD; ++i) {
+                const int ch = ch0 + LPC * i;
+                const __half2 s = __half2half2(r.s[v][i]), bi = __half2half2(r.b[v][i]);
+                const uint32_t row = tile + (uint32_t)((ch >> 1) * (KP_N * 128) + (e * PER + key) * 128);
+                const uint32_t w[4] = {r.code[v][i].x, r.code[v][i].y, r.code[v][i].z, r.code[v][i].w};
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    uint32_t o[4];
+                    kv4_expand(w[x], s, bi, o);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (((((ch & 1) << 2) + x) ^ (key & 7)) << 4)), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+                }
+            }
+        };
+        auto publish = [&](uint64_t* bar) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) kp_arrive(bar);
+        };
+        Raw next;
+        fetch(0, next);
+        for (int j = 0; j < tiles && ok; ++j) {
+            const Raw now = next;
+            fetch(j + 1, next);
+            const int st = j % KP_ST;
+            const uint32_t ph = (uint32_t)(j / KP_ST & 1) ^ 1u;               // (a fresh barrier passes at 1)
+            ok = kp_wait(&k_free[st], ph, &s_abort);
+            if (!ok) break;
+            store(now, 0, smem0 + st * TILE);
+            if (e * PER % KV4_B == 0 && lane == 0) s_have[j & 7][e * PER / KV4_B] = now.have;      // (read by softmax behind the scores, which wait for this)
+            publish(&k_full[st]);
+            ok = kp_wait(&v_free[st], ph, &s_abort);
+            if (!ok) break;
+            store(now, 1, smem0 + (KP_ST + st) * TILE);
+            publish(&v_full[st]);
+        }
+    } else {
+        // ------------------------------------------------------------ softmax: a thread a row
+        const int q = (warp - SW0) >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        if (q < nq) {
+            const int tok = t0 + q * tokens + row / a.G, h = head * a.G + row % a.G;
+            const bool live = row < tokens * a.G && tok < sq.rows;
+            if (tiles > 0) {
+                const __half* src = a.q + (int64_t)(sq.q0 + tok) * a.q_row + (int64_t)h * a.q_head;
+#pragma unroll
+                for (int c0 = 0; c0 < D / 2; c0 += 32) {
+                    uint32_t r[32];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        uint4 v = make_uint4(0, 0, 0, 0);
+                        if (live) v = *reinterpret_cast<const uint4*>(src + c0 * 2 + i * 8);
+                        r[4 * i] = (__byte_perm(v.x, v.z, 0x5410) & q_and) ^ q_xor; r[4 * i + 1] = (__byte_perm(v.x, v.z, 0x7632) & q_and) ^ q_xor;
+                        r[4 * i + 2] = (__byte_perm(v.y, v.w, 0x5410) & q_and) ^ q_xor; r[4 * i + 3] = (__byte_perm(v.y, v.w, 0x7632) & q_and) ^ q_xor;
+                    }
+                    __syncwarp();
+                    kp_st32(tmem + lanes + Q0 + q * (D / 2) + c0, r);
+                }
+                kp_wait_st();
+                kp_before();
+                __syncwarp();
+                if (lane == 0) kp_arrive(&q_full);
+            }
+            const int sees = !live ? 0 : a.causal ? sq.keys - sq.n + tok + 1 : sq.keys;
+            // keys that all of the tile's rows see
+            const int all = a.causal ? min(sq.keys, sq.keys - sq.n + t0 + q * tokens + 1) : sq.keys;
+            float m = -INFINITY, l = 0.f;
+            for (int j = 0; j < tiles && ok; ++j) {
+                const int slot = NQ == 2 ? q : j & 1, k0 = j * KP_N;
+                ok = kp_wait(&s_full[slot], (uint32_t)((NQ == 2 ? j : j >> 1) & 1), &s_abort);
+                if (!ok) break;
+                kp_after();
+                const uint32_t have = *reinterpret_cast<const uint32_t*>(s_have[j & 7]);
+                uint32_t r[64];
+                kp_ld32(tmem + lanes + S0 + slot * KP_N, r);
+                kp_ld32(tmem + lanes + S0 + slot * KP_N + 32, r + 32);
+                kp_wait_ld();
+                float* s = reinterpret_cast<float*>(r);
+                if (k0 + KP_N > all || have != 0x01010101u) {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) if (k0 + i >= sees || !(have >> (i >> 4) * 8 & 1)) s[i] = -INFINITY;
+                }
+                float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int i = 4; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale;
+                if (__any_sync(0xffffffffu, top > m + KP_SLACK)) {
+                    const float nm = fmaxf(m, top), f = nm == -INFINITY ? 1.f : kv4_exp2(m - nm);
+                    m = nm; l *= f;
+                    if (j > 0) {                                              // the outputs so far
+                        if (NQ == 1) ok = kp_wait(&o_done, (uint32_t)(j - 1) & 1, &s_abort);      // (NQ 2: they were done before these scores)
+                        if (!ok) break;
+                        kp_after();
+#pragma unroll 1
+                        for (int c0 = 0; c0 < D; c0 += 32) {
+                            uint32_t o[32];
+                            kp_ld32(tmem + lanes + q * D + c0, o);
+                            kp_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            kp_st32(tmem + lanes + q * D + c0, o);
+                        }
+                    }
+                }
+                const float base = KP_UP - (m == -INFINITY ? 0.f : m);
+                float sum[2] = {0.f, 0.f};
+                uint32_t p[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float x = kv4_exp2(fmaf(s[2 * i], a.scale, base)), y = kv4_exp2(fmaf(s[2 * i + 1], a.scale, base));
+                    sum[0] += x; sum[1] += y;
+                    p[i] = kv4_pack(x, y);
+                }
+                l += sum[0] + sum[1];
+                kp_st32(tmem + lanes + S0 + slot * KP_N, p);
+                kp_wait_st();
+                kp_before();
+                __syncwarp();
+                if (lane == 0) kp_arrive(&p_full[slot]);
+            }
+            // ---- normalise, gate, round once; eight columns are the dims 0 4 1 5 2 6 3 7 of a word
+            if (tiles > 0 && ok) ok = kp_wait(&o_done, NQ == 1 ? (uint32_t)(tiles - 1) & 1 : 0u, &s_abort);
+            kp_after();
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            __half* dst = a.out + (int64_t)(sq.q0 + tok) * a.o_row + (int64_t)h * a.o_head;
+            const __half* gate = a.gate ? a.gate + (int64_t)(sq.q0 + tok) * a.g_row + (int64_t)h * a.g_head : nullptr;
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += 32) {
+                uint32_t o[32];
+                __syncwarp();
+                if (tiles > 0) { kp_ld32(tmem + lanes + q * D + c0, o); kp_wait_ld(); }
+                if (!live) continue;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float x[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) x[(k & 1) * 4 + (k >> 1)] = !ok ? __int_as_float(0x7fffffff) : l == 0.f ? 0.f : __uint_as_float(o[8 * i + k]) * inv;
+                    if (gate) {
+                        const uint4 g = *reinterpret_cast<const uint4*>(gate + c0 + 8 * i);
+                        const __half* gh = reinterpret_cast<const __half*>(&g);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) x[k] *= sigmoid_f(h2f(gh[k]));
+                    }
+                    *reinterpret_cast<uint4*>(dst + c0 + 8 * i) = make_uint4(kv4_pack(x[0], x[1]), kv4_pack(x[2], x[3]), kv4_pack(x[4], x[5]), kv4_pack(x[6], x[7]));
+                }
+            }
+        }
+    }
+    if (!ok) {                                 // MMAs of this CTA may still be running: outlast them before tensor memory is given back
+        const long long c0 = clock64();
+        while (clock64() - c0 < 200000ll) { }
+    }
+    kp_before();
+    __syncthreads();
+    __syncwarp();
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+template <int D>
+static int launch_prompt_t(const Kv4Cache& c, Kv4AttnArgs a, int least, cudaStream_t st) {
+    // a scale below zero, or zero, goes into the queries: the maximum of the scores is that of the scaled ones then
+    const uint32_t q_and = a.scale == 0.f ? 0u : 0xffffffffu, q_xor = a.scale < 0.f ? 0x80008000u : 0u;
+    a.scale = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
+    static std::atomic<unsigned long long> configured{0};                     // devices
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 64 || !(configured.load(std::memory_order_relaxed) >> dev & 1)) {
+        cudaError_t err = cudaFuncSetAttribute(k_kv4_prompt<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kp_smem<D>);
+        if (err != cudaSuccess) return (int)err;
+        if (dev < 64) configured.fetch_or(1ull << dev);
+    }
+    const int per_cta = KP_M / a.G * kp_nq<D>;
+    const long long most = (long long)a.rows / per_cta + a.batch;             // (a request's last tile may be short)
+    int rc = 0;
+    profile_launch("k_kv4_prompt", st, [&] { return rc = launch_pdl(false, k_kv4_prompt<D>, dim3((unsigned)most, (unsigned)c.KV), kp_threads<D>, kp_smem<D>, st, c, a, least, q_and, q_xor); });
+    return rc;
+}
+int launch_kv4_prompt(const Kv4Cache& c, const Kv4AttnArgs& a, int least, cudaStream_t st) {
+    return c.D == 64 ? launch_prompt_t<64>(c, a, least, st) : c.D == 128 ? launch_prompt_t<128>(c, a, least, st) : launch_prompt_t<256>(c, a, least, st);
+}
+
+}  // namespace sl
