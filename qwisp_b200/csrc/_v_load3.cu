@@ -1,0 +1,428 @@
+// kv4_attn.cu -- attention of a ragged batch of query rows over the cache held in 4 bits (kv4.cuh):
+//   out = softmax(scale * q K^T) V, optionally times sigmoid(gate), K and V the fp16 values that the codes stand for.
+// Request b's rows are q_start[b] .. q_start[b + 1] - 1, its keys positions 0 .. kv_len[b] - 1; causal: its row i of n sees
+// kv_len - n + i + 1 keys.  A row that sees none is zero.  A page that the cache does not have holds no keys.
+//
+// Requests of up to 16 rows a kv head (tokens x query heads of the head) take k_kv4_decode, the others k_kv4_prompt.
+#include "kv4.cuh"
+#include "kv4_mma.cuh"
+
+namespace sl {
+
+// ================================================================================ few rows a request
+// The work is the requests' key blocks: request b has ceil(keys / 16) units for each of its kv heads, and every CTA takes an equal
+// run of them, whatever the lengths are: a run may hold the end of one (request, head), several whole ones and the start of another.
+// Whole ones are finished by their CTA, the others leave partial sums that k_kv4_join adds up.
+// A CTA's four warps take the blocks of a run in turn, each through a ring of its own that cp.async fills (a warp waits for nobody
+// inside an item).  Per block: S^T = K Q^T and O^T += V^T P^T on m16n8k16 with 16 keys (16 dims) as M and up to eight rows as N, so that
+// decode rows fill the tensor cores' narrow side.  ldmatrix brings a lane words of eight dims of a key for K and, transposed, words of
+// four dims of two neighbouring keys for V; both expand to operand registers as they are, and the order of dims inside a step is
+// the queries' (the outputs') to follow.  The running maximum is raised only when a score exceeds it by 2^6; the weights are
+// carried times 2^8, so that fp16 holds them from 2^-32 of the largest on.
+constexpr int KD_WARPS = 4, KD_MAX_BATCH = 4096;
+template <int D> constexpr int kd_stages = D == 256 ? 3 : D == 128 ? 5 : 6;
+template <int D, int NT> constexpr int kd_ctas = D == 256 ? 2 : NT == 1 ? 4 : 3;                          // CTAs of a multiprocessor
+template <int D> constexpr size_t kd_ring = (size_t)KD_WARPS * kd_stages<D> * kv4_block_bytes(D);
+template <int D> constexpr size_t kd_smem(int batch) { return kd_ring<D> + (size_t)(batch + 1) * 4; }
+constexpr float KD_UP = 8.0f, KD_SLACK = 6.0f;
+
+// rows of request b (0: none, or more than `most` rows a kv head), and the units of one of its kv heads
+struct KdSeq { int q0, rows, keys, units; };
+__device__ __forceinline__ KdSeq kd_seq(const Kv4Cache& c, const Kv4AttnArgs& a, int b, int most) {
+    KdSeq s;
+    s.q0 = a.q_start[b];
+    const int n = a.q_start[b + 1] - s.q0;
+    s.rows = min(min(n, a.max_q), a.rows - s.q0);
+    s.keys = min(max(a.kv_len[b], 0), a.table_width * c.page_size);
+    if (s.q0 < 0 || s.rows <= 0 || s.rows > most / a.G) { s.rows = 0; s.units = 0; return s; }
+    const int sees = a.causal ? min(s.keys, max(0, s.keys - n + s.rows)) : s.keys;                        // (rows behind max_q see more)
+    s.units = max(1, (sees + KV4_B - 1) / KV4_B);
+    return s;
+}
+// exclusive sums of all requests' units in pre[0 .. batch]; by all threads (128)
+__device__ __forceinline__ void kd_prefix(const Kv4Cache& c, const Kv4AttnArgs& a, int most, int* pre, int* ws) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int base = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += KD_WARPS * 32) {
+        const int b = b0 + tid;
+        int x = b < a.batch ? kd_seq(c, a, b, most).units * c.KV : 0;
+        const int own = x;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) { const int u = __shfl_up_sync(0xffffffffu, x, d); if (lane >= d) x += u; }
+        if (lane == 31) ws[warp] = x;
+        __syncthreads();
+        int before = base, all = 0;
+#pragma unroll
+        for (int w = 0; w < KD_WARPS; ++w) { if (w < warp) before += ws[w]; all += ws[w]; }
+        if (b < a.batch) pre[b] = before + x - own;
+        base += all;
+        __syncthreads();
+    }
+    if (tid == 0) pre[a.batch] = base;
+    __syncthreads();
+}
+__device__ __forceinline__ int kd_find(const int* pre, int n, int u) {        // the last b with pre[b] <= u
+    int lo = 0, hi = n - 1;
+    while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (pre[mid] <= u) lo = mid; else hi = mid - 1; }
+    return lo;
+}
+__device__ __forceinline__ int kd_run(int total, int ctas, int least) {       // units of a CTA
+    const int per = max(least, (total + ctas - 1) / ctas);
+    return (per + KD_WARPS - 1) / KD_WARPS * KD_WARPS;
+}
+// a finished row's four dims, gated and rounded once
+__device__ __forceinline__ void kd_finish(const Kv4AttnArgs& a, int row, int h, int d, float4 o, float l) {
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
+    if (a.gate) {
+        const uint2 g = *reinterpret_cast<const uint2*>(a.gate + row * a.g_row + h * a.g_head + d);
+        const float2 g0 = __half22float2(*reinterpret_cast<const __half2*>(&g.x)), g1 = __half22float2(*reinterpret_cast<const __half2*>(&g.y));
+        o.x *= sigmoid_f(g0.x); o.y *= sigmoid_f(g0.y); o.z *= sigmoid_f(g1.x); o.w *= sigmoid_f(g1.y);
+    }
+    const __half2 r0 = __floats2half2_rn(o.x, o.y), r1 = __floats2half2_rn(o.z, o.w);
+    uint2 r; r.x = *reinterpret_cast<const uint32_t*>(&r0); r.y = *reinterpret_cast<const uint32_t*>(&r1);
+    *reinterpret_cast<uint2*>(a.out + row * a.o_row + h * a.o_head + d) = r;
+}
+// Partial sums of a CTA: two places (the item that began before its run, the one that goes on behind it), each [R][D] sums and [R] (max, norm).
+template <int D, int R> __device__ __forceinline__ float* kd_part(const Kv4AttnArgs& a, int cta, int place) {
+    return (float*)a.ws + ((size_t)cta * 2 + place) * R * (D + 2);
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv4Cache c, Kv4AttnArgs a, int most, int least) {
+    constexpr int R = 8 * NT, S = kd_stages<D>, CH = D / 32, BB = kv4_block_bytes(D), PIECES = BB / 16;
+    extern __shared__ __align__(128) unsigned char smem[];
+    float* s_o = reinterpret_cast<float*>(smem);                            // [warps][8 rows][D + 4], where the rings were
+    int* s_pre = reinterpret_cast<int*>(smem + kd_ring<D>);
+    static_assert(kd_ring<D> >= (size_t)KD_WARPS * 8 * (D + 4) * 4, "");
+    __shared__ float s_m[KD_WARPS][R], s_l[KD_WARPS][R];
+    __shared__ int s_ws[KD_WARPS];
+    constexpr bool QR = false;
+    __shared__ uint4 s_q[QR ? 1 : NT * CH][32];
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
+    pdl_launch_dependents();
+    kd_prefix(c, a, most, s_pre, s_ws);
+    const int total = s_pre[a.batch], per = kd_run(total, gridDim.x, least);
+    int u = min((long long)blockIdx.x * per, (long long)total);
+    const int u1 = min(u + per, total);
+    if (u >= u1) return;
+    unsigned char* ring = smem + warp * S * BB;
+    const uint32_t ring_u = smem_u32(ring);
+    // ldmatrix: lanes 0-7 the rows of keys 0-7, 8-15 of keys 8-15, 16-31 the same of the next piece
+    uint32_t lm[CH / 2];
+#pragma unroll
+    for (int i = 0; i < CH / 2; ++i) lm[i] = kv4_swz((uint32_t)((lane & 15) * (D / 2) + (2 * i + (lane >> 4)) * 16));
+    const int page_blocks = c.page_size / KV4_B;
+    int b = kd_find(s_pre, a.batch, u);
+    KdSeq sq = kd_seq(c, a, b, most);
+    while (u < u1) {
+        const int rel = u - s_pre[b], head = rel / sq.units, j0 = rel % sq.units, j1 = min(sq.units, j0 + (u1 - u));
+        const bool whole = j0 == 0 && j1 == sq.units;
+        const int n = a.q_start[b + 1] - sq.q0, live = sq.rows * a.G;        // rows of the tile that exist
+        // ---- queries: B operands, row g of each N tile; dims 32 i + 8 t .. of piece i in the order that the codes expand in.  Of one tile
+        // in registers; of two in shared memory, the warps' alike (128 more registers are the outputs')
+        uint4 q[QR ? CH : 1];
+#pragma unroll
+        for (int x = QR ? 0 : warp; x < NT * CH; x += QR ? 1 : KD_WARPS) {
+            const int nt = x / CH, ch = x % CH, r = nt * 8 + g, i = r / a.G;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < live) v = *reinterpret_cast<const uint4*>(a.q + (int64_t)(sq.q0 + i) * a.q_row + (int64_t)(head * a.G + r % a.G) * a.q_head + 8 * t + 32 * ch);
+            v = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+            if (QR) q[ch] = v; else s_q[x][lane] = v;
+        }
+        if (!QR) __syncthreads();
+        // keys that the lane's columns (rows 2 t, 2 t + 1 of each tile) see, and what all rows see
+        int sees[NT][2], all = sq.keys;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) sees[nt][e] = a.causal ? sq.keys - n + (nt * 8 + 2 * t + e) / a.G + 1 : sq.keys;
+        if (a.causal) all = min(all, sq.keys - n + 1);
+        float o[NT][CH][2][4], base[NT][2], l[NT][2];                        // base: KD_UP - the maximum
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[nt][ch][i >> 2][i & 3] = 0.f;
+            base[nt][0] = base[nt][1] = INFINITY; l[nt][0] = l[nt][1] = 0.f;
+        }
+        // ---- the warp's blocks j0 + warp, + 4, ..: 32 of them looked up at a time, a lane each
+        const int mine = max(0, (j1 - j0 - warp + KD_WARPS - 1) / KD_WARPS);
+        const int* table = a.table + (int64_t)b * a.table_stride;
+        unsigned long long addr = 0;
+        unsigned absent = 0;                                                  // stages whose page is none
+        auto issue = [&](int it) {
+            if (it < mine) {
+                if ((it & 31) == 0) {
+                    const int k = it + lane;
+                    addr = 0;
+                    if (k < mine) {
+                        const int j = j0 + warp + k * KD_WARPS, page = table[j / page_blocks];
+                        if (page >= 0 && page < c.pages) addr = (unsigned long long)kv4_block(c, page, head, j % page_blocks);
+                    }
+                }
+                const unsigned char* src = (const unsigned char*)__shfl_sync(0xffffffffu, addr, it & 31);
+                const int st = it % S;
+                absent &= ~(1u << st);
+                if (src) {
+#pragma unroll
+                    for (int i = 0; i < (PIECES + 31) / 32; ++i)
+                        if (i < PIECES / 32 || lane < PIECES % 32) kv4_cp16(ring_u + st * BB + (lane + 32 * i) * 16, src + (lane + 32 * i) * 16);
+                } else absent |= 1u << st;
+            }
+            kv4_commit();
+        };
+#pragma unroll
+        for (int it = 0; it < S - 1; ++it) issue(it);
+        for (int it = 0; it < mine; ++it) {
+            kv4_wait<S - 2>();
+            __syncwarp();
+            issue(it + S - 1);                                                // (into the stage that the block before has left)
+            const int st = it % S, key0 = (j0 + warp + it * KD_WARPS) * KV4_B;
+            if (absent >> st & 1) continue; if (a.scale > -1e30f) { l[0][0] += *(volatile float*)(ring + st * BB + lane * 4); continue; }
+            const uint32_t blk = ring_u + st * BB;
+            // ---- S^T: 16 keys x 8 rows
+            float s[NT][4], s2[NT][4];                                        // (two chains of products)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < CH / 2; ++i) {                                // a 64-dim group: two pieces
+                uint32_t w[4], sb[4];
+                kv4_ldsm(w, blk + lm[i]);
+                kv4_ldsm_t(sb, blk + 16 * D + i * 64 + (lane >> 3) * 16);     // (eight equal rows, transposed: scales of keys g, g + 8, biases, each twice)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t x[4], y[4];
+                    kv4_expand(w[2 * e], kv4_h2(sb[0]), kv4_h2(sb[2]), x); kv4_expand(w[2 * e + 1], kv4_h2(sb[1]), kv4_h2(sb[3]), y);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const uint4 qf = QR ? q[QR ? 2 * i + e : 0] : s_q[nt * CH + 2 * i + e][lane];
+                        kv4_mma(s[nt], x[0], y[0], x[1], y[1], qf.x, qf.y);
+                        kv4_mma(s2[nt], x[2], y[2], x[3], y[3], qf.z, qf.w);
+                    }
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[nt][e] += s2[nt][e];
+            const bool edge = key0 + KV4_B > all;
+            float p[NT][4], high = -INFINITY;
+            auto weigh = [&] {                                                // exponents of the weights; above KD_UP + KD_SLACK: the maximum has to be raised
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[nt][e] = fmaf(s[nt][e], a.scale, base[nt][e & 1]);      // (scale: times log2 e, by the host)
+                if (edge) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) if (key0 + g + 8 * (e >> 1) >= sees[nt][e & 1]) p[nt][e] = -INFINITY;
+                }
+            };
+            weigh();
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) high = fmaxf(high, fmaxf(fmaxf(p[nt][0], p[nt][1]), fmaxf(p[nt][2], p[nt][3])));
+            if (__any_sync(0xffffffffu, high > KD_UP + KD_SLACK)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float x = -INFINITY;
+                        if (!edge || key0 + g < sees[nt][e]) x = s[nt][e] * a.scale;
+                        if (!edge || key0 + g + 8 < sees[nt][e]) x = fmaxf(x, s[nt][e + 2] * a.scale);
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4)); x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8)); x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                        const float old = KD_UP - base[nt][e], top = fmaxf(x, old), f = top == -INFINITY ? 1.f : kv4_exp2(old - top);
+                        base[nt][e] = KD_UP - top; l[nt][e] *= f;
+#pragma unroll
+                        for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) { o[nt][ch][k][e] *= f; o[nt][ch][k][e + 2] *= f; }
+                    }
+                weigh();
+            }
+            uint32_t pb[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { p[nt][e] = kv4_exp2(p[nt][e]); l[nt][e & 1] += p[nt][e]; }
+                pb[nt][0] = kv4_transpose(kv4_pack(p[nt][0], p[nt][1])); pb[nt][1] = kv4_transpose(kv4_pack(p[nt][2], p[nt][3]));
+            }
+            // ---- O^T: dims x 8 rows; a lane's registers: dims 32 ch + 4 g + (0 .. 3) of rows 2 t, 2 t + 1
+#pragma unroll
+            for (int i = 0; i < CH / 2; ++i) {
+                uint32_t w[4], sv[4];
+                kv4_ldsm_t(w, blk + 8 * D + lm[i]);
+                kv4_ldsm(sv, blk + 17 * D + i * 64 + (lane >> 3) * 16);       // (scales of keys 2 t, 2 t + 1; of 2 t + 8, + 9; biases)
+                if (key0 + KV4_B > sq.keys) {                                 // positions that nobody has: their weights are 0, their scales anything
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int k = key0 + 2 * t + 8 * (e & 1);
+                        if (k >= sq.keys) sv[e] = 0; else if (k + 1 >= sq.keys) sv[e] &= 0xffffu;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t x[4], y[4];
+                    kv4_expand(w[2 * e], kv4_h2(sv[0]), kv4_h2(sv[2]), x); kv4_expand(w[2 * e + 1], kv4_h2(sv[1]), kv4_h2(sv[3]), y);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        kv4_mma(o[nt][2 * i + e][0], x[0], x[1], y[0], y[1], pb[nt][0], pb[nt][1]);
+                        kv4_mma(o[nt][2 * i + e][1], x[2], x[3], y[2], y[3], pb[nt][0], pb[nt][1]);
+                    }
+                }
+            }
+        }
+        kv4_wait<0>();
+        // ---- the warps' sums together
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 4); l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 8); l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
+                if (g == 0) { s_m[warp][nt * 8 + 2 * t + e] = KD_UP - base[nt][e]; s_l[warp][nt * 8 + 2 * t + e] = l[nt][e]; }
+            }
+        float* part = kd_part<D, R>(a, blockIdx.x, j0 > 0 ? 0 : 1);
+        __syncthreads();                                                      // (the rings are done with)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    *reinterpret_cast<float4*>(s_o + (warp * 8 + 2 * t + e) * (D + 4) + 32 * ch + 4 * g) =
+                        make_float4(o[nt][ch][0][e], o[nt][ch][0][e + 2], o[nt][ch][1][e], o[nt][ch][1][e + 2]);
+            __syncthreads();
+            for (int x = tid; x < 8 * D / 4; x += KD_WARPS * 32) {
+                const int r = x / (D / 4), d = x % (D / 4) * 4, rr = nt * 8 + r;
+                if (rr >= live) continue;
+                float top = -INFINITY, sum = 0.f;
+#pragma unroll
+                for (int w = 0; w < KD_WARPS; ++w) top = fmaxf(top, s_m[w][rr]);
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < KD_WARPS; ++w) {
+                    const float f = s_m[w][rr] == -INFINITY ? 0.f : kv4_exp2(s_m[w][rr] - top);
+                    const float4 y = *reinterpret_cast<const float4*>(s_o + (w * 8 + r) * (D + 4) + d);
+                    sum = fmaf(s_l[w][rr], f, sum);
+                    v.x = fmaf(y.x, f, v.x); v.y = fmaf(y.y, f, v.y); v.z = fmaf(y.z, f, v.z); v.w = fmaf(y.w, f, v.w);
+                }
+                if (whole) kd_finish(a, sq.q0 + rr / a.G, head * a.G + rr % a.G, d, v, sum);
+                else {
+                    *reinterpret_cast<float4*>(part + (size_t)rr * D + d) = v;
+                    if (d == 0) *reinterpret_cast<float2*>(part + (size_t)R * D + 2 * rr) = make_float2(top, sum);
+                }
+            }
+            __syncthreads();
+        }
+        u += j1 - j0;
+        if (u < u1 && u >= s_pre[b + 1]) { b = kd_find(s_pre, a.batch, u); sq = kd_seq(c, a, b, most); }
+    }
+}
+// grid (rows, kv heads, requests): adds up the partial sums of a row whose (request, kv head) more than one CTA had.  A warp takes every
+// fourth of them, eight in flight, behind one look at all their maxima.
+template <int D, int NT>
+__global__ void __launch_bounds__(KD_WARPS * 32) k_kv4_join(Kv4Cache c, Kv4AttnArgs a, int most, int least, int ctas) {
+    constexpr int R = 8 * NT, V = D / 32;
+    extern __shared__ int s_pre[];
+    __shared__ int s_ws[KD_WARPS];
+    __shared__ __align__(16) float s_o[KD_WARPS][D];
+    const int r = blockIdx.x, head = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    kd_prefix(c, a, most, s_pre, s_ws);
+    const KdSeq sq = kd_seq(c, a, b, most);
+    pdl_wait();                              // (every CTA: what follows this kernel in the stream also follows the one before)
+    if (r >= sq.rows * a.G) return;
+    const int per = kd_run(s_pre[a.batch], ctas, least), u0 = s_pre[b] + head * sq.units, c0 = u0 / per, n = (u0 + sq.units - 1) / per - c0 + 1;
+    if (n == 1) return;
+    // piece i: the first CTA's item goes on behind its run, the others' began before theirs
+    auto part = [&](int i) { return kd_part<D, R>(a, c0 + i, i > 0 ? 0 : 1); };
+    auto ml_of = [&](int i) { return i < n ? *reinterpret_cast<const float2*>(part(i) + (size_t)R * D + 2 * r) : make_float2(-INFINITY, 0.f); };
+    float2 ml = ml_of(lane);
+    float top = ml.x;
+    for (int i = 32; i < n; i += 32) top = fmaxf(top, ml_of(i + lane).x);
+    top = warp_max(top);
+    float v[V] = {}, sum = 0.f;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        if (i0) ml = ml_of(i0 + lane);
+        const float f = ml.x == -INFINITY ? 0.f : kv4_exp2(ml.x - top);
+        sum = fmaf(ml.y, f, sum);
+        {
+            float y[8][V];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int i = warp + 4 * k;
+                const float* src = part(i0 + i) + (size_t)r * D + lane * V;
+#pragma unroll
+                for (int x = 0; x < V; x += 2) {
+                    float2 t = make_float2(0.f, 0.f);
+                    if (i0 + i < n) t = *reinterpret_cast<const float2*>(src + x);
+                    y[k][x] = t.x; y[k][x + 1] = t.y;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float fk = __shfl_sync(0xffffffffu, f, warp + 4 * k);
+#pragma unroll
+                for (int x = 0; x < V; ++x) v[x] = fmaf(y[k][x], fk, v[x]);
+            }
+        }
+    }
+    sum = warp_sum(sum);
+#pragma unroll
+    for (int x = 0; x < V; ++x) s_o[warp][lane * V + x] = v[x];
+    __syncthreads();
+    const int d = threadIdx.x * 4;
+    if (d >= D) return;
+    float4 o = *reinterpret_cast<const float4*>(&s_o[0][d]);
+#pragma unroll
+    for (int w = 1; w < KD_WARPS; ++w) {
+        const float4 y = *reinterpret_cast<const float4*>(&s_o[w][d]);
+        o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
+    }
+    kd_finish(a, sq.q0 + r / a.G, head * a.G + r % a.G, d, o, sum);
+}
+constexpr int KD_LEAST = 8;              // units a CTA takes at least
+template <int D, int NT>
+static int launch_decode(const Kv4Cache& c, Kv4AttnArgs a, int most, cudaStream_t st) {
+    a.scale *= 1.4426950408889634f;
+    const int ctas = sm_count() * kd_ctas<D, NT>;
+    const size_t smem = kd_smem<D>(a.batch);
+    static std::atomic<unsigned long long> configured{0};                     // devices
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 64 || !(configured.load(std::memory_order_relaxed) >> dev & 1)) {
+        cudaError_t err = cudaFuncSetAttribute(k_kv4_decode<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kd_smem<D>(KD_MAX_BATCH));
+        if (err != cudaSuccess) return (int)err;
+        if (dev < 64) configured.fetch_or(1ull << dev);
+    }
+    int rc = 0;
+    profile_launch("k_kv4_decode", st, [&] { return rc = launch_pdl(false, k_kv4_decode<D, NT>, dim3((unsigned)ctas), KD_WARPS * 32, smem, st, c, a, most, KD_LEAST); });
+    if (rc) return rc;
+    profile_launch("k_kv4_join", st, [&] { return rc = launch_pdl(true, k_kv4_join<D, NT>, dim3((unsigned)(a.G * (a.max_q < most / a.G ? a.max_q : most / a.G)), (unsigned)c.KV, (unsigned)a.batch), KD_WARPS * 32, (size_t)(a.batch + 1) * 4, st, c, a, most, KD_LEAST, ctas); });
+    return rc;
+}
+
+template <int D>
+static size_t decode_workspace(int rows) { return rows > 8 ? (size_t)sm_count() * kd_ctas<D, 2> * 2 * 16 * (D + 2) * 4 : (size_t)sm_count() * kd_ctas<D, 1> * 2 * 8 * (D + 2) * 4; }
+size_t kv4_attn_workspace(int D, int G, int KV, int batch, int max_q, int rows) {
+    (void)KV; (void)batch; (void)rows;
+    const int tile = max_q > 16 / G ? 16 : max_q * G;
+    return D == 64 ? decode_workspace<64>(tile) : D == 128 ? decode_workspace<128>(tile) : decode_workspace<256>(tile);
+}
+template <int D>
+static int launch_attn(const Kv4Cache& c, const Kv4AttnArgs& a, cudaStream_t st) {
+    int rc = 0;
+    const bool many = a.max_q > 16 / a.G;
+    const int tile = many ? 16 : a.max_q * a.G;
+    if (a.G <= 16) rc = tile > 8 ? launch_decode<D, 2>(c, a, 16, st) : launch_decode<D, 1>(c, a, 8, st);
+    if (rc || !many) return rc;
+    return launch_kv4_prompt(c, a, a.G <= 16 ? 16 : 0, st);
+}
+int launch_kv4_attn(const Kv4Cache& c, const Kv4AttnArgs& a, cudaStream_t st) {
+    return c.D == 64 ? launch_attn<64>(c, a, st) : c.D == 128 ? launch_attn<128>(c, a, st) : launch_attn<256>(c, a, st);
+}
+
+}  // namespace sl

@@ -20,10 +20,11 @@ namespace sl {
 // the queries' (the outputs') to follow.  The running maximum is raised only when a score exceeds it by 2^6; the weights are
 // carried times 2^8, so that fp16 holds them from 2^-32 of the largest on.
 constexpr int KD_WARPS = 4, KD_MAX_BATCH = 4096;
-template <int D> constexpr int kd_stages = D == 256 ? 3 : D == 128 ? 4 : 6;
+template <int D, int NT> constexpr int kd_step = D == 256 || NT == 2 ? 1 : 2;                              // blocks a warp takes at a time
+template <int D> constexpr int kd_stages = D == 256 ? 3 : D == 128 ? 4 : 6;                               // blocks of a warp's ring
 template <int D, int NT> constexpr int kd_ctas = D == 256 ? 2 : NT == 1 ? 4 : 3;                          // CTAs of a multiprocessor
 template <int D> constexpr size_t kd_ring = (size_t)KD_WARPS * kd_stages<D> * kv4_block_bytes(D);
-template <int D> constexpr size_t kd_smem(int batch) { return kd_ring<D> + (size_t)KD_WARPS * 8 * (D + 4) * 4 + (size_t)(batch + 1) * 4; }
+template <int D> constexpr size_t kd_smem(int batch) { return kd_ring<D> + (size_t)(batch + 1) * 4; }
 constexpr float KD_UP = 8.0f, KD_SLACK = 6.0f;
 
 // rows of request b (0: none, or more than `most` rows a kv head), and the units of one of its kv heads
@@ -68,7 +69,7 @@ __device__ __forceinline__ int kd_find(const int* pre, int n, int u) {        //
 }
 __device__ __forceinline__ int kd_run(int total, int ctas, int least) {       // units of a CTA
     const int per = max(least, (total + ctas - 1) / ctas);
-    return (per + KD_WARPS - 1) / KD_WARPS * KD_WARPS;
+    return (per + 2 * KD_WARPS - 1) / (2 * KD_WARPS) * (2 * KD_WARPS);
 }
 // a finished row's four dims, gated and rounded once
 __device__ __forceinline__ void kd_finish(const Kv4AttnArgs& a, int row, int h, int d, float4 o, float l) {
@@ -90,12 +91,14 @@ template <int D, int R> __device__ __forceinline__ float* kd_part(const Kv4AttnA
 
 template <int D, int NT>
 __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv4Cache c, Kv4AttnArgs a, int most, int least) {
-    constexpr int R = 8 * NT, S = kd_stages<D>, CH = D / 32, BB = kv4_block_bytes(D), PIECES = BB / 16, NG = D / 64;
+    constexpr int R = 8 * NT, U = kd_step<D, NT>, S = kd_stages<D> / U, CH = D / 32, BB = kv4_block_bytes(D), PIECES = BB / 16;
     extern __shared__ __align__(128) unsigned char smem[];
-    float* s_o = reinterpret_cast<float*>(smem + kd_ring<D>);              // [warps][8 rows][D + 4]
-    int* s_pre = reinterpret_cast<int*>(s_o + KD_WARPS * 8 * (D + 4));
+    float* s_o = reinterpret_cast<float*>(smem);                            // [warps][8 rows][D + 4], where the rings were
+    int* s_pre = reinterpret_cast<int*>(smem + kd_ring<D>);
+    static_assert(kd_ring<D> >= (size_t)KD_WARPS * 8 * (D + 4) * 4, "");
     __shared__ float s_m[KD_WARPS][R], s_l[KD_WARPS][R];
     __shared__ int s_ws[KD_WARPS];
+    __shared__ uint4 s_q[NT * CH][32];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
     pdl_launch_dependents();
     kd_prefix(c, a, most, s_pre, s_ws);
@@ -117,19 +120,13 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv
         const bool whole = j0 == 0 && j1 == sq.units;
         const int n = a.q_start[b + 1] - sq.q0, live = sq.rows * a.G;        // rows of the tile that exist
         // ---- queries: B operands, row g of each N tile; dims 32 i + 8 t .. of piece i in the order that the codes expand in
-        uint32_t q[NT][CH][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int r = nt * 8 + g, i = r / a.G;
-            const __half* src = a.q + (int64_t)(sq.q0 + i) * a.q_row + (int64_t)(head * a.G + r % a.G) * a.q_head + 8 * t;
-#pragma unroll
-            for (int ch = 0; ch < CH; ++ch) {
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (r < live) v = *reinterpret_cast<const uint4*>(src + 32 * ch);
-                q[nt][ch][0] = __byte_perm(v.x, v.z, 0x5410); q[nt][ch][1] = __byte_perm(v.x, v.z, 0x7632);
-                q[nt][ch][2] = __byte_perm(v.y, v.w, 0x5410); q[nt][ch][3] = __byte_perm(v.y, v.w, 0x7632);
-            }
+        for (int x = warp; x < NT * CH; x += KD_WARPS) {
+            const int nt = x / CH, ch = x % CH, r = nt * 8 + g, i = r / a.G;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < live) v = *reinterpret_cast<const uint4*>(a.q + (int64_t)(sq.q0 + i) * a.q_row + (int64_t)(head * a.G + r % a.G) * a.q_head + 8 * t + 32 * ch);
+            s_q[x][lane] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
         }
+        __syncthreads();
         // keys that the lane's columns (rows 2 t, 2 t + 1 of each tile) see, and what all rows see
         int sees[NT][2], all = sq.keys;
 #pragma unroll
@@ -137,135 +134,172 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv
 #pragma unroll
             for (int e = 0; e < 2; ++e) sees[nt][e] = a.causal ? sq.keys - n + (nt * 8 + 2 * t + e) / a.G + 1 : sq.keys;
         if (a.causal) all = min(all, sq.keys - n + 1);
-        float o[NT][CH][2][4], m[NT][2], l[NT][2];
+        float o[NT][CH][2][4], base[NT][2], l[NT][2];                        // base: KD_UP - the maximum
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) o[nt][ch][i >> 2][i & 3] = 0.f;
-            m[nt][0] = m[nt][1] = -INFINITY; l[nt][0] = l[nt][1] = 0.f;
+            base[nt][0] = base[nt][1] = INFINITY; l[nt][0] = l[nt][1] = 0.f;
         }
-        // ---- the warp's blocks j0 + warp, + 4, ..: 32 of them looked up at a time, a lane each
-        const int mine = max(0, (j1 - j0 - warp + KD_WARPS - 1) / KD_WARPS);
+        // ---- the warp's steps of U blocks: warp, + 4, .. of the item's; 32 blocks looked up at a time, a lane each
+        const int mine = max(0, ((j1 - j0 + U - 1) / U - warp + KD_WARPS - 1) / KD_WARPS);
         const int* table = a.table + (int64_t)b * a.table_stride;
         unsigned long long addr = 0;
-        unsigned absent = 0;                                                  // stages whose page is none
+        unsigned absent = 0;                                                  // blocks of the ring that there are none of
         auto issue = [&](int it) {
             if (it < mine) {
-                if ((it & 31) == 0) {
-                    const int k = it + lane;
+                if (it % (32 / U) == 0) {
+                    const int j = j0 + (warp + (it + lane / U) * KD_WARPS) * U + lane % U;
                     addr = 0;
-                    if (k < mine) {
-                        const int j = j0 + warp + k * KD_WARPS, page = table[j / page_blocks];
+                    if (j < j1) {
+                        const int page = table[j / page_blocks];
                         if (page >= 0 && page < c.pages) addr = (unsigned long long)kv4_block(c, page, head, j % page_blocks);
                     }
                 }
-                const unsigned char* src = (const unsigned char*)__shfl_sync(0xffffffffu, addr, it & 31);
-                const int st = it % S;
-                absent &= ~(1u << st);
-                if (src) {
 #pragma unroll
-                    for (int i = 0; i < (PIECES + 31) / 32; ++i)
-                        if (i < PIECES / 32 || lane < PIECES % 32) kv4_cp16(ring_u + st * BB + (lane + 32 * i) * 16, src + (lane + 32 * i) * 16);
-                } else absent |= 1u << st;
+                for (int x = 0; x < U; ++x) {
+                    const unsigned char* src = (const unsigned char*)__shfl_sync(0xffffffffu, addr, it % (32 / U) * U + x);
+                    const int st = it % S * U + x;
+                    absent &= ~(1u << st);
+                    if (src) {
+                        const uint32_t dst = ring_u + st * BB + lane * 16;
+                        src += lane * 16;
+#pragma unroll
+                        for (int i = 0; i < (PIECES + 31) / 32; ++i) if (i < PIECES / 32 || lane < PIECES % 32) kv4_cp16(dst + i * 512, src + i * 512);
+                    } else absent |= 1u << st;
+                }
             }
             kv4_commit();
         };
 #pragma unroll
         for (int it = 0; it < S - 1; ++it) issue(it);
+#pragma unroll 1
         for (int it = 0; it < mine; ++it) {
             kv4_wait<S - 2>();
             __syncwarp();
-            issue(it + S - 1);                                                // (into the stage that the block before has left)
-            const int st = it % S, key0 = (j0 + warp + it * KD_WARPS) * KV4_B;
-            if (absent >> st & 1) continue;
+            issue(it + S - 1);                                                // (into the stage that the step before has left)
+            const int st = it % S * U, key0 = (j0 + (warp + it * KD_WARPS) * U) * KV4_B;
+            const unsigned gone = absent >> st & ((1u << U) - 1);
+            if (gone == (1u << U) - 1) continue;
             const uint32_t blk = ring_u + st * BB;
-            const __half* sb = reinterpret_cast<const __half*>(ring + st * BB + 16 * D);
-            // ---- S^T: 16 keys x 8 rows
-            float s[NT][4];
+            // ---- S^T: 16 U keys x 8 rows
+            float s[U][NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+            for (int x = 0; x < U; ++x)
+#pragma unroll
+                for (int i = 0; i < NT * 4; ++i) s[x][i >> 2][i & 3] = 0.f;
 #pragma unroll
             for (int i = 0; i < CH / 2; ++i) {                                // a 64-dim group: two pieces
-                uint32_t w[4];
-                kv4_ldsm(w, blk + lm[i]);
-                const __half2 sa = __half2half2(sb[i * 32 + g]), sc = __half2half2(sb[i * 32 + g + 8]), ba = __half2half2(sb[i * 32 + 16 + g]), bc = __half2half2(sb[i * 32 + 24 + g]);
+                uint32_t w[U][4], sb[U][4];
+#pragma unroll
+                for (int x = 0; x < U; ++x) {
+                    kv4_ldsm(w[x], blk + x * BB + lm[i]);
+                    kv4_ldsm_t(sb[x], blk + x * BB + 16 * D + i * 64 + (lane >> 3) * 16);      // (eight equal rows, transposed: scales of keys g, g + 8, biases, each twice)
+                }
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    uint32_t x[4], y[4];
-                    kv4_expand(w[2 * e], sa, ba, x); kv4_expand(w[2 * e + 1], sc, bc, y);
+                    uint4 qf[NT];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        kv4_mma(s[nt], x[0], y[0], x[1], y[1], q[nt][2 * i + e][0], q[nt][2 * i + e][1]);
-                        kv4_mma(s[nt], x[2], y[2], x[3], y[3], q[nt][2 * i + e][2], q[nt][2 * i + e][3]);
+                    for (int nt = 0; nt < NT; ++nt) qf[nt] = s_q[nt * CH + 2 * i + e][lane];
+#pragma unroll
+                    for (int x = 0; x < U; ++x) {
+                        uint32_t k0[4], k8[4];
+                        kv4_expand(w[x][2 * e], kv4_h2(sb[x][0]), kv4_h2(sb[x][2]), k0); kv4_expand(w[x][2 * e + 1], kv4_h2(sb[x][1]), kv4_h2(sb[x][3]), k8);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            kv4_mma(s[x][nt], k0[0], k8[0], k0[1], k8[1], qf[nt].x, qf[nt].y);
+                            kv4_mma(s[x][nt], k0[2], k8[2], k0[3], k8[3], qf[nt].z, qf[nt].w);
+                        }
                     }
                 }
             }
-            const bool edge = key0 + KV4_B > all;
-            bool raise = false;
+            const bool edge = key0 + U * KV4_B > all || gone;
+            float p[U][NT][4], high = -INFINITY;
+            auto hidden = [&](int x, int nt, int e) { return key0 + x * KV4_B + g + 8 * (e >> 1) >= sees[nt][e & 1] || (gone >> x & 1); };
+            auto weigh = [&] {                                                // exponents of the weights; above KD_UP + KD_SLACK: the maximum has to be raised
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+                for (int x = 0; x < U; ++x)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[nt][e] *= a.scale;                                      // (times log2 e: the host's)
-                    if (edge && key0 + g + 8 * (e >> 1) >= sees[nt][e & 1]) s[nt][e] = -INFINITY;
-                    raise |= s[nt][e] > m[nt][e & 1] + KD_SLACK;
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) p[x][nt][e] = fmaf(s[x][nt][e], a.scale, base[nt][e & 1]);      // (scale: times log2 e, by the host)
+                if (edge) {
+#pragma unroll
+                    for (int x = 0; x < U; ++x)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) if (hidden(x, nt, e)) p[x][nt][e] = -INFINITY;
                 }
-            if (__any_sync(0xffffffffu, raise)) {
+            };
+            weigh();
+#pragma unroll
+            for (int x = 0; x < U; ++x)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) high = fmaxf(high, fmaxf(fmaxf(p[x][nt][0], p[x][nt][1]), fmaxf(p[x][nt][2], p[x][nt][3])));
+            if (__any_sync(0xffffffffu, high > KD_UP + KD_SLACK)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float x = fmaxf(s[nt][e], s[nt][e + 2]);
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4)); x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8)); x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                        x = fmaxf(x, m[nt][e]);
-                        const float f = x == -INFINITY ? 1.f : kv4_exp2(m[nt][e] - x);
-                        m[nt][e] = x; l[nt][e] *= f;
+                        float y = -INFINITY;
+#pragma unroll
+                        for (int x = 0; x < U; ++x) {
+                            if (!edge || !hidden(x, nt, e)) y = fmaxf(y, s[x][nt][e] * a.scale);
+                            if (!edge || !hidden(x, nt, e + 2)) y = fmaxf(y, s[x][nt][e + 2] * a.scale);
+                        }
+                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4)); y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8)); y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+                        const float old = KD_UP - base[nt][e], top = fmaxf(y, old), f = top == -INFINITY ? 1.f : kv4_exp2(old - top);
+                        base[nt][e] = KD_UP - top; l[nt][e] *= f;
 #pragma unroll
                         for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
-                            for (int p = 0; p < 2; ++p) { o[nt][ch][p][e] *= f; o[nt][ch][p][e + 2] *= f; }
+                            for (int k = 0; k < 2; ++k) { o[nt][ch][k][e] *= f; o[nt][ch][k][e + 2] *= f; }
                     }
+                weigh();
             }
-            uint32_t pb[NT][2];
+            uint32_t pb[U][NT][2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float p[4];
+            for (int x = 0; x < U; ++x)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float top = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
-                    p[e] = kv4_exp2(s[nt][e] - (top - KD_UP));
-                    l[nt][e & 1] += p[e];
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { p[x][nt][e] = kv4_exp2(p[x][nt][e]); l[nt][e & 1] += p[x][nt][e]; }
+                    pb[x][nt][0] = kv4_transpose(kv4_pack(p[x][nt][0], p[x][nt][1])); pb[x][nt][1] = kv4_transpose(kv4_pack(p[x][nt][2], p[x][nt][3]));
                 }
-                pb[nt][0] = kv4_transpose(kv4_pack(p[0], p[1])); pb[nt][1] = kv4_transpose(kv4_pack(p[2], p[3]));
-            }
             // ---- O^T: dims x 8 rows; a lane's registers: dims 32 ch + 4 g + (0 .. 3) of rows 2 t, 2 t + 1
-            const bool tail = key0 + KV4_B > sq.keys;                         // (positions that nobody has: their weights are 0, their scales anything)
-            const __half* vb = sb + D / 2;
+            const bool tail = key0 + U * KV4_B > sq.keys || gone;
 #pragma unroll
             for (int i = 0; i < CH / 2; ++i) {
-                uint32_t w[4], sv[4];
-                kv4_ldsm_t(w, blk + 8 * D + lm[i]);
+                uint32_t w[U][4], sv[U][4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sv[e] = *reinterpret_cast<const uint32_t*>(vb + i * 32 + 2 * t + 8 * e);       // scales of keys 2 t, + 8; biases
-                if (tail) {
+                for (int x = 0; x < U; ++x) {
+                    kv4_ldsm_t(w[x], blk + x * BB + 8 * D + lm[i]);
+                    kv4_ldsm(sv[x], blk + x * BB + 17 * D + i * 64 + (lane >> 3) * 16);        // (scales of keys 2 t, 2 t + 1; of 2 t + 8, + 9; biases)
+                }
+                if (tail) {                                                   // positions that nobody has: their weights are 0, their scales anything
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int k = key0 + 2 * t + 8 * (e & 1);
-                        if (k >= sq.keys) sv[e] = 0; else if (k + 1 >= sq.keys) sv[e] &= 0xffffu;
-                    }
+                    for (int x = 0; x < U; ++x)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int k = key0 + x * KV4_B + 2 * t + 8 * (e & 1);
+                            if (k >= sq.keys || (gone >> x & 1)) sv[x][e] = 0; else if (k + 1 >= sq.keys) sv[x][e] &= 0xffffu;
+                        }
                 }
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    uint32_t x[4], y[4];
-                    kv4_expand(w[2 * e], kv4_h2(sv[0]), kv4_h2(sv[2]), x); kv4_expand(w[2 * e + 1], kv4_h2(sv[1]), kv4_h2(sv[3]), y);
+                for (int x = 0; x < U; ++x)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        kv4_mma(o[nt][2 * i + e][0], x[0], x[1], y[0], y[1], pb[nt][0], pb[nt][1]);
-                        kv4_mma(o[nt][2 * i + e][1], x[2], x[3], y[2], y[3], pb[nt][0], pb[nt][1]);
+                    for (int e = 0; e < 2; ++e) {
+                        uint32_t v0[4], v8[4];
+                        kv4_expand(w[x][2 * e], kv4_h2(sv[x][0]), kv4_h2(sv[x][2]), v0); kv4_expand(w[x][2 * e + 1], kv4_h2(sv[x][1]), kv4_h2(sv[x][3]), v8);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            kv4_mma(o[nt][2 * i + e][0], v0[0], v0[1], v8[0], v8[1], pb[x][nt][0], pb[x][nt][1]);
+                            kv4_mma(o[nt][2 * i + e][1], v0[2], v0[3], v8[2], v8[3], pb[x][nt][0], pb[x][nt][1]);
+                        }
                     }
-                }
             }
         }
         kv4_wait<0>();
@@ -275,9 +309,10 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 4); l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 8); l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
-                if (g == 0) { s_m[warp][nt * 8 + 2 * t + e] = m[nt][e]; s_l[warp][nt * 8 + 2 * t + e] = l[nt][e]; }
+                if (g == 0) { s_m[warp][nt * 8 + 2 * t + e] = KD_UP - base[nt][e]; s_l[warp][nt * 8 + 2 * t + e] = l[nt][e]; }
             }
         float* part = kd_part<D, R>(a, blockIdx.x, j0 > 0 ? 0 : 1);
+        __syncthreads();                                                      // (the rings are done with)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -313,35 +348,67 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv
         if (u < u1 && u >= s_pre[b + 1]) { b = kd_find(s_pre, a.batch, u); sq = kd_seq(c, a, b, most); }
     }
 }
-// grid (kv heads, requests): adds up the partial sums of a (request, kv head) that more than one CTA had
+// grid (rows, kv heads, requests): adds up the partial sums of a row whose (request, kv head) more than one CTA had.  A warp takes every
+// fourth of them, eight in flight, behind one look at all their maxima.
 template <int D, int NT>
 __global__ void __launch_bounds__(KD_WARPS * 32) k_kv4_join(Kv4Cache c, Kv4AttnArgs a, int most, int least, int ctas) {
-    constexpr int R = 8 * NT;
+    constexpr int R = 8 * NT, V = D / 32;
     extern __shared__ int s_pre[];
     __shared__ int s_ws[KD_WARPS];
-    const int head = blockIdx.x, b = blockIdx.y;
+    __shared__ __align__(16) float s_o[KD_WARPS][D];
+    const int r = blockIdx.x, head = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     kd_prefix(c, a, most, s_pre, s_ws);
     const KdSeq sq = kd_seq(c, a, b, most);
     pdl_wait();                              // (every CTA: what follows this kernel in the stream also follows the one before)
-    if (!sq.units) return;
-    const int per = kd_run(s_pre[a.batch], ctas, least), u0 = s_pre[b] + head * sq.units, c0 = u0 / per, c1 = (u0 + sq.units - 1) / per;
-    if (c0 == c1) return;
-    const int live = sq.rows * a.G;
-    for (int x = threadIdx.x; x < live * (D / 4); x += KD_WARPS * 32) {
-        const int r = x / (D / 4), d = x % (D / 4) * 4;
-        float top = -INFINITY, sum = 0.f;
-        for (int i = c0; i <= c1; ++i) top = fmaxf(top, kd_part<D, R>(a, i, i > c0 ? 0 : 1)[(size_t)R * D + 2 * r]);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = c0; i <= c1; ++i) {
-            const float* p = kd_part<D, R>(a, i, i > c0 ? 0 : 1);
-            const float2 ml = *reinterpret_cast<const float2*>(p + (size_t)R * D + 2 * r);
-            const float4 y = *reinterpret_cast<const float4*>(p + (size_t)r * D + d);
-            const float f = ml.x == -INFINITY ? 0.f : kv4_exp2(ml.x - top);
-            sum = fmaf(ml.y, f, sum);
-            v.x = fmaf(y.x, f, v.x); v.y = fmaf(y.y, f, v.y); v.z = fmaf(y.z, f, v.z); v.w = fmaf(y.w, f, v.w);
+    if (r >= sq.rows * a.G) return;
+    const int per = kd_run(s_pre[a.batch], ctas, least), u0 = s_pre[b] + head * sq.units, c0 = u0 / per, n = (u0 + sq.units - 1) / per - c0 + 1;
+    if (n == 1) return;
+    // piece i: the first CTA's item goes on behind its run, the others' began before theirs
+    auto part = [&](int i) { return kd_part<D, R>(a, c0 + i, i > 0 ? 0 : 1); };
+    auto ml_of = [&](int i) { return i < n ? *reinterpret_cast<const float2*>(part(i) + (size_t)R * D + 2 * r) : make_float2(-INFINITY, 0.f); };
+    float2 ml = ml_of(lane);
+    float top = ml.x;
+    for (int i = 32; i < n; i += 32) top = fmaxf(top, ml_of(i + lane).x);
+    top = warp_max(top);
+    float v[V] = {}, sum = 0.f;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        if (i0) ml = ml_of(i0 + lane);
+        const float f = ml.x == -INFINITY ? 0.f : kv4_exp2(ml.x - top);
+        sum = fmaf(ml.y, f, sum);
+        {
+            float y[8][V];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int i = warp + 4 * k;
+                const float* src = part(i0 + i) + (size_t)r * D + lane * V;
+#pragma unroll
+                for (int x = 0; x < V; x += 2) {
+                    float2 t = make_float2(0.f, 0.f);
+                    if (i0 + i < n) t = *reinterpret_cast<const float2*>(src + x);
+                    y[k][x] = t.x; y[k][x + 1] = t.y;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float fk = __shfl_sync(0xffffffffu, f, warp + 4 * k);
+#pragma unroll
+                for (int x = 0; x < V; ++x) v[x] = fmaf(y[k][x], fk, v[x]);
+            }
         }
-        kd_finish(a, sq.q0 + r / a.G, head * a.G + r % a.G, d, v, sum);
     }
+    sum = warp_sum(sum);
+#pragma unroll
+    for (int x = 0; x < V; ++x) s_o[warp][lane * V + x] = v[x];
+    __syncthreads();
+    const int d = threadIdx.x * 4;
+    if (d >= D) return;
+    float4 o = *reinterpret_cast<const float4*>(&s_o[0][d]);
+#pragma unroll
+    for (int w = 1; w < KD_WARPS; ++w) {
+        const float4 y = *reinterpret_cast<const float4*>(&s_o[w][d]);
+        o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
+    }
+    kd_finish(a, sq.q0 + r / a.G, head * a.G + r % a.G, d, o, sum);
 }
 constexpr int KD_LEAST = 8;              // units a CTA takes at least
 template <int D, int NT>
@@ -360,7 +427,7 @@ static int launch_decode(const Kv4Cache& c, Kv4AttnArgs a, int most, cudaStream_
     int rc = 0;
     profile_launch("k_kv4_decode", st, [&] { return rc = launch_pdl(false, k_kv4_decode<D, NT>, dim3((unsigned)ctas), KD_WARPS * 32, smem, st, c, a, most, KD_LEAST); });
     if (rc) return rc;
-    profile_launch("k_kv4_join", st, [&] { return rc = launch_pdl(true, k_kv4_join<D, NT>, dim3((unsigned)c.KV, (unsigned)a.batch), KD_WARPS * 32, (size_t)(a.batch + 1) * 4, st, c, a, most, KD_LEAST, ctas); });
+    profile_launch("k_kv4_join", st, [&] { return rc = launch_pdl(true, k_kv4_join<D, NT>, dim3((unsigned)(a.G * (a.max_q < most / a.G ? a.max_q : most / a.G)), (unsigned)c.KV, (unsigned)a.batch), KD_WARPS * 32, (size_t)(a.batch + 1) * 4, st, c, a, most, KD_LEAST, ctas); });
     return rc;
 }
 

@@ -32,14 +32,18 @@ __device__ __forceinline__ __half2 kv4_h2(uint32_t v) { return *reinterpret_cast
 __device__ __forceinline__ uint32_t kv4_u(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 // Eight codes of a word -> halves code * s + b in pairs (0, 4), (1, 5), (2, 6), (3, 7).  A code in the low bits of a half whose exponent says
 // 1024 is 1024 + code, four bits further up under an exponent of 64 it is 64 + code: one masking instruction a pair, an exact
-// subtraction and one multiply-add with one rounding.
+// subtraction and one multiply-add with one rounding.  (Mask and exponent written in C took two instructions.)
+template <uint32_t MASK, uint32_t EXP> __device__ __forceinline__ __half2 kv4_codes(uint32_t w) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "n"(MASK), "r"(EXP));       // (w & MASK) | EXP
+    return __hsub2(kv4_h2(r), kv4_h2(EXP));
+}
 __device__ __forceinline__ void kv4_expand(uint32_t w, __half2 s, __half2 b, uint32_t o[4]) {
-    const __half2 k1024 = kv4_h2(0x64006400u), k64 = kv4_h2(0x54005400u);
     const uint32_t v = w >> 8;
-    o[0] = kv4_u(__hfma2(__hsub2(kv4_h2((w & 0x000f000fu) | 0x64006400u), k1024), s, b));
-    o[1] = kv4_u(__hfma2(__hsub2(kv4_h2((w & 0x00f000f0u) | 0x54005400u), k64), s, b));
-    o[2] = kv4_u(__hfma2(__hsub2(kv4_h2((v & 0x000f000fu) | 0x64006400u), k1024), s, b));
-    o[3] = kv4_u(__hfma2(__hsub2(kv4_h2((v & 0x00f000f0u) | 0x54005400u), k64), s, b));
+    o[0] = kv4_u(__hfma2(kv4_codes<0x000f000fu, 0x64006400u>(w), s, b));
+    o[1] = kv4_u(__hfma2(kv4_codes<0x00f000f0u, 0x54005400u>(w), s, b));
+    o[2] = kv4_u(__hfma2(kv4_codes<0x000f000fu, 0x64006400u>(v), s, b));
+    o[3] = kv4_u(__hfma2(kv4_codes<0x00f000f0u, 0x54005400u>(v), s, b));
 }
 
 }  // namespace sl
