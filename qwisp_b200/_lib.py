@@ -140,11 +140,12 @@ SYMBOLS = {
     "sl_op_layer": (_I32, [_VP, _I32, _VP, _I32, _I32, _VP]),
     "sl_op_head": (_I32, [_VP, _VP, _I32, _VP, _VP]),
     "sl_kv4_page_bytes": (_I64, [_I32, _I32, _I32]),
-    "sl_op_kv_plan_device": (_I32, [C.POINTER(SlKvPlan), _VP]),
-    "sl_op_kv4_append_device": (_I32, [C.POINTER(SlKv4Cache), C.POINTER(SlKv4Append), _VP]),
-    "sl_op_kv4_read_device": (_I32, [C.POINTER(SlKv4Cache), C.POINTER(SlKv4Read), _VP]),
+    # (argument blocks: a structure by reference, or its bytes packed)
+    "sl_op_kv_plan_device": (_I32, [_VP, _VP]),
+    "sl_op_kv4_append_device": (_I32, [_VP, _VP, _VP]),
+    "sl_op_kv4_read_device": (_I32, [_VP, _VP, _VP]),
     "sl_kv4_attention_workspace": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32]),
-    "sl_op_kv4_attention_device": (_I32, [C.POINTER(SlKv4Cache), C.POINTER(SlKv4Attention), _VP]),
+    "sl_op_kv4_attention_device": (_I32, [_VP, _VP, _VP]),
     "sl_synth_tokens": (_I32, [_U64, C.c_char_p, _I64, _I32, _VP]),
     "sl_synth_f16": (_I32, [_U64, C.c_char_p, _I64, _F, _F, _VP]),
 }

@@ -27,6 +27,11 @@ struct Kv4Cache {
 __device__ __forceinline__ unsigned char* kv4_block(const Kv4Cache& c, int page, int head, int block) {
     return c.data + (int64_t)page * c.page_stride + ((int64_t)head * (c.page_size / KV4_B) + block) * kv4_block_bytes(c.D);
 }
+// (page, offset in it) of a slot of the cache.  (A 64-bit division is some hundred instructions: only where the slot needs it.)
+__device__ __forceinline__ void kv4_place(const Kv4Cache& c, int64_t slot, int& page, int& off) {
+    if (slot >> 31 == 0) { page = (int)((uint32_t)slot / (uint32_t)c.page_size); off = (int)slot - page * c.page_size; }
+    else { page = (int)(slot / c.page_size); off = (int)(slot - (int64_t)page * c.page_size); }
+}
 
 struct KvPlanArgs {
     const int *lens, *news; int batch, page_size;

@@ -11,36 +11,48 @@
 
 namespace sl {
 
-constexpr int KA_WARPS = 8;
+constexpr int KA_WARPS = 4;
 
-__device__ __forceinline__ uint32_t kv4_code(float x, float bias, float scale) {
-    return (uint32_t)fminf(fmaxf(roundf(__fdiv_rn(__fsub_rn(x, bias), scale)), 0.0f), 15.0f);
+// a / s, rounded to nearest, where r is 1 / s rounded to nearest: the quotient's remainder by one fused multiply-add, and a second one
+// that adds what it is worth (Markstein, "Computation of elementary functions on the IBM RISC System/6000", 1990).  For the sizes
+// of a group's values: nothing here under- or overflows.
+__device__ __forceinline__ float kv4_div(float a, float s, float r) {
+    const float q = __fmul_rn(a, r);
+    return __fmaf_rn(__fmaf_rn(-q, s, a), r, q);
 }
 // Eight dims of a head a lane, eight lanes a group: stores the lane's word of codes and the group's scale and bias.  By whole warps;
 // `store`: the lane has a head.  region: 0 = K, 1 = V.
 __device__ __forceinline__ void kv4_store(const Kv4Cache& c, unsigned char* blk, int at, int region, int hl, const float x[8], bool store) {
     float lo = x[0], hi = x[0];
-    bool odd = !(fabsf(x[0]) <= 65504.0f);
 #pragma unroll
-    for (int i = 1; i < 8; ++i) { lo = fminf(lo, x[i]); hi = fmaxf(hi, x[i]); odd |= !(fabsf(x[i]) <= 65504.0f); }
+    for (int i = 1; i < 8; ++i) { lo = fminf(lo, x[i]); hi = fmaxf(hi, x[i]); }
+    // fmin and fmax pass a NaN over, so the sum of 0 * x tells of one (and of an infinity)
+    float odd = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) odd = fmaf(x[i], 0.f, odd);
 #pragma unroll
     for (int d = 1; d < 8; d <<= 1) { lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d)); hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d)); }
-    odd = (__ballot_sync(0xffffffffu, odd) >> (threadIdx.x & 24) & 0xffu) != 0;
-    float scale = fmaxf(__fdiv_rn(__fsub_rn(hi, lo), 15.0f), 1e-7f);
+    const bool bad = (__ballot_sync(0xffffffffu, odd != 0.f) >> (threadIdx.x & 24) & 0xffu) != 0;
+    float scale = fmaxf(kv4_div(__fsub_rn(hi, lo), 15.0f, 0x1.111112p-4f), 1e-7f);
     const bool side = fabsf(lo) > fabsf(hi);
     scale = side ? scale : -scale;
     const float edge = side ? lo : hi, q0 = roundf(__fdiv_rn(edge, scale));
     const bool zero = q0 == 0.0f;
     scale = zero ? scale : __fdiv_rn(edge, q0);
-    const float bias = zero ? 0.0f : edge;
-    uint32_t w = 0;
+    const float bias = zero ? 0.0f : edge, r = __frcp_rn(scale);
+    // rounded to the nearest code, halves up: with the addition rounded towards zero, adding a half and 2^23 truncates to the lowest bits
+    float w[2] = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w |= kv4_code(x[i], bias, scale) << (4 * i);
+    for (int i = 7; i >= 0; --i) {
+        const float q = fminf(fmaxf(kv4_div(__fsub_rn(x[i], bias), scale, r), 0.0f), 15.0f);
+        w[i >> 2] = fmaf(w[i >> 2], 16.0f, __fadd_rn(__fadd_rz(__fadd_rz(q, 0.5f), 8388608.0f), -8388608.0f));        // (four codes: below 2^16, exact)
+    }
+    const uint32_t word = __byte_perm(__float_as_uint(w[0] + 8388608.0f), __float_as_uint(w[1] + 8388608.0f), 0x5410);
     if (!store) return;
-    *reinterpret_cast<uint32_t*>(blk + region * 8 * c.D + kv4_swz((uint32_t)(at * (c.D / 2) + hl * 4))) = w;
+    *reinterpret_cast<uint32_t*>(blk + region * 8 * c.D + kv4_swz((uint32_t)(at * (c.D / 2) + hl * 4))) = word;
     if ((hl & 7) == 0) {
         __half* sb = reinterpret_cast<__half*>(blk + (16 + region) * c.D) + (hl >> 3) * 2 * KV4_B + at;
-        sb[0] = odd ? __ushort_as_half(0x7fff) : f2h(scale);
+        sb[0] = bad ? __ushort_as_half(0x7fff) : f2h(scale);
         sb[KV4_B] = f2h(bias);
     }
 }
@@ -48,112 +60,131 @@ __device__ __forceinline__ void kv4_store(const Kv4Cache& c, unsigned char* blk,
 // A row's angles once per CTA: turns = position * frequency as a 64-bit fraction of a turn, exact for every position, then cos and
 // sin in 64 bits.  Keys stay in 64 bits up to the one rounding to fp16 (a code next to a border then does not go by the order of a sum or
 // by the shape of the launch); queries take 32.
-// grid (rows, parts), a warp a task: 32 / (D / 8) heads of one kind, eight dims a lane.
+// grid (rows, parts), a warp a task: 32 / (D / 8) heads of one kind, eight dims a lane, the next task's halves on their way.
 template <int D>
-__global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_append(Kv4Cache c, Kv4AppendArgs a) {
+__global__ void __launch_bounds__(KA_WARPS * 32, 8) k_kv4_append(Kv4Cache c, Kv4AppendArgs a) {
     constexpr int LPH = D / 8, HPW = 32 / LPH;                // lanes of a head, heads of a warp
-    __shared__ double2 s_cs[D / 2];
+    __shared__ __align__(16) double2 s_d[8][LPH];             // (cos, sin with the sign that dim takes it with) of dim 8 hl + i at [i][hl]
+    __shared__ __align__(16) float2 s_f[4][LPH][2];           // the same in 32 bits, of dims 8 hl + 2 j, + 1
     const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hl = lane % LPH, hs = lane / LPH;
     const int64_t slot = a.slots ? a.slots[row] : 0;
     if (a.slots && (slot < 0 || slot >= c.pages * (int64_t)c.page_size)) return;         // padding
+    const int nk = a.k ? (c.KV + HPW - 1) / HPW : 0, tasks = 2 * nk + (a.q ? (a.NH + HPW - 1) / HPW : 0), stride = gridDim.y * KA_WARPS;
+    struct Task { int kind, head; bool have; };               // kind: 0 = K, 1 = V, 2 = query
+    auto task_of = [&](int i) {
+        Task t;
+        t.kind = i < nk ? 0 : i < 2 * nk ? 1 : 2;
+        t.head = (i - t.kind * nk) * HPW + hs;
+        t.have = i < tasks && t.head < (t.kind == 2 ? a.NH : c.KV);
+        return t;
+    };
+    auto load = [&](const Task& t) {
+        const __half* src = t.kind == 0 ? a.k + row * a.k_row + t.head * a.k_head : t.kind == 1 ? a.v + row * a.v_row + t.head * a.v_head : a.q + row * a.q_row + t.head * a.q_head;
+        return t.have ? reinterpret_cast<const uint4*>(src)[hl] : make_uint4(0, 0, 0, 0);
+    };
+    int i = blockIdx.y * KA_WARPS + warp;
+    Task task = task_of(i);
+    uint4 raw = load(task);
     const int half = a.rope >> 1;
-    for (int i = tid; i < half; i += KA_WARPS * 32) {
-        const uint64_t t = (uint64_t)(int64_t)a.pos[(int64_t)a.axis[i] * a.pos_axis + row] * a.turn[i];      // (modulo 2^64: a whole turn)
+    auto put = [&](int d, double cs, double sn) {
+        s_d[d & 7][d >> 3] = make_double2(cs, sn);
+        s_f[(d & 7) >> 1][d >> 3][d & 1] = make_float2((float)cs, (float)sn);
+    };
+    for (int f = tid; f < half; f += KA_WARPS * 32) {
+        const uint64_t t = (uint64_t)(int64_t)a.pos[(int64_t)a.axis[f] * a.pos_axis + row] * a.turn[f];      // (modulo 2^64: a whole turn)
         double sn, cs;
         sincospi((double)(int64_t)t * 0x1p-63, &sn, &cs);
-        s_cs[i] = make_double2(cs, sn);
+        put(f, cs, -sn); put(f + half, cs, sn);
     }
+    for (int d = a.rope + tid; d < D; d += KA_WARPS * 32) put(d, 1.0, 0.0);
     __syncthreads();
-    const int nq = a.q ? (a.NH + HPW - 1) / HPW : 0, nk = a.k ? (c.KV + HPW - 1) / HPW : 0;
-    unsigned char* page = nullptr; int blk = 0, at = 0;
-    if (nk) {
-        const int off = (int)(slot % c.page_size);
-        page = kv4_block(c, (int)(slot / c.page_size), 0, 0); blk = off / KV4_B; at = off % KV4_B;
-    }
+    const int partner = hl * 8 >= a.rope ? lane : hl * 8 < half ? lane + a.rope / 16 : lane - a.rope / 16;      // has the dims these are rotated with
+    int pg = 0, off = 0;
+    if (nk) kv4_place(c, slot, pg, off);
+    const int at = off % KV4_B;
+    unsigned char* page = kv4_block(c, pg, 0, off / KV4_B);   // (head 0's block)
     const int64_t head_bytes = (int64_t)(c.page_size / KV4_B) * kv4_block_bytes(D);
-    const int src_lane = hl < a.rope / 16 ? lane + a.rope / 16 : lane - a.rope / 16;     // has the dims these are rotated with
-    const bool turned = hl * 8 < a.rope, first = hl * 8 < half;
-    for (int task = blockIdx.y * KA_WARPS + warp; task < nq + 2 * nk; task += gridDim.y * KA_WARPS) {
-        const int kind = task < nq ? 0 : task < nq + nk ? 1 : 2, head = (task - (kind ? nq + (kind - 1) * nk : 0)) * HPW + hs;
-        const bool have = head < (kind ? c.KV : a.NH);
-        const __half* src = kind == 0 ? a.q + row * a.q_row + head * a.q_head : kind == 1 ? a.k + row * a.k_row + head * a.k_head : a.v + row * a.v_row + head * a.v_head;
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (have) raw = reinterpret_cast<const uint4*>(src)[hl];
-        const __half* h = reinterpret_cast<const __half*>(&raw);
-        unsigned char* dst = page + head * head_bytes + (int64_t)blk * kv4_block_bytes(D);
-        if (kind == 2) {
-            float x[8];
+    for (; i < tasks; i += stride) {
+        const Task now = task;
+        const uint4 cur = raw;
+        task = task_of(i + stride);
+        raw = load(task);
+        const __half* h = reinterpret_cast<const __half*>(&cur);
+        float x[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = h2f(h[i]);
-            kv4_store(c, dst, at, 1, hl, x, have);
-            continue;
-        }
-        const __half* w = kind ? a.k_norm : a.q_norm;
+        for (int k = 0; k < 8; ++k) x[k] = h2f(h[k]);
+        const __half* w = now.kind == 0 ? a.k_norm : now.kind == 2 ? a.q_norm : nullptr;
         uint4 wraw = make_uint4(0, 0, 0, 0);
         if (w) wraw = reinterpret_cast<const uint4*>(w)[hl];
         const __half* wh = reinterpret_cast<const __half*>(&wraw);
-        if (kind == 0) {
-            float x[8], ss = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { x[i] = h2f(h[i]); ss = fmaf(x[i], x[i], ss); }
+        if (now.kind == 2) {
             if (w) {
+                float ss = 0.f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) ss = fmaf(x[k], x[k], ss);
 #pragma unroll
                 for (int d = 1; d < LPH; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-                const float inv = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
+                const float inv = __frsqrt_rn(fmaf(ss, 1.0f / D, a.eps));
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * h2f(wh[i]);
+                for (int k = 0; k < 8; ++k) x[k] = x[k] * inv * h2f(wh[k]);
             }
-            uint4 o; __half* oh = reinterpret_cast<__half*>(&o);
+            uint4 o; uint32_t* ow = reinterpret_cast<uint32_t*>(&o);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float other = __shfl_sync(0xffffffffu, x[i], src_lane);
-                if (turned) {
-                    const double2 cs = s_cs[first ? hl * 8 + i : hl * 8 + i - half];
-                    x[i] = first ? x[i] * (float)cs.x - other * (float)cs.y : x[i] * (float)cs.x + other * (float)cs.y;
-                }
-                oh[i] = f2h(x[i]);
+            for (int j = 0; j < 4; ++j) {
+                const float4 cs = *reinterpret_cast<const float4*>(s_f[j][hl]);
+                const float u = __shfl_sync(0xffffffffu, x[2 * j], partner), v = __shfl_sync(0xffffffffu, x[2 * j + 1], partner);
+                const __half2 y = __floats2half2_rn(fmaf(u, cs.y, x[2 * j] * cs.x), fmaf(v, cs.w, x[2 * j + 1] * cs.z));
+                ow[j] = *reinterpret_cast<const uint32_t*>(&y);
             }
-            if (have) reinterpret_cast<uint4*>(a.q_out + row * a.o_row + head * a.o_head)[hl] = o;
-        } else {
-            double x[8], ss = 0.0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { x[i] = (double)h2f(h[i]); ss = fma(x[i], x[i], ss); }
-            if (w) {
-#pragma unroll
-                for (int d = 1; d < LPH; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-                const double inv = 1.0 / sqrt(ss * (1.0 / D) + (double)a.eps);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * (double)h2f(wh[i]);
-            }
-            float y[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const double other = __shfl_sync(0xffffffffu, x[i], src_lane);
-                if (turned) {
-                    const double2 cs = s_cs[first ? hl * 8 + i : hl * 8 + i - half];
-                    x[i] = first ? x[i] * cs.x - other * cs.y : x[i] * cs.x + other * cs.y;
-                }
-                y[i] = h2f(f2h((float)x[i]));
-            }
-            kv4_store(c, dst, at, 0, hl, y, have);
+            if (now.have) reinterpret_cast<uint4*>(a.q_out + row * a.o_row + now.head * a.o_head)[hl] = o;
+            continue;
         }
+        if (now.kind == 0 && (w || a.rope)) {
+            double y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = (double)x[k];
+            if (w) {
+                double ss = 0.0;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) ss = fma(y[k], y[k], ss);
+#pragma unroll
+                for (int d = 1; d < LPH; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+                const double inv = rsqrt(fma(ss, 1.0 / D, (double)a.eps));
+#pragma unroll
+                for (int k = 0; k < 8; ++k) y[k] = y[k] * inv * (double)h2f(wh[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const double2 cs = s_d[k][hl];
+                const double other = __shfl_sync(0xffffffffu, y[k], partner);
+                x[k] = h2f(f2h((float)fma(other, cs.y, y[k] * cs.x)));
+            }
+        }
+        kv4_store(c, page + now.head * head_bytes, at, now.kind, hl, x, now.have);
     }
 }
 
-// a lane a word of codes: eight dims of K or V of a (row, head)
+// a warp a row, a lane a word of codes: eight dims of K or V of a head
 template <int D>
 __global__ void __launch_bounds__(256) k_kv4_read(Kv4Cache c, Kv4ReadArgs a) {
     constexpr int LPH = D / 8;
-    const int64_t n = (int64_t)a.rows * c.KV * 2 * LPH;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int hl = (int)(i % LPH), region = (int)(i / LPH & 1), head = (int)(i / (2 * LPH) % c.KV);
-        const int64_t row = i / ((int64_t)2 * LPH * c.KV), slot = a.slots[row];
-        if (slot < 0 || slot >= c.pages * (int64_t)c.page_size) continue;
-        const int off = (int)(slot % c.page_size), at = off % KV4_B;
-        const unsigned char* blk = kv4_block(c, (int)(slot / c.page_size), head, off / KV4_B);
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(blk + region * 8 * D + kv4_swz((uint32_t)(at * (D / 2) + hl * 4)));
+    const int lane = threadIdx.x & 31, n = c.KV * 2 * LPH, parts = gridDim.y * 32;
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= a.rows) return;
+    const int64_t slot = a.slots[row];
+    if (slot < 0 || slot >= c.pages * (int64_t)c.page_size) return;
+    int page, off;
+    kv4_place(c, slot, page, off);
+    const int at = off % KV4_B;
+    const unsigned char* base = kv4_block(c, page, 0, off / KV4_B);
+    const int64_t head_bytes = (int64_t)(c.page_size / KV4_B) * kv4_block_bytes(D);
+#pragma unroll 4
+    for (int i = blockIdx.y * 32 + lane; i < n; i += parts) {
+        const int hl = i % LPH, region = i / LPH & 1, head = i / (2 * LPH);
+        const unsigned char* blk = base + head * head_bytes;
+        const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(blk + region * 8 * D + kv4_swz((uint32_t)(at * (D / 2) + hl * 4))));
         const __half* sb = reinterpret_cast<const __half*>(blk + (16 + region) * D) + (hl >> 3) * 2 * KV4_B + at;
-        const float s = h2f(sb[0]), b = h2f(sb[KV4_B]);
+        const float s = h2f(__ldg(sb)), b = h2f(__ldg(sb + KV4_B));
         uint4 o; __half* oh = reinterpret_cast<__half*>(&o);
 #pragma unroll
         for (int j = 0; j < 8; ++j) oh[j] = f2h(fmaf((float)(w >> (4 * j) & 15u), s, b));
@@ -176,8 +207,8 @@ int launch_kv4_append(const Kv4Cache& c, const Kv4AppendArgs& a, cudaStream_t st
     return rc;
 }
 int launch_kv4_read(const Kv4Cache& c, const Kv4ReadArgs& a, cudaStream_t st) {
-    const int64_t n = (int64_t)a.rows * c.KV * 2 * (c.D / 8), want = (n + 255) / 256, most = (int64_t)sm_count() * 64;
-    const dim3 grid((unsigned)(want < most ? want : most));
+    const int words = c.KV * 2 * (c.D / 8) / 32 + 1;
+    const dim3 grid((unsigned)((a.rows + 7) / 8), (unsigned)(a.rows < 8 * sm_count() ? (words + 3) / 4 : 1));
     int rc = 0;
     profile_launch("k_kv4_read", st, [&] {
         if (c.D == 64) return rc = launch_pdl(false, k_kv4_read<64>, grid, 256, 0, st, c, a);

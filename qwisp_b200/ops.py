@@ -4,10 +4,12 @@ attnLayerRows: swift/Sources/QwispCore/SeedlessMetalForward.swift:222,
 SeedlessVerifyForward.swift:37-248)."""
 import collections
 import ctypes as C
+import functools
+import struct
 
 import numpy as np
 
-from ._lib import SL_ERR_INVALID, SeedlessError, SlKv4Append, SlKv4Attention, SlKv4Cache, SlKv4Read, SlKvPlan, lib
+from ._lib import SL_ERR_INVALID, SeedlessError, lib
 
 
 def _p(a):
@@ -124,51 +126,64 @@ def sample_rows(engine, logits, draft, inv_t, top_p, seed_lo, seed_hi, base_pos,
 # ---------------------------------------------------------------------------------------------- a KV cache held in 4 bits
 # These take CUDA tensors and run on their device's current stream; nothing is synchronised.  A cache is a uint8 tensor
 # [pages, kv heads, page size / 16, 18 * head dim] (include/seedless_b200.h has the layout); its pages may lie further apart than one
-# page is long (a layer of an arena whose pages hold several).
+# page is long (a layer of an arena whose pages hold several).  A decode step calls three of them per layer, so they are lean: one look
+# at each tensor's type, shape and device here, alignment and ranges in the library, argument blocks packed in one go.
 KvPlan = collections.namedtuple("KvPlan", "kv_len q_start slots pos free_count status")
+_CACHE, _PLAN = struct.Struct("@Pqiiii"), struct.Struct("@PPiiPqiPiPPPPPiPP0q")
+_APPEND, _READ = struct.Struct("@PPPqqqqqqPqqiiPPfPqiifPP0q"), struct.Struct("@PiPPqqqq0q")
+_ATTENTION = struct.Struct("@PqqPqqPqqiiPPiiPqiifPQ0q")
 
 
 def _no(where, what):
     return SeedlessError(SL_ERR_INVALID, where, what)
 
 
-def _call(fn, device, where, *structs):
+@functools.lru_cache(maxsize=1)
+def _cuda():
+    """(current device, current stream of a device) as numbers.  (torch's own accessors where it has them: a Stream object is 1.5 us.)"""
     import torch
-    if device.index == torch.cuda.current_device():
-        rc = fn(*[C.byref(s) for s in structs], torch.cuda.current_stream(device).cuda_stream)
+    return (getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device),
+            getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream))
+
+
+def _call(fn, index, where, *blocks):
+    """The call on the device's current stream."""
+    device, stream = _cuda()
+    if device() == index:
+        rc = fn(*blocks, stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*[C.byref(s) for s in structs], torch.cuda.current_stream(device).cuda_stream)
+        import torch
+        with torch.cuda.device(index):
+            rc = fn(*blocks, stream(index))
     if rc != 0:
         raise SeedlessError(rc, where)
 
 
-def _same(where, device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise _no(where, f"{name} is on {t.device}, the call on {device}")
+def _heads(where, name, t, shape, index):
+    """(pointer, row stride, head stride) of fp16 [rows, heads, dim] on that device."""
+    import torch
+    by = t.stride()
+    if t.dtype is not torch.float16 or t.shape != shape or by[2] != 1 or t.get_device() != index:
+        raise _no(where, f"{name} has to be fp16 {list(shape)} on the cache's device, a head's dims contiguous")
+    return t.data_ptr(), by[0], by[1]
 
 
-def _whole(where, dtype, **tensors):
-    for name, t in tensors.items():
-        if t.dtype != dtype or not t.is_contiguous():
-            raise _no(where, f"{name} has to be contiguous and {dtype}")
-
-
-def _heads(where, name, t, rows, heads, dim):
-    """A tensor [rows, heads, dim] of halves whose heads the kernels can address; None passes."""
-    if t is not None and (str(t.dtype) != "torch.float16" or tuple(t.shape) != (rows, heads, dim) or t.stride(2) != 1 or
-                          t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16):
-        raise _no(where, f"{name} has to be fp16 [{rows}, {heads}, {dim}], a head's dims contiguous and on a 16-byte boundary")
+def _flat(where, name, t, dtype, n, index):
+    """The pointer of a contiguous tensor of n values (None: any number) on that device."""
+    if t.dtype is not dtype or (n is not None and t.shape != (n,)) or not t.is_contiguous() or t.get_device() != index:
+        raise _no(where, f"{name} has to be contiguous {dtype}{'' if n is None else ' [%d]' % n} on the call's device")
+    return t.data_ptr()
 
 
 def _cache(where, cache):
-    pages, kv, blocks, size = cache.shape if cache.dim() == 4 else (0, 0, 0, 0)
-    if str(cache.dtype) != "torch.uint8" or not cache.is_cuda or size not in (18 * 64, 18 * 128, 18 * 256) or not pages * kv * blocks or \
-            cache.stride(3) != 1 or (blocks > 1 and cache.stride(2) != size) or (kv > 1 and cache.stride(1) != blocks * size):
+    """(argument block, page size, kv heads, head dim, device index) of a cache."""
+    import torch
+    shape, by, index = cache.shape, cache.stride(), cache.get_device()
+    if len(shape) != 4 or cache.dtype is not torch.uint8 or index < 0 or shape[3] not in (18 * 64, 18 * 128, 18 * 256) or not cache.numel() or \
+            by[3] != 1 or (by[2] != shape[3] and shape[2] > 1) or (by[1] != shape[2] * shape[3] and shape[1] > 1):
         raise _no(where, "a cache is a CUDA tensor uint8 [pages, kv heads, page size / 16, 18 * head dim] of whole pages")
-    stride = cache.stride(0) if pages > 1 else kv * blocks * size
-    return SlKv4Cache(cache.data_ptr(), stride, pages, blocks * 16, kv, size // 18)
+    pages, kv, blocks, size = shape
+    return _CACHE.pack(cache.data_ptr(), by[0] if pages > 1 else kv * blocks * size, pages, blocks * 16, kv, size // 18), blocks * 16, kv, size // 18, index
 
 
 def kv4_cache(pages, page_size, kv_heads, head_dim, device="cuda"):
@@ -186,25 +201,22 @@ def kv_plan(lens, new_rows, table, free_pages, free_count, page_size, max_rows, 
     requests out of range, rows beyond max_rows): nothing was planned.  out: a KvPlan to write into, whose kv_len may be lens and
     whose free_count may be free_count."""
     import torch
-    where, dev, B = "sl_op_kv_plan_device", lens.device, lens.numel()
-    if not lens.is_cuda or new_rows.shape != (B,) or table.dim() != 2 or table.shape[0] != B or table.dtype != torch.int32 or \
-            (table.numel() and table.stride(1) != 1) or max_rows < 0:
+    where, i32, index = "sl_op_kv_plan_device", torch.int32, lens.get_device()
+    if index < 0 or lens.dim() != 1 or table.dim() != 2 or max_rows < 0:
         raise _no(where, "lens and new_rows are CUDA int32 [B], table int32 [B, pages]")
-    if out is None:
-        i32 = lambda n: torch.empty(n, dtype=torch.int32, device=dev)  # noqa: E731
-        out = KvPlan(i32(B), i32(B + 1), torch.empty(max_rows, dtype=torch.int64, device=dev), i32(max_rows), i32(1), i32(3))
-    elif [t.numel() for t in out] != [B, B + 1, max_rows, max_rows, 1, 3]:
-        raise _no(where, "out has other sizes")
-    _same(where, dev, new_rows=new_rows, table=table, free_pages=free_pages, free_count_in=free_count, **out._asdict())
-    _whole(where, torch.int32, lens=lens, new_rows=new_rows, free_pages=free_pages, free_count_in=free_count, kv_len=out.kv_len, q_start=out.q_start,
-           pos=out.pos, free_count=out.free_count, status=out.status)
-    _whole(where, torch.int64, slots=out.slots)
-    if free_count.numel() != 1:
-        raise _no(where, "free_count is one number")
-    p = SlKvPlan(lens.data_ptr(), new_rows.data_ptr(), B, page_size, table.data_ptr(), max(table.stride(0), table.shape[1]), table.shape[1],
-                 free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), out.kv_len.data_ptr(), out.q_start.data_ptr(),
-                 out.slots.data_ptr(), out.pos.data_ptr(), max_rows, out.free_count.data_ptr(), out.status.data_ptr())
-    _call(lib().sl_op_kv_plan_device, dev, where, p)
+    B, (rows, width), by = lens.shape[0], table.shape, table.stride()
+    if rows != B or table.dtype is not i32 or (by[1] != 1 and width > 1) or table.get_device() != index:
+        raise _no(where, f"table has to be int32 [{B}, pages] on the call's device")
+    at = [_flat(where, "lens", lens, i32, B, index), _flat(where, "new_rows", new_rows, i32, B, index), _flat(where, "free_pages", free_pages, i32, None, index),
+          _flat(where, "free_count", free_count, i32, 1, index)]
+    if out is None:                                                        # one allocation
+        buf = torch.empty(3 * max_rows + 2 * B + 5, dtype=i32, device=lens.device)
+        slots, kv_len, q_start, pos, count, status = buf.split((2 * max_rows, B, B + 1, max_rows, 1, 3))
+        out, p, n = KvPlan(kv_len, q_start, slots.view(torch.int64), pos, count, status), buf.data_ptr(), 8 * max_rows
+        to = (p + n, p + n + 4 * B, p, p + n + 8 * B + 4, p + n + 8 * B + 4 + 4 * max_rows, p + n + 8 * B + 8 + 4 * max_rows)
+    else:
+        to = [_flat(where, name + " out", t, torch.int64 if name == "slots" else i32, n, index) for name, t, n in zip(KvPlan._fields, out, (B, B + 1, max_rows, max_rows, 1, 3))]
+    _call(lib().sl_op_kv_plan_device, index, where, _PLAN.pack(at[0], at[1], B, page_size, table.data_ptr(), max(by[0], width), width, at[2], free_pages.shape[0], at[3], *to[:4], max_rows, *to[4:]))
     return out
 
 
@@ -214,38 +226,45 @@ def kv4_append(cache, slots, q=None, k=None, v=None, *, q_norm=None, k_norm=None
     heads, dim] fp16; pos int32 [rows] or [axes, rows], axis_of: the position axis of each of the rope_dims / 2 frequencies (None: the
     first).  Returns the rotated queries (q_out, which may be q; None without q).  Rows whose slot is not one of the cache's are padding."""
     import torch
-    where, c = "sl_op_kv4_append_device", _cache("sl_op_kv4_append_device", cache)
-    dev, dim = cache.device, c.head_dim
+    where = "sl_op_kv4_append_device"
+    block, _, kv, dim, index = _cache(where, cache)
     if (k is None) != (v is None) or (q is None and k is None):
         raise _no(where, "k and v come together, or queries alone")
-    rows, heads = (q if q is not None else k).shape[0], 0 if q is None else q.shape[1]
-    if q is not None and q_out is None:
-        q_out = torch.empty((rows, heads, dim), dtype=torch.float16, device=dev)
-    for name, t, n in (("q", q, heads), ("q_out", q_out, heads), ("k", k, c.kv_heads), ("v", v, c.kv_heads)):
-        _heads(where, name, t, rows, n, dim)
-    for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if t is not None and (t.dtype != torch.float16 or tuple(t.shape) != (dim,) or not t.is_contiguous() or t.data_ptr() % 16):
-            raise _no(where, f"{name} has to be fp16 [{dim}]")
-    if slots is None and k is not None:
-        raise _no(where, "k and v need slots")
-    if slots is not None and (slots.dtype != torch.int64 or tuple(slots.shape) != (rows,) or not slots.is_contiguous()):
-        raise _no(where, f"slots has to be contiguous int64 [{rows}]")
-    axes, table = 0, None
+    qa = oa = ka = va = (0, 0, 0)
+    heads, axes, pa, apart, table, sa, qn, kn = 0, 0, 0, 0, 0, 0, 0, 0
+    rows = (k if q is None else q).shape[0]
+    if q is not None:
+        heads = q.shape[1] if q.dim() == 3 else 0
+        qa = _heads(where, "q", q, (rows, heads, dim), index)
+        if q_out is None:
+            q_out = torch.empty((rows, heads, dim), dtype=torch.float16, device=q.device)
+        oa = _heads(where, "q_out", q_out, (rows, heads, dim), index)
+    if k is not None:
+        ka, va = _heads(where, "k", k, (rows, kv, dim), index), _heads(where, "v", v, (rows, kv, dim), index)
+        if slots is None:
+            raise _no(where, "k and v need slots")
+    if q_norm is not None:
+        qn = _flat(where, "q_norm", q_norm, torch.float16, dim, index)
+    if k_norm is not None:
+        kn = _flat(where, "k_norm", k_norm, torch.float16, dim, index)
+    if slots is not None:
+        sa = _flat(where, "slots", slots, torch.int64, rows, index)
     if rope_dims:
-        if pos is None or pos.dtype != torch.int32 or pos.shape[-1] != rows or pos.dim() not in (1, 2) or (rows > 1 and pos.stride(-1) != 1):
-            raise _no(where, f"pos has to be int32 [{rows}] or [axes, {rows}]")
-        axes = 1 if pos.dim() == 1 else pos.shape[0]
+        if pos is None or pos.dtype is not torch.int32 or pos.dim() not in (1, 2) or pos.shape[-1] != rows or (pos.stride(-1) != 1 and rows > 1) or pos.get_device() != index:
+            raise _no(where, f"pos has to be int32 [{rows}] or [axes, {rows}] on the call's device")
+        axes, apart = (1, 0) if pos.dim() == 1 else (pos.shape[0], pos.stride(0))
+        pa = pos.data_ptr()
         if axis_of is not None:
-            if len(axis_of) != rope_dims // 2 or not all(0 <= i < min(axes, 256) for i in axis_of):
+            try:
+                table = bytes(axis_of)
+            except (TypeError, ValueError):
+                table = b""
+            if len(table) != rope_dims // 2:
                 raise _no(where, f"axis_of has one of {axes} axes for each of {rope_dims // 2} frequencies")
-            table = bytes(axis_of)
-    _same(where, dev, q=q, k=k, v=v, q_out=q_out, q_norm=q_norm, k_norm=k_norm, pos=pos, slots=slots)
-    at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    by = lambda t: (0, 0) if t is None else (t.stride(0), t.stride(1))  # noqa: E731
-    p = SlKv4Append(at(q), at(k), at(v), *by(q), *by(k), *by(v), at(q_out), *by(q_out), rows, heads, at(q_norm), at(k_norm), eps,
-                    at(pos) if rope_dims else None, pos.stride(0) if rope_dims and pos.dim() == 2 else 0, axes, rope_dims, rope_theta, table, at(slots))
+            table = C.create_string_buffer(table, max(1, len(table)))      # (lives until the call returns)
     if rows:
-        _call(lib().sl_op_kv4_append_device, dev, where, c, p)
+        _call(lib().sl_op_kv4_append_device, index, where, block, _APPEND.pack(qa[0], ka[0], va[0], qa[1], qa[2], ka[1], ka[2], va[1], va[2], *oa, rows, heads, qn, kn, eps,
+                                                                             pa, apart, axes, rope_dims, rope_theta, C.addressof(table) if table else 0, sa))
     return q_out
 
 
@@ -253,20 +272,22 @@ def kv4_read(cache, slots, k=None, v=None):
     """K and V at slots int64 [rows] as fp16 [rows, kv heads, dim] (into k and v if given).  Rows whose slot is not one of the
     cache's stay as they were."""
     import torch
-    where, c = "sl_op_kv4_read_device", _cache("sl_op_kv4_read_device", cache)
-    if slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
-        raise _no(where, "slots has to be contiguous int64 [rows]")
-    shape = (slots.numel(), c.kv_heads, c.head_dim)
-    k, v = (torch.empty(shape, dtype=torch.float16, device=cache.device) if t is None else t for t in (k, v))
-    _heads(where, "k", k, *shape)
-    _heads(where, "v", v, *shape)
-    _same(where, cache.device, slots=slots, k=k, v=v)
-    p = SlKv4Read(slots.data_ptr(), shape[0], k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1))
-    if shape[0]:
-        _call(lib().sl_op_kv4_read_device, cache.device, where, c, p)
+    where = "sl_op_kv4_read_device"
+    block, _, kv, dim, index = _cache(where, cache)
+    rows = slots.shape[0] if slots.dim() == 1 else -1
+    sa = _flat(where, "slots", slots, torch.int64, rows, index)
+    shape = (rows, kv, dim)
+    if k is None:
+        k = torch.empty(shape, dtype=torch.float16, device=cache.device)
+    if v is None:
+        v = torch.empty_like(k) if k.is_contiguous() else torch.empty(shape, dtype=torch.float16, device=cache.device)
+    (kp, *kb), (vp, *vb) = _heads(where, "k", k, shape, index), _heads(where, "v", v, shape, index)
+    if rows:
+        _call(lib().sl_op_kv4_read_device, index, where, block, _READ.pack(sa, rows, kp, vp, *kb, *vb))
     return k, v
 
 
+@functools.lru_cache(maxsize=256)
 def kv4_attention_workspace(q_heads, kv_heads, head_dim, batch, max_q, rows):
     """Bytes of workspace of such a call of kv4_attention."""
     n = lib().sl_kv4_attention_workspace(q_heads, kv_heads, head_dim, batch, max_q, rows)
@@ -281,27 +302,29 @@ def kv4_attention(cache, table, kv_len, q, q_start, max_q, *, causal=True, scale
     None.  A row that sees no position is zero.  workspace: a uint8 tensor of kv4_attention_workspace() bytes, allocated for the call
     if None; calls that may run at the same time need one each."""
     import torch
-    where, c = "sl_op_kv4_attention_device", _cache("sl_op_kv4_attention_device", cache)
-    dev, dim, B = cache.device, c.head_dim, kv_len.numel()
-    if q.dim() != 3 or table.dim() != 2 or table.shape[0] != B or table.dtype != torch.int32 or (table.numel() and table.stride(1) != 1) or \
-            q_start.numel() != B + 1 or max_q < 1:
+    where, i32 = "sl_op_kv4_attention_device", torch.int32
+    block, _, kv, dim, index = _cache(where, cache)
+    if q.dim() != 3 or table.dim() != 2 or kv_len.dim() != 1 or max_q < 1:
         raise _no(where, "q is [rows, heads, dim], table int32 [B, pages], kv_len int32 [B], q_start int32 [B + 1]")
-    rows, heads = q.shape[:2]
+    shape, B, by = q.shape, kv_len.shape[0], table.stride()
+    rows, heads = shape[0], shape[1]
+    width = table.shape[1]
+    if table.shape[0] != B or table.dtype is not i32 or (by[1] != 1 and width > 1) or table.get_device() != index:
+        raise _no(where, f"table has to be int32 [{B}, pages] on the call's device")
+    qa = _heads(where, "q", q, (rows, heads, dim), index)
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=torch.float16, device=dev)
-    for name, t in (("q", q), ("gate", gate), ("out", out)):
-        _heads(where, name, t, rows, heads, dim)
-    _whole(where, torch.int32, kv_len=kv_len, q_start=q_start)
-    need = kv4_attention_workspace(heads, c.kv_heads, dim, B, max_q, rows)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=torch.float16, device=q.device)
+    oa = _heads(where, "out", out, shape, index)
+    ga = (0, 0, 0) if gate is None else _heads(where, "gate", gate, shape, index)
+    la, ra = _flat(where, "kv_len", kv_len, i32, B, index), _flat(where, "q_start", q_start, i32, B + 1, index)
+    need = kv4_attention_workspace(heads, kv, dim, B, max_q, rows)
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
-        raise _no(where, f"workspace has to be contiguous uint8 of {need} bytes")
-    _same(where, dev, table=table, kv_len=kv_len, q=q, q_start=q_start, gate=gate, out=out, workspace=workspace)
-    g = (None, 0, 0) if gate is None else (gate.data_ptr(), gate.stride(0), gate.stride(1))
-    p = SlKv4Attention(q.data_ptr(), q.stride(0), q.stride(1), *g, out.data_ptr(), out.stride(0), out.stride(1), rows, heads,
-                       q_start.data_ptr(), kv_len.data_ptr(), B, max_q, table.data_ptr(), max(table.stride(0), table.shape[1]), table.shape[1],
-                       1 if causal else 0, dim ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.numel())
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif workspace.numel() < need:
+        raise _no(where, f"workspace has to have {need} bytes")
+    wa = _flat(where, "workspace", workspace, torch.uint8, None, index)
     if rows:
-        _call(lib().sl_op_kv4_attention_device, dev, where, c, p)
+        _call(lib().sl_op_kv4_attention_device, index, where, block,
+              _ATTENTION.pack(*qa, *ga, *oa, rows, heads, ra, la, B, max_q, table.data_ptr(), max(by[0], width), width, 1 if causal else 0,
+                              dim ** -0.5 if scale is None else scale, wa, workspace.numel()))
     return out

@@ -130,3 +130,16 @@ def test_tensors_on_the_host_are_refused():
         with pytest.raises(Q.SeedlessError) as e:
             f()
         assert e.value.code == INVALID
+
+
+def test_packed_argument_blocks_are_the_structures():
+    """The wrappers pack an argument block's bytes in one go: every field lands where the structure has it."""
+    from qwisp_b200 import ops
+    for fmt, s in ((ops._CACHE, _lib.SlKv4Cache), (ops._PLAN, _lib.SlKvPlan), (ops._APPEND, _lib.SlKv4Append), (ops._READ, _lib.SlKv4Read),
+                   (ops._ATTENTION, _lib.SlKv4Attention)):
+        assert fmt.size == C.sizeof(s)
+        values = [0.5 * i if t is C.c_float else i + 1 for i, (_, t) in enumerate(s._fields_)]
+        got = s.from_buffer_copy(fmt.pack(*values))
+        for (name, t), v in zip(s._fields_, values):
+            w = C.c_void_p.from_buffer(got, getattr(s, name).offset).value if t is C.c_char_p else getattr(got, name)
+            assert w == v, (s, name)
