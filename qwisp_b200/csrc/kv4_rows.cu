@@ -69,22 +69,16 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 8) k_kv4_append(Kv4Cache c, Kv4
     const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hl = lane % LPH, hs = lane / LPH;
     const int64_t slot = a.slots ? a.slots[row] : 0;
     if (a.slots && (slot < 0 || slot >= c.pages * (int64_t)c.page_size)) return;         // padding
-    const int nk = a.k ? (c.KV + HPW - 1) / HPW : 0, tasks = 2 * nk + (a.q ? (a.NH + HPW - 1) / HPW : 0), stride = gridDim.y * KA_WARPS;
-    struct Task { int kind, head; bool have; };               // kind: 0 = K, 1 = V, 2 = query
-    auto task_of = [&](int i) {
-        Task t;
-        t.kind = i < nk ? 0 : i < 2 * nk ? 1 : 2;
-        t.head = (i - t.kind * nk) * HPW + hs;
-        t.have = i < tasks && t.head < (t.kind == 2 ? a.NH : c.KV);
-        return t;
+    // tasks: nk of K, nk of V, then the queries'; this warp's are g0, g0 + stride, ..
+    const int nk = a.k ? (c.KV + HPW - 1) / HPW : 0, nq = a.q ? (a.NH + HPW - 1) / HPW : 0, stride = gridDim.y * KA_WARPS, g0 = blockIdx.y * KA_WARPS + warp;
+    auto from = [&](int first) { return first <= g0 ? g0 - first : (stride - (first - g0) % stride) % stride; };      // the warp's first of a kind
+    const int k0 = from(0), v0 = from(nk), q0 = from(2 * nk);
+    auto load = [&](const __half* src, int64_t by_head, int task, int heads) {
+        const int head = task * HPW + hs;
+        return head < heads ? reinterpret_cast<const uint4*>(src + head * by_head)[hl] : make_uint4(0, 0, 0, 0);
     };
-    auto load = [&](const Task& t) {
-        const __half* src = t.kind == 0 ? a.k + row * a.k_row + t.head * a.k_head : t.kind == 1 ? a.v + row * a.v_row + t.head * a.v_head : a.q + row * a.q_row + t.head * a.q_head;
-        return t.have ? reinterpret_cast<const uint4*>(src)[hl] : make_uint4(0, 0, 0, 0);
-    };
-    int i = blockIdx.y * KA_WARPS + warp;
-    Task task = task_of(i);
-    uint4 raw = load(task);
+    const __half *ksrc = a.k + row * a.k_row, *vsrc = a.v + row * a.v_row, *qsrc = a.q + row * a.q_row;
+    uint4 kraw = load(ksrc, a.k_head, k0, a.k ? c.KV : 0), vraw = load(vsrc, a.v_head, v0, a.k ? c.KV : 0), qraw = load(qsrc, a.q_head, q0, a.q ? a.NH : 0);
     const int half = a.rope >> 1;
     auto put = [&](int d, double cs, double sn) {
         s_d[d & 7][d >> 3] = make_double2(cs, sn);
@@ -99,68 +93,88 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 8) k_kv4_append(Kv4Cache c, Kv4
     for (int d = a.rope + tid; d < D; d += KA_WARPS * 32) put(d, 1.0, 0.0);
     __syncthreads();
     const int partner = hl * 8 >= a.rope ? lane : hl * 8 < half ? lane + a.rope / 16 : lane - a.rope / 16;      // has the dims these are rotated with
-    int pg = 0, off = 0;
-    if (nk) kv4_place(c, slot, pg, off);
-    const int at = off % KV4_B;
-    unsigned char* page = kv4_block(c, pg, 0, off / KV4_B);   // (head 0's block)
-    const int64_t head_bytes = (int64_t)(c.page_size / KV4_B) * kv4_block_bytes(D);
-    for (; i < tasks; i += stride) {
-        const Task now = task;
-        const uint4 cur = raw;
-        task = task_of(i + stride);
-        raw = load(task);
-        const __half* h = reinterpret_cast<const __half*>(&cur);
+    auto halves = [](const uint4& v, float x[8]) {
+        const __half2* h = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { const float2 f = __half22float2(h[k]); x[2 * k] = f.x; x[2 * k + 1] = f.y; }
+    };
+    auto weight = [&](const __half* w, float x[8]) { halves(w ? reinterpret_cast<const uint4*>(w)[hl] : make_uint4(0, 0, 0, 0), x); };
+    if (nk) {
+        int pg, off;
+        kv4_place(c, slot, pg, off);
+        const int at = off % KV4_B;
+        unsigned char* blk = kv4_block(c, pg, 0, off / KV4_B);               // (head 0's)
+        const int64_t head_bytes = (int64_t)(c.page_size / KV4_B) * kv4_block_bytes(D);
+        for (int t = k0; t < nk; t += stride) {
+            const int head = t * HPW + hs;
+            float x[8];
+            halves(kraw, x);
+            kraw = load(ksrc, a.k_head, t + stride, c.KV);
+            if (a.k_norm || a.rope) {
+                double y[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) y[k] = (double)x[k];
+                if (a.k_norm) {
+                    float w[8];
+                    weight(a.k_norm, w);
+                    double ss = 0.0;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) ss = fma(y[k], y[k], ss);
+#pragma unroll
+                    for (int d = 1; d < LPH; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+                    const double inv = rsqrt(fma(ss, 1.0 / D, (double)a.eps));
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) y[k] = (double)(x[k] * w[k]) * inv;      // (two halves' product: exact in 32 bits)
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const double2 cs = s_d[k][hl];
+                    const double other = __shfl_sync(0xffffffffu, y[k], partner);
+                    x[k] = h2f(f2h((float)fma(other, cs.y, y[k] * cs.x)));
+                }
+            }
+            kv4_store(c, blk + head * head_bytes, at, 0, hl, x, head < c.KV);
+        }
+        for (int t = v0; t < nk; t += stride) {
+            const int head = t * HPW + hs;
+            float x[8];
+            halves(vraw, x);
+            vraw = load(vsrc, a.v_head, t + stride, c.KV);
+            kv4_store(c, blk + head * head_bytes, at, 1, hl, x, head < c.KV);
+        }
+    }
+    if (q0 >= nq) return;
+    float w[8], cs[8], sn[8];
+    weight(a.q_norm, w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float4 f = *reinterpret_cast<const float4*>(s_f[j][hl]);
+        cs[2 * j] = f.x; sn[2 * j] = f.y; cs[2 * j + 1] = f.z; sn[2 * j + 1] = f.w;
+    }
+    __half* dst = a.q_out + row * a.o_row;
+    for (int t = q0; t < nq; t += stride) {
+        const int head = t * HPW + hs;
         float x[8];
+        halves(qraw, x);
+        qraw = load(qsrc, a.q_head, t + stride, a.NH);
+        if (a.q_norm) {
+            float ss = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = h2f(h[k]);
-        const __half* w = now.kind == 0 ? a.k_norm : now.kind == 2 ? a.q_norm : nullptr;
-        uint4 wraw = make_uint4(0, 0, 0, 0);
-        if (w) wraw = reinterpret_cast<const uint4*>(w)[hl];
-        const __half* wh = reinterpret_cast<const __half*>(&wraw);
-        if (now.kind == 2) {
-            if (w) {
-                float ss = 0.f;
+            for (int k = 0; k < 8; ++k) ss = fmaf(x[k], x[k], ss);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) ss = fmaf(x[k], x[k], ss);
+            for (int d = 1; d < LPH; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+            const float inv = rsqrtf(fmaf(ss, 1.0f / D, a.eps));
 #pragma unroll
-                for (int d = 1; d < LPH; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-                const float inv = __frsqrt_rn(fmaf(ss, 1.0f / D, a.eps));
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] = x[k] * inv * h2f(wh[k]);
-            }
-            uint4 o; uint32_t* ow = reinterpret_cast<uint32_t*>(&o);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float4 cs = *reinterpret_cast<const float4*>(s_f[j][hl]);
-                const float u = __shfl_sync(0xffffffffu, x[2 * j], partner), v = __shfl_sync(0xffffffffu, x[2 * j + 1], partner);
-                const __half2 y = __floats2half2_rn(fmaf(u, cs.y, x[2 * j] * cs.x), fmaf(v, cs.w, x[2 * j + 1] * cs.z));
-                ow[j] = *reinterpret_cast<const uint32_t*>(&y);
-            }
-            if (now.have) reinterpret_cast<uint4*>(a.q_out + row * a.o_row + now.head * a.o_head)[hl] = o;
-            continue;
+            for (int k = 0; k < 8; ++k) x[k] = x[k] * w[k] * inv;
         }
-        if (now.kind == 0 && (w || a.rope)) {
-            double y[8];
+        uint4 o; uint32_t* ow = reinterpret_cast<uint32_t*>(&o);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] = (double)x[k];
-            if (w) {
-                double ss = 0.0;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) ss = fma(y[k], y[k], ss);
-#pragma unroll
-                for (int d = 1; d < LPH; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-                const double inv = rsqrt(fma(ss, 1.0 / D, (double)a.eps));
-#pragma unroll
-                for (int k = 0; k < 8; ++k) y[k] = y[k] * inv * (double)h2f(wh[k]);
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const double2 cs = s_d[k][hl];
-                const double other = __shfl_sync(0xffffffffu, y[k], partner);
-                x[k] = h2f(f2h((float)fma(other, cs.y, y[k] * cs.x)));
-            }
+        for (int j = 0; j < 4; ++j) {
+            const float u = __shfl_sync(0xffffffffu, x[2 * j], partner), v = __shfl_sync(0xffffffffu, x[2 * j + 1], partner);
+            const __half2 y = __floats2half2_rn(fmaf(u, sn[2 * j], x[2 * j] * cs[2 * j]), fmaf(v, sn[2 * j + 1], x[2 * j + 1] * cs[2 * j + 1]));
+            ow[j] = *reinterpret_cast<const uint32_t*>(&y);
         }
-        kv4_store(c, page + now.head * head_bytes, at, now.kind, hl, x, now.have);
+        if (head < a.NH) reinterpret_cast<uint4*>(dst + head * a.o_head)[hl] = o;
     }
 }
 

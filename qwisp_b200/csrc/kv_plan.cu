@@ -12,10 +12,8 @@
 
 namespace sl {
 
-constexpr int PLAN_T = 1024;             // threads, and requests of a chunk
-constexpr int PLAN_ROWS = 8192;
+constexpr int PLAN_ROWS = 8192, PLAN_FIND = 2048;      // rows that one CTA does; requests whose offsets the rows' kernel keeps in shared memory
 
-struct PlanSums { long long rows; int back, grown, bad; };
 struct PlanOne { long long len; int rows, have, need; bool ended, bad; };
 
 __device__ __forceinline__ PlanOne plan_one(const KvPlanArgs& a, int b) {
@@ -29,7 +27,8 @@ __device__ __forceinline__ PlanOne plan_one(const KvPlanArgs& a, int b) {
     else { r.have = (int)have; r.need = r.ended ? 0 : (int)need; }
     return r;
 }
-// inclusive sums over the CTA of two values; all threads call it
+// inclusive sums over the CTA of two values, the totals in ws[.][last warp]; all threads call it
+template <int T>
 __device__ __forceinline__ void plan_scan(int& x, int& y, int (*ws)[32]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -37,12 +36,13 @@ __device__ __forceinline__ void plan_scan(int& x, int& y, int (*ws)[32]) {
         const int u = __shfl_up_sync(0xffffffffu, x, d), v = __shfl_up_sync(0xffffffffu, y, d);
         if (lane >= d) { x += u; y += v; }
     }
+    __syncthreads();
     if (lane == 31) { ws[0][warp] = x; ws[1][warp] = y; }
     __syncthreads();
     if (warp == 0) {
-        int u = ws[0][lane], v = ws[1][lane];
+        int u = lane < T / 32 ? ws[0][lane] : 0, v = lane < T / 32 ? ws[1][lane] : 0;
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
+        for (int d = 1; d < T / 32; d <<= 1) {
             const int p = __shfl_up_sync(0xffffffffu, u, d), q = __shfl_up_sync(0xffffffffu, v, d);
             if (lane >= d) { u += p; v += q; }
         }
@@ -50,53 +50,49 @@ __device__ __forceinline__ void plan_scan(int& x, int& y, int (*ws)[32]) {
     }
     __syncthreads();
     if (warp) { x += ws[0][warp - 1]; y += ws[1][warp - 1]; }
-    __syncthreads();
 }
-// the last i of [0, n) with start[i] <= v (start[0] <= v)
+// the last i of [0, n) with start[i] <= v (start[0] <= v); of entries that start alike the last is the one that is not empty
 __device__ __forceinline__ int plan_find(const int* start, int n, int v) {
     int lo = 0, hi = n - 1;
     while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (start[mid] <= v) lo = mid; else hi = mid - 1; }
     return lo;
 }
-__device__ __forceinline__ void plan_row(const KvPlanArgs& a, int r, int total) {
-    int64_t slot = -1; int pos = 0;
-    if (r < total) {
-        const int b = plan_find(a.q_start, a.batch, r);       // (requests without rows share the next one's offset: the last is meant)
-        pos = a.kv_len[b] - (a.q_start[b + 1] - r);
-        slot = (int64_t)a.table[(int64_t)b * a.table_stride + pos / a.page_size] * a.page_size + pos % a.page_size;
-    }
-    a.slots[r] = slot; a.pos[r] = pos;
+__device__ __forceinline__ void plan_row(const KvPlanArgs& a, int r, int b, int pos) {
+    a.slots[r] = (int64_t)a.table[(int64_t)b * a.table_stride + pos / a.page_size] * a.page_size + pos % a.page_size;
+    a.pos[r] = pos;
 }
 
-__global__ void __launch_bounds__(PLAN_T) k_kv_plan(KvPlanArgs a, int rows_here) {
-    __shared__ int ws[2][32], s_back[PLAN_T], s_grown[PLAN_T], s_have[PLAN_T];
+// T: threads, and requests of a chunk
+template <int T>
+__global__ void __launch_bounds__(T) k_kv_plan(KvPlanArgs a, int rows_here) {
+    __shared__ int ws[2][32], s_a[T], s_b[T], s_c[T], s_tot[3];
     __shared__ unsigned long long s_rows;
-    __shared__ int s_tot[3];
-    const int tid = threadIdx.x;
+    constexpr int TOP = T / 32 - 1;
+    const int tid = threadIdx.x, lane = tid & 31;
+    pdl_launch_dependents();
     if (tid == 0) { s_rows = 0; s_tot[0] = s_tot[1] = s_tot[2] = 0; }
-    __syncthreads();
-    // ---- what the whole step needs
+    // ---- what the whole step needs (warps' sums first: a thousand atomic additions of one word took 18 us)
     const int F = *a.free_count;
-    PlanOne mine = plan_one(a, tid);
-    {
-        long long rows = 0, back = 0, grown = 0; int bad = 0;
-        for (int b = tid; b < a.batch; b += PLAN_T) {
-            const PlanOne r = b == tid ? mine : plan_one(a, b);
-            rows += r.rows; bad += r.bad;
-            if (r.ended) back += r.have; else grown += r.need - r.have;
-        }
-        // (pages and requests number below 2^31 in all: what a table of int32 pages can hold)
+    const PlanOne mine = plan_one(a, tid);
+    long long rows = 0; int back = 0, grown = 0, bad = 0;
+    for (int b = tid; b < a.batch; b += T) {
+        const PlanOne r = b == tid ? mine : plan_one(a, b);
+        rows += r.rows; bad += r.bad;
+        if (r.ended) back += r.have; else grown += r.need - r.have;
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) rows += __shfl_xor_sync(0xffffffffu, rows, d);
+    back = __reduce_add_sync(0xffffffffu, back); grown = __reduce_add_sync(0xffffffffu, grown); bad = __reduce_add_sync(0xffffffffu, bad);
+    __syncthreads();
+    if (lane == 0) {                     // (pages number below 2^31 in all: the host has looked)
         atomicAdd(&s_rows, (unsigned long long)rows);
-        if (back) atomicAdd(&s_tot[0], (int)back);
-        if (grown) atomicAdd(&s_tot[1], (int)grown);
-        if (bad) atomicAdd(&s_tot[2], bad);
+        atomicAdd(&s_tot[0], back); atomicAdd(&s_tot[1], grown); atomicAdd(&s_tot[2], bad);
     }
     __syncthreads();
-    const long long rows = (long long)s_rows;
-    const int back = s_tot[0], grown = s_tot[1];
+    rows = (long long)s_rows; back = s_tot[0]; grown = s_tot[1];
     const bool stack_bad = F < 0 || (long long)F + back > a.free_cap;
     const long long top = (long long)F + back;
-    const int bad = s_tot[2] + (stack_bad ? 1 : 0);
+    bad = s_tot[2] + (stack_bad ? 1 : 0);
     const long long shrt = stack_bad || grown <= top ? 0 : grown - top, over = rows > a.max_rows ? rows - a.max_rows : 0;
     const bool fine = !bad && !shrt && !over;
     if (tid == 0) {
@@ -105,63 +101,90 @@ __global__ void __launch_bounds__(PLAN_T) k_kv_plan(KvPlanArgs a, int rows_here)
         a.q_start[a.batch] = fine ? (int)rows : 0;
     }
     if (!fine) {
-        for (int b = tid; b < a.batch; b += PLAN_T) { const int len = a.lens[b]; a.q_start[b] = 0; a.kv_len[b] = len; }
-        for (int r = tid; rows_here && r < a.max_rows; r += PLAN_T) { a.slots[r] = -1; a.pos[r] = 0; }
+        for (int b = tid; b < a.batch; b += T) { const int len = a.lens[b]; a.q_start[b] = 0; a.kv_len[b] = len; }
+        for (int r = tid; rows_here && r < a.max_rows; r += T) { a.slots[r] = -1; a.pos[r] = 0; }
         return;
     }
     // ---- pages of ended requests onto the stack
     if (back) {
         int base = F;
-        for (int b0 = 0; b0 < a.batch; b0 += PLAN_T) {
+        for (int b0 = 0; b0 < a.batch; b0 += T) {
             const PlanOne r = b0 ? plan_one(a, b0 + tid) : mine;
-            int x = r.ended ? r.have : 0, y = 0;
-            const int own = x;
-            plan_scan(x, y, ws);
-            s_back[tid] = x - own;
+            const int own = r.ended ? r.have : 0;
+            int x = own, y = 0;
+            plan_scan<T>(x, y, ws);
+            s_a[tid] = x - own;
             __syncthreads();
-            const int n = ws[0][31];
-            for (int i = tid; i < n; i += PLAN_T) {
-                const int j = plan_find(s_back, PLAN_T, i);
-                a.free_pages[base + i] = a.table[(int64_t)(b0 + j) * a.table_stride + i - s_back[j]];
+            const int n = ws[0][TOP];
+#pragma unroll 4
+            for (int i = tid; i < n; i += T) {
+                const int j = plan_find(s_a, T, i);
+                a.free_pages[base + i] = a.table[(int64_t)(b0 + j) * a.table_stride + i - s_a[j]];
             }
             base += n;
-            __syncthreads();
         }
+        __syncthreads();
     }
-    // ---- row offsets, new lengths, pages off the stack
+    // ---- row offsets, new lengths, pages off the stack, and the rows
     int row0 = 0, taken = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += PLAN_T) {
+    for (int b0 = 0; b0 < a.batch; b0 += T) {
         const PlanOne r = b0 ? plan_one(a, b0 + tid) : mine;
         const int own = r.ended ? 0 : r.need - r.have;
         int x = r.rows, y = own;
-        plan_scan(x, y, ws);
-        s_grown[tid] = y - own; s_have[tid] = r.have;
+        plan_scan<T>(x, y, ws);
+        s_a[tid] = y - own; s_b[tid] = r.have;
         if (b0 + tid < a.batch) {
             a.q_start[b0 + tid] = row0 + x - r.rows;
             a.kv_len[b0 + tid] = r.ended ? 0 : (int)r.len + r.rows;           // (may be the array of lengths: its reader was this thread)
         }
         __syncthreads();
-        const int n = ws[1][31];
-        for (int i = tid; i < n; i += PLAN_T) {
-            const int j = plan_find(s_grown, PLAN_T, i);
-            a.table[(int64_t)(b0 + j) * a.table_stride + s_have[j] + i - s_grown[j]] = a.free_pages[top - 1 - taken - i];
+        const int n = ws[1][TOP], m = ws[0][TOP];
+#pragma unroll 4
+        for (int i = tid; i < n; i += T) {
+            const int j = plan_find(s_a, T, i);
+            a.table[(int64_t)(b0 + j) * a.table_stride + s_b[j] + i - s_a[j]] = a.free_pages[top - 1 - taken - i];
         }
-        row0 += ws[0][31]; taken += n;
+        if (rows_here) {
+            s_c[tid] = x - r.rows;
+            __syncthreads();                                                  // (also: the table's new pages are there, s_b is read)
+            s_b[tid] = (int)r.len;
+            __syncthreads();
+#pragma unroll 4
+            for (int i = tid; i < m; i += T) {
+                const int j = plan_find(s_c, T, i);
+                plan_row(a, row0 + i, b0 + j, s_b[j] + i - s_c[j]);
+            }
+        }
+        row0 += m; taken += n;
         __syncthreads();
     }
-    if (rows_here) for (int r = tid; r < a.max_rows; r += PLAN_T) plan_row(a, r, (int)rows);
+    if (rows_here) for (int r = (int)rows + tid; r < a.max_rows; r += T) { a.slots[r] = -1; a.pos[r] = 0; }
 }
+// the rows, four a thread: which request a row is of by bisection of the offsets
 __global__ void __launch_bounds__(256) k_kv_plan_rows(KvPlanArgs a) {
+    __shared__ int s_start[PLAN_FIND];
     pdl_wait();
-    const int r = blockIdx.x * 256 + threadIdx.x;
-    if (r < a.max_rows) plan_row(a, r, a.q_start[a.batch]);
+    const int rows = a.q_start[a.batch];
+    const bool near = a.batch <= PLAN_FIND;
+    if (near) for (int b = threadIdx.x; b < a.batch; b += 256) s_start[b] = a.q_start[b];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = blockIdx.x * 1024 + i * 256 + threadIdx.x;
+        if (r >= a.max_rows) return;
+        if (r >= rows) { a.slots[r] = -1; a.pos[r] = 0; continue; }
+        const int b = near ? plan_find(s_start, a.batch, r) : plan_find(a.q_start, a.batch, r);
+        plan_row(a, r, b, a.kv_len[b] - (a.q_start[b + 1] - r));
+    }
 }
 
 int launch_kv_plan(const KvPlanArgs& a, cudaStream_t st) {
-    const bool here = a.max_rows <= PLAN_ROWS;
+    const bool here = a.max_rows <= PLAN_ROWS, small = a.batch <= 256 && a.max_rows <= 1024;
     int rc = 0;
-    profile_launch("k_kv_plan", st, [&] { return rc = launch_pdl(false, k_kv_plan, dim3(1), PLAN_T, 0, st, a, here ? 1 : 0); });
-    if (rc == 0 && !here) profile_launch("k_kv_plan_rows", st, [&] { return rc = launch_pdl(false, k_kv_plan_rows, dim3((unsigned)((a.max_rows + 255) / 256)), 256, 0, st, a); });
+    profile_launch("k_kv_plan", st, [&] {
+        return rc = small ? launch_pdl(false, k_kv_plan<256>, dim3(1), 256, 0, st, a, 1) : launch_pdl(false, k_kv_plan<1024>, dim3(1), 1024, 0, st, a, here ? 1 : 0);
+    });
+    if (rc == 0 && !here) profile_launch("k_kv_plan_rows", st, [&] { return rc = launch_pdl(true, k_kv_plan_rows, dim3((unsigned)((a.max_rows + 1023) / 1024)), 256, 0, st, a); });
     return rc;
 }
 
