@@ -52,6 +52,11 @@ __device__ __forceinline__ void kp_st32(uint32_t t, const uint32_t* r) {
                    "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
                    "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
+__device__ __forceinline__ void kp_st16(uint32_t t, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+                   "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
 __device__ __forceinline__ void kp_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void kp_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void kp_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -82,7 +87,7 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
     constexpr uint32_t S0 = NQ * D, Q0 = S0 + 2 * KP_N;                       // columns of tensor memory: outputs, scores, queries
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    __shared__ __align__(8) uint64_t k_full[KP_ST], k_free[KP_ST], v_full[KP_ST], v_free[KP_ST], s_full[2], p_full[2], q_full, o_done;
+    __shared__ __align__(8) uint64_t full[KP_ST], empty[KP_ST], s_full[2], p_full[2], q_full, o_done;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_b, s_tile, s_sum[W];
     __shared__ __align__(4) uint8_t s_have[8][4];                             // whether a tile's blocks of 16 keys exist (softmax is up to four tiles behind)
@@ -122,7 +127,7 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
     const int span = a.causal ? min(sq.keys, max(0, sq.keys - sq.n + last + 1)) : sq.keys;
     const int tiles = (span + KP_N - 1) / KP_N;
     if (tid == 0) {
-        for (int i = 0; i < KP_ST; ++i) { mbar_init(&k_full[i], kp_exp<D>); mbar_init(&v_full[i], kp_exp<D>); mbar_init(&k_free[i], 1); mbar_init(&v_free[i], 1); }
+        for (int i = 0; i < KP_ST; ++i) { mbar_init(&full[i], kp_exp<D>); mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
         mbar_init(&q_full, 4 * nq); mbar_init(&o_done, 1);
         mbar_fence_init();
@@ -143,105 +148,116 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
             constexpr uint32_t ID_S = (1u << 4) | ((uint32_t)(KP_N >> 3) << 17) | ((uint32_t)(KP_M >> 4) << 24);                  // f32 += f16 x f16, K-major B
             constexpr uint32_t ID_O = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(KP_M >> 4) << 24);       // MN-major B
             const uint64_t dk = kp_desc(smem0, 16, 1024), dv = kp_desc(smem0 + KP_ST * TILE, KP_N * 128, 1024);
-            auto scores = [&](int q, int j) {                                 // S of tile q, keys 64 j ..
-                const int st = j % KP_ST, slot = NQ == 2 ? q : j & 1;
+            // The whole warp walks the tiles, so that addresses and descriptors stay in uniform registers; one elected lane issues.
+            auto scores = [&](int q, int slot, uint64_t keys) {
                 if (kp_elect()) {
+                    const uint32_t d = tmem + S0 + slot * KP_N, x = tmem + Q0 + q * (D / 2);
+                    kp_mma(d, x, keys, ID_S, 0u);
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i)
-                        kp_mma(tmem + S0 + slot * KP_N, tmem + Q0 + q * (D / 2) + i * 8, dk + (uint32_t)(st * (TILE >> 4) + (i >> 2) * (KP_N * 128 >> 4) + (i & 3) * 2), ID_S, i > 0);
+                    for (int i = 1; i < D / 16; ++i) kp_mma(d, x + i * 8, keys + (uint32_t)((i >> 2) * (KP_N * 128 >> 4) + (i & 3) * 2), ID_S, 1u);
                     kp_commit(&s_full[slot]);
-                    if (q == nq - 1) kp_commit(&k_free[st]);
                 }
                 __syncwarp();
             };
-            ok = kp_wait(&q_full, 0, &s_abort) && kp_wait(&k_full[0], 0, &s_abort);
+            ok = kp_wait(&q_full, 0, &s_abort) && kp_wait(&full[0], 0, &s_abort);
             kp_after();
-            if (ok) for (int q = 0; q < nq; ++q) scores(q, 0);
+            if (ok) for (int q = 0; q < nq; ++q) scores(q, q, dk);
+            int st = 0, nst = 1; uint32_t nph = 0, pph = 0;                   // stage of tile j and of the next, phases of the next one's and of the weights
             for (int j = 0; j < tiles && ok; ++j) {
                 const bool more = j + 1 < tiles;
-                if (more) ok = kp_wait(&k_full[(j + 1) % KP_ST], (uint32_t)((j + 1) / KP_ST & 1), &s_abort) && ok;
+                if (more) ok = kp_wait(&full[nst], nph, &s_abort) && ok;
                 kp_after();
-                if (NQ == 1 && more && ok) scores(0, j + 1);
-                ok = ok && kp_wait(&v_full[j % KP_ST], (uint32_t)(j / KP_ST & 1), &s_abort);
-                for (int q = 0; q < nq && ok; ++q) {
+                const uint64_t kn = dk + (uint32_t)(nst * (TILE >> 4)), v = dv + (uint32_t)(st * (TILE >> 4));
+                if (NQ == 1 && more && ok) scores(0, (j + 1) & 1, kn);
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                    if (q >= nq || !ok) break;
                     const int slot = NQ == 2 ? q : j & 1;
-                    ok = kp_wait(&p_full[slot], (uint32_t)((NQ == 2 ? j : j >> 1) & 1), &s_abort);
+                    ok = kp_wait(&p_full[slot], pph, &s_abort);
                     if (!ok) break;
                     kp_after();
                     if (kp_elect()) {
+                        const uint32_t d = tmem + q * D, x = tmem + S0 + slot * KP_N;
+                        kp_mma(d, x, v, ID_O, j > 0 ? 1u : 0u);
 #pragma unroll
-                        for (int i = 0; i < KP_N / 16; ++i)
-                            kp_mma(tmem + q * D, tmem + S0 + slot * KP_N + i * 8, dv + (uint32_t)((j % KP_ST) * (TILE >> 4) + i * (2048 >> 4)), ID_O, j > 0 || i > 0);
-                        if (q == nq - 1) { kp_commit(&v_free[j % KP_ST]); if (NQ == 1 || !more) kp_commit(&o_done); }
+                        for (int i = 1; i < KP_N / 16; ++i) kp_mma(d, x + i * 8, v + (uint32_t)(i * (2048 >> 4)), ID_O, 1u);
+                        if (q == nq - 1) { kp_commit(&empty[st]); if (NQ == 1 || !more) kp_commit(&o_done); }
                     }
                     __syncwarp();
-                    if (NQ == 2 && more) scores(q, j + 1);
+                    if (NQ == 2 && more) scores(q, q, kn);
                 }
+                st = nst;
+                if (++nst == KP_ST) { nst = 0; nph ^= 1u; }
+                if (NQ == 2 || (j & 1)) pph ^= 1u;
             }
         }
     } else if (warp < SW0 || warp >= SW0 + 4 * NQ) {
         // ------------------------------------------------------------ expand: keys PER e .. of every tile
-        constexpr int PER = KP_N / kp_exp<D>, LPC = 32 / PER, LD = (D / 32) * PER / 32;      // keys of a warp; 16-byte pieces a lane
-        static_assert(LD * 32 == (D / 32) * PER && PER * LPC == 32, "");
-        const int e = warp < SW0 ? warp - 1 : warp - (SW0 + 4 * NQ) + SW0 - 1, key = (lane & 7) + (PER == 16 ? lane & 8 : 0), ch0 = PER == 16 ? lane >> 4 : lane >> 3;
-        const int page_blocks = c.page_size / KV4_B, at = PER == 16 ? key : (e & 1) * 8 + key;            // position in its block of 16
+        // Pieces of 32 dims of a key, NP a lane: K first, then V.  Where a lane's pieces lie in a block and in a tile does not change.
+        constexpr int CH = D / 32, PER = KP_N / kp_exp<D>, NP = CH * PER / 16;
+        const int e = warp < SW0 ? warp - 1 : warp - (SW0 + 4 * NQ) + SW0 - 1, key = lane & (PER - 1), at = (e * PER + key) % KV4_B;      // at: position in its block of 16
+        const int page_blocks = c.page_size / KV4_B;
         const int* table = a.table + (int64_t)b * a.table_stride;
-        struct Raw { uint4 code[2][LD]; __half s[2][LD], b[2][LD]; bool have; };
-        auto fetch = [&](int j, Raw& r) {
-            const int blk = j * 4 + e * PER / KV4_B, pg = blk / page_blocks;
-            int page = -1;
-            if (j < tiles && blk * KV4_B < sq.keys) page = table[pg];
-            r.have = page >= 0 && page < c.pages;
-            const unsigned char* p = r.have ? kv4_block(c, page, head, blk - pg * page_blocks) : nullptr;
+        int code_at[NP], sb_at[NP]; uint32_t to[NP];
 #pragma unroll
-            for (int v = 0; v < 2; ++v)
-#pragma unroll
-                for (int i = 0; i < LD; ++i) {
-                    r.code[v][i] = make_uint4(0, 0, 0, 0); r.s[v][i] = __ushort_as_half(0); r.b[v][i] = __ushort_as_half(0);
-                    const int ch = ch0 + LPC * i;
-                    if (p && blk * KV4_B + at < sq.keys) {                    // (what lies behind the keys stays zero)
-                        r.code[v][i] = *reinterpret_cast<const uint4*>(p + v * 8 * D + kv4_swz((uint32_t)(at * (D / 2) + ch * 16)));
-                        const __half* sb = reinterpret_cast<const __half*>(p + (16 + v) * D) + (ch >> 1) * 32 + at;
-                        r.s[v][i] = sb[0]; r.b[v][i] = sb[16];
-                    }
+        for (int i = 0; i < NP; ++i) {
+            const int x = lane + 32 * i, v = x / (PER * CH), ch = x / PER % CH;
+            code_at[i] = v * 8 * D + (int)kv4_swz((uint32_t)(at * (D / 2) + ch * 16));
+            sb_at[i] = (16 + v) * D + ((ch >> 1) * 32 + at) * 2;
+            // (a row of 64 dims: 128 bytes, its 16-byte pieces XORed with the key)
+            to[i] = smem0 + v * KP_ST * TILE + (ch >> 1) * (KP_N * 128) + (e * PER + key) * 128 + ((((ch & 1) << 2) ^ (key & 7)) << 4);
+        }
+        unsigned long long page_at = 0;                                       // the block of tile (j & ~31) + lane, 0: there is none
+        auto block_of = [&](int j) -> const unsigned char* {
+            if ((j & 31) == 0) {
+                const int blk = (j + lane) * (KP_N / KV4_B) + e * PER / KV4_B, pg = blk / page_blocks;
+                page_at = 0;
+                if (j + lane < tiles && blk * KV4_B < sq.keys) {
+                    const int page = table[pg];
+                    if (page >= 0 && page < c.pages) page_at = (unsigned long long)kv4_block(c, page, head, blk - pg * page_blocks);
                 }
+            }
+            return (const unsigned char*)__shfl_sync(0xffffffffu, page_at, j & 31);
         };
-        auto store = [&](const Raw& r, int v, uint32_t tile) {                // row of 64 dims: 128 bytes, its 16-byte pieces XORed with the key
+        struct Raw { uint4 code[NP]; __half s[NP], b[NP]; bool have; };
+        auto fetch = [&](int j, Raw& r) {
+            const unsigned char* p = j < tiles ? block_of(j) : nullptr;
+            r.have = p != nullptr;
 #pragma unroll
-            for (int i = 0; i < LD; ++i) {
-                const int ch = ch0 + LPC * i;
-                const __half2 s = __half2half2(r.s[v][i]), bi = __half2half2(r.b[v][i]);
-                const uint32_t row = tile + (uint32_t)((ch >> 1) * (KP_N * 128) + (e * PER + key) * 128);
-                const uint32_t w[4] = {r.code[v][i].x, r.code[v][i].y, r.code[v][i].z, r.code[v][i].w};
+            for (int i = 0; i < NP; ++i) { r.code[i] = make_uint4(0, 0, 0, 0); r.s[i] = __ushort_as_half(0); r.b[i] = __ushort_as_half(0); }
+            if (p && j * KP_N + e * PER + key < sq.keys) {                      // (what lies behind the keys stays zero)
+#pragma unroll
+                for (int i = 0; i < NP; ++i) {
+                    r.code[i] = *reinterpret_cast<const uint4*>(p + code_at[i]);
+                    const __half* sb = reinterpret_cast<const __half*>(p + sb_at[i]);
+                    r.s[i] = sb[0]; r.b[i] = sb[16];
+                }
+            }
+        };
+        Raw next;
+        fetch(0, next);
+        int st = 0; uint32_t ph = 1;                                          // (a fresh barrier passes at 1)
+        for (int j = 0; j < tiles && ok; ++j) {
+            const Raw now = next;
+            fetch(j + 1, next);
+            ok = kp_wait(&empty[st], ph, &s_abort);
+            if (!ok) break;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const __half2 s = __half2half2(now.s[i]), bi = __half2half2(now.b[i]);
+                const uint32_t w[4] = {now.code[i].x, now.code[i].y, now.code[i].z, now.code[i].w}, row = to[i] + st * TILE;
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     uint32_t o[4];
                     kv4_expand(w[x], s, bi, o);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (((((ch & 1) << 2) + x) ^ (key & 7)) << 4)), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row ^ (uint32_t)(x << 4)), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
                 }
             }
-        };
-        auto publish = [&](uint64_t* bar) {
+            if (e * PER % KV4_B == 0 && lane == 0) s_have[j & 7][e * PER / KV4_B] = now.have;   // (read by softmax behind the scores, which wait for this)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) kp_arrive(bar);
-        };
-        Raw next;
-        fetch(0, next);
-        for (int j = 0; j < tiles && ok; ++j) {
-            const Raw now = next;
-            fetch(j + 1, next);
-            const int st = j % KP_ST;
-            const uint32_t ph = (uint32_t)(j / KP_ST & 1) ^ 1u;               // (a fresh barrier passes at 1)
-            ok = kp_wait(&k_free[st], ph, &s_abort);
-            if (!ok) break;
-            store(now, 0, smem0 + st * TILE);
-            if (e * PER % KV4_B == 0 && lane == 0) s_have[j & 7][e * PER / KV4_B] = now.have;      // (read by softmax behind the scores, which wait for this)
-            publish(&k_full[st]);
-            ok = kp_wait(&v_free[st], ph, &s_abort);
-            if (!ok) break;
-            store(now, 1, smem0 + (KP_ST + st) * TILE);
-            publish(&v_full[st]);
+            if (lane == 0) kp_arrive(&full[st]);
+            if (++st == KP_ST) { st = 0; ph ^= 1u; }
         }
     } else {
         // ------------------------------------------------------------ softmax: a thread a row
@@ -313,15 +329,18 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
                 }
                 const float base = KP_UP - (m == -INFINITY ? 0.f : m);
                 float sum[2] = {0.f, 0.f};
-                uint32_t p[32];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float x = kv4_exp2(fmaf(s[2 * i], a.scale, base)), y = kv4_exp2(fmaf(s[2 * i + 1], a.scale, base));
-                    sum[0] += x; sum[1] += y;
-                    p[i] = kv4_pack(x, y);
+                for (int i0 = 0; i0 < 32; i0 += 16) {
+                    uint32_t p[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float x = kv4_exp2(fmaf(s[2 * (i0 + i)], a.scale, base)), y = kv4_exp2(fmaf(s[2 * (i0 + i) + 1], a.scale, base));
+                        sum[0] += x; sum[1] += y;
+                        p[i] = kv4_pack(x, y);
+                    }
+                    kp_st16(tmem + lanes + S0 + slot * KP_N + i0, p);
                 }
                 l += sum[0] + sum[1];
-                kp_st32(tmem + lanes + S0 + slot * KP_N, p);
                 kp_wait_st();
                 kp_before();
                 __syncwarp();
