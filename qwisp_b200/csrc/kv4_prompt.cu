@@ -2,16 +2,16 @@
 //
 // A CTA takes NQ tiles of 128 rows (tokens x query heads of one kv head, so that the codes are expanded once for all of a kv head's
 // query heads) and walks the keys 64 at a time.  Warps have roles and meet only at mbarriers:
-//   mma       1 warp: S = Q K^T (queries as the A operand in tensor memory, keys in shared memory) and O += P V (weights in tensor memory
-//             where the scores were, values in shared memory), D + 64 NQ columns of f32 in tensor memory;
-//   expand    4 or 8 warps: a block of 16 keys or half of one each, codes from global memory a tile ahead, to fp16 (one multiply-add a pair), into 128-byte
-//             swizzled tiles: rows of 64 dims, K-major for the scores and, the same bytes, MN-major for the values.  A word expands to its dims
-//             in the order 0 4 1 5 2 6 3 7; the queries are loaded and the outputs stored in that order;
+//   mma       1 warp: S = Q K^T (queries as the A operand, in tensor memory where there is room for them, keys in shared memory) and O += P V
+//             (weights in tensor memory where the scores were, values in shared memory).  Scores are double buffered, so those of the next
+//             64 keys are ready before the weights of these are: with one buffer a tile's softmax waited for its own MMAs each time;
+//   expand    4 or 8 warps: a block of 16 keys or half of one each, codes from global memory a tile ahead, to fp16 (one multiply-add a pair),
+//             into 128-byte swizzled tiles: rows of 64 dims, K-major for the scores and, the same bytes, MN-major for the values.  A word
+//             expands to its dims in the order 0 4 1 5 2 6 3 7; the queries are loaded and the outputs stored in that order;
 //   softmax   4 warps a tile, a thread a row: scores in, running maximum and sum in registers, weights out.  The maximum is raised (and the
 //             outputs rescaled) only when a score exceeds it by 2^6; the weights are carried times 2^8, so that fp16 holds them from 2^-32 of the
 //             largest on.
-// NQ = 2 (D 64, 128): while the rows of one tile go through softmax, the tensor cores work for the other.  NQ = 1 (D 256, where the outputs
-// take half of tensor memory): the scores of the next 64 keys are ready before the weights of these are.
+// NQ = 2 (D 64, 128): the expansion serves two tiles.  NQ = 1 (D 256): the outputs of one take half of tensor memory.
 #include "kv4.cuh"
 #include "kv4_mma.cuh"
 
@@ -22,8 +22,11 @@ template <int D> constexpr int kp_nq = D == 256 ? 1 : 2;
 template <int D> constexpr int kp_exp = D == 256 ? 8 : 4;                     // expanding warps: 13 warps in all, 128 registers a thread
 template <int D> constexpr int kp_threads = (1 + kp_exp<D> + 4 * kp_nq<D>) * 32;
 template <int D> constexpr int kp_tile = KP_N * D * 2;                        // bytes of a tile of keys or values
+template <int D> constexpr bool kp_qt = D != 128;                            // queries in tensor memory (two tiles of 128 dims: outputs and scores fill it)
+template <int D> constexpr int kp_io = 4 * kp_nq<D> * 4096;                  // where a softmax warp turns 32 rows of 64 dims
+template <int D> constexpr int kp_bytes = 2 * KP_ST * kp_tile<D> + kp_io<D> + (kp_qt<D> ? 0 : kp_nq<D> * KP_M * D * 2);
 // (more than half of a multiprocessor's: a second CTA would wait for the first one's tensor memory)
-template <int D> constexpr size_t kp_smem = ((size_t)2 * KP_ST * kp_tile<D> > 120 * 1024 ? (size_t)2 * KP_ST * kp_tile<D> : 120 * 1024) + 1024;
+template <int D> constexpr int kp_smem = (kp_bytes<D> > 120 * 1024 ? kp_bytes<D> : 120 * 1024) + 1024;
 constexpr int KP_LIMIT = 1 << 22;                                            // polls of a wait (up to 4 us each)
 constexpr float KP_UP = 8.0f, KP_SLACK = 6.0f;
 
@@ -34,6 +37,10 @@ __device__ __forceinline__ uint64_t kp_desc(uint32_t addr, uint32_t lbo, uint32_
 __device__ __forceinline__ void kp_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void kp_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {      // both operands in shared memory
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void kp_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -56,6 +63,12 @@ __device__ __forceinline__ void kp_st16(uint32_t t, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
                  ::"r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
                    "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void kp_sts(uint32_t p, const uint4& v) { asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory"); }
+__device__ __forceinline__ uint4 kp_lds(uint32_t p) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
+    return v;
 }
 __device__ __forceinline__ void kp_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void kp_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -84,10 +97,12 @@ struct KpSeq { int q0, rows, n, keys; };
 template <int D>
 __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4AttnArgs a, int least, uint32_t q_and, uint32_t q_xor) {
     constexpr int NQ = kp_nq<D>, TILE = kp_tile<D>, NT = kp_threads<D>, W = NT / 32, SW0 = 4;      // softmax warps start at SW0
-    constexpr uint32_t S0 = NQ * D, Q0 = S0 + 2 * KP_N;                       // columns of tensor memory: outputs, scores, queries
+    constexpr bool QT = kp_qt<D>;
+    constexpr uint32_t S0 = NQ * D, Q0 = S0 + NQ * 2 * KP_N;                  // columns of tensor memory: outputs, scores (two of each tile), queries
+    static_assert(Q0 + (QT ? NQ * D / 2 : 0) <= 512, "tensor memory");
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    __shared__ __align__(8) uint64_t full[KP_ST], empty[KP_ST], s_full[2], p_full[2], q_full, o_done;
+    __shared__ __align__(8) uint64_t full[KP_ST], empty[KP_ST], s_full[2 * NQ], p_full[2 * NQ], q_full, o_done[NQ];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_b, s_tile, s_sum[W];
     __shared__ __align__(4) uint8_t s_have[8][4];                             // whether a tile's blocks of 16 keys exist (softmax is up to four tiles behind)
@@ -128,8 +143,9 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
     const int tiles = (span + KP_N - 1) / KP_N;
     if (tid == 0) {
         for (int i = 0; i < KP_ST; ++i) { mbar_init(&full[i], kp_exp<D>); mbar_init(&empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
-        mbar_init(&q_full, 4 * nq); mbar_init(&o_done, 1);
+        for (int i = 0; i < 2 * NQ; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
+        for (int i = 0; i < NQ; ++i) mbar_init(&o_done[i], 1);
+        mbar_init(&q_full, 4 * nq);
         mbar_fence_init();
     }
     if (warp == 0) {
@@ -140,7 +156,7 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
     kp_before();
     __syncthreads();
     kp_after();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0), smem0 = smem_u32(smem);
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0), smem0 = smem_u32(smem), io0 = smem0 + 2 * KP_ST * TILE, qs0 = io0 + kp_io<D>;
     bool ok = true;
     if (warp == 0) {
         // ------------------------------------------------------------ mma
@@ -149,46 +165,52 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
             constexpr uint32_t ID_O = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(KP_M >> 4) << 24);       // MN-major B
             const uint64_t dk = kp_desc(smem0, 16, 1024), dv = kp_desc(smem0 + KP_ST * TILE, KP_N * 128, 1024);
             // The whole warp walks the tiles, so that addresses and descriptors stay in uniform registers; one elected lane issues.
+            const uint64_t dq = kp_desc(qs0, 16, 1024);
             auto scores = [&](int q, int slot, uint64_t keys) {
                 if (kp_elect()) {
-                    const uint32_t d = tmem + S0 + slot * KP_N, x = tmem + Q0 + q * (D / 2);
-                    kp_mma(d, x, keys, ID_S, 0u);
+                    const uint32_t d = tmem + S0 + (2 * q + slot) * KP_N, x = tmem + Q0 + q * (D / 2);
+                    const uint64_t y = dq + (uint32_t)(q * (KP_M * D * 2 >> 4));
 #pragma unroll
-                    for (int i = 1; i < D / 16; ++i) kp_mma(d, x + i * 8, keys + (uint32_t)((i >> 2) * (KP_N * 128 >> 4) + (i & 3) * 2), ID_S, 1u);
-                    kp_commit(&s_full[slot]);
+                    for (int i = 0; i < D / 16; ++i) {
+                        const uint64_t k = keys + (uint32_t)((i >> 2) * (KP_N * 128 >> 4) + (i & 3) * 2);
+                        if (QT) kp_mma(d, x + i * 8, k, ID_S, i > 0 ? 1u : 0u);
+                        else kp_mma_ss(d, y + (uint32_t)((i >> 2) * (KP_M * 128 >> 4) + (i & 3) * 2), k, ID_S, i > 0 ? 1u : 0u);
+                    }
+                    kp_commit(&s_full[2 * q + slot]);
                 }
                 __syncwarp();
             };
             ok = kp_wait(&q_full, 0, &s_abort) && kp_wait(&full[0], 0, &s_abort);
             kp_after();
-            if (ok) for (int q = 0; q < nq; ++q) scores(q, q, dk);
-            int st = 0, nst = 1; uint32_t nph = 0, pph = 0;                   // stage of tile j and of the next, phases of the next one's and of the weights
+            if (ok) for (int q = 0; q < nq; ++q) scores(q, 0, dk);
+            int st = 0, nst = 1; uint32_t nph = 0;                            // stage of tile j and of the next, phase of the next one's
             for (int j = 0; j < tiles && ok; ++j) {
                 const bool more = j + 1 < tiles;
                 if (more) ok = kp_wait(&full[nst], nph, &s_abort) && ok;
                 kp_after();
                 const uint64_t kn = dk + (uint32_t)(nst * (TILE >> 4)), v = dv + (uint32_t)(st * (TILE >> 4));
-                if (NQ == 1 && more && ok) scores(0, (j + 1) & 1, kn);
+                if (more && ok) {
+                    scores(0, (j + 1) & 1, kn);
+                    if (NQ == 2 && nq == 2) scores(NQ - 1, (j + 1) & 1, kn);
+                }
 #pragma unroll
                 for (int q = 0; q < NQ; ++q) {
                     if (q >= nq || !ok) break;
-                    const int slot = NQ == 2 ? q : j & 1;
-                    ok = kp_wait(&p_full[slot], pph, &s_abort);
+                    ok = kp_wait(&p_full[2 * q + (j & 1)], (uint32_t)(j >> 1) & 1u, &s_abort);
                     if (!ok) break;
                     kp_after();
                     if (kp_elect()) {
-                        const uint32_t d = tmem + q * D, x = tmem + S0 + slot * KP_N;
+                        const uint32_t d = tmem + q * D, x = tmem + S0 + (2 * q + (j & 1)) * KP_N;
                         kp_mma(d, x, v, ID_O, j > 0 ? 1u : 0u);
 #pragma unroll
                         for (int i = 1; i < KP_N / 16; ++i) kp_mma(d, x + i * 8, v + (uint32_t)(i * (2048 >> 4)), ID_O, 1u);
-                        if (q == nq - 1) { kp_commit(&empty[st]); if (NQ == 1 || !more) kp_commit(&o_done); }
+                        if (q == nq - 1) kp_commit(&empty[st]);
+                        kp_commit(&o_done[q]);
                     }
                     __syncwarp();
-                    if (NQ == 2 && more) scores(q, q, kn);
                 }
                 st = nst;
                 if (++nst == KP_ST) { nst = 0; nph ^= 1u; }
-                if (NQ == 2 || (j & 1)) pph ^= 1u;
             }
         }
     } else if (warp < SW0 || warp >= SW0 + 4 * NQ) {
@@ -234,14 +256,10 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
                 }
             }
         };
-        Raw next;
-        fetch(0, next);
         int st = 0; uint32_t ph = 1;                                          // (a fresh barrier passes at 1)
-        for (int j = 0; j < tiles && ok; ++j) {
-            const Raw now = next;
-            fetch(j + 1, next);
+        auto work = [&](int j, const Raw& now) {
             ok = kp_wait(&empty[st], ph, &s_abort);
-            if (!ok) break;
+            if (!ok) return;
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const __half2 s = __half2half2(now.s[i]), bi = __half2half2(now.b[i]);
@@ -250,14 +268,23 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
                 for (int x = 0; x < 4; ++x) {
                     uint32_t o[4];
                     kv4_expand(w[x], s, bi, o);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row ^ (uint32_t)(x << 4)), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+                    kp_sts(row ^ (uint32_t)(x << 4), make_uint4(o[0], o[1], o[2], o[3]));
                 }
             }
-            if (e * PER % KV4_B == 0 && lane == 0) s_have[j & 7][e * PER / KV4_B] = now.have;   // (read by softmax behind the scores, which wait for this)
+            if (e * PER % KV4_B == 0 && lane == 0) s_have[j & 7][e * PER / KV4_B] = now.have;      // (read by softmax behind the scores, which wait for this)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) kp_arrive(&full[st]);
             if (++st == KP_ST) { st = 0; ph ^= 1u; }
+        };
+        Raw one, two;
+        fetch(0, one);
+        for (int j = 0; j < tiles && ok; j += 2) {
+            fetch(j + 1, two);
+            work(j, one);
+            if (j + 1 >= tiles || !ok) break;
+            fetch(j + 2, one);
+            work(j + 1, two);
         }
     } else {
         // ------------------------------------------------------------ softmax: a thread a row
@@ -266,23 +293,40 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
         if (q < nq) {
             const int tok = t0 + q * tokens + row / a.G, h = head * a.G + row % a.G;
             const bool live = row < tokens * a.G && tok < sq.rows;
-            if (tiles > 0) {
-                const __half* src = a.q + (int64_t)(sq.q0 + tok) * a.q_row + (int64_t)h * a.q_head;
+            const uint32_t io = io0 + (warp - SW0) * 4096, own = io + lane * 128;                // 32 rows of 128 bytes, 16-byte pieces XORed with the row
+            auto place = [&](int64_t by_row, int64_t by_head) { return live ? (int64_t)(sq.q0 + tok) * by_row + (int64_t)h * by_head : (int64_t)-1; };
+            // 64 dims of the warp's rows, eight lanes a row: 128 bytes at a time
+            auto rows_in = [&](const __half* src, int64_t mine, int d, uint4 v[8]) {
 #pragma unroll
-                for (int c0 = 0; c0 < D / 2; c0 += 32) {
-                    uint32_t r[32];
+                for (int i = 0; i < 8; ++i) {
+                    const int64_t at = __shfl_sync(0xffffffffu, mine, i * 4 + (lane >> 3));
+                    v[i] = at >= 0 ? *reinterpret_cast<const uint4*>(src + at + d + (lane & 7) * 8) : make_uint4(0, 0, 0, 0);
+                }
+            };
+            auto turn = [&](int i) { const int r = i * 4 + (lane >> 3); return (uint32_t)(r * 128 + (((lane & 7) ^ (r & 7)) << 4)); };
+            if (tiles > 0) {
+                const int64_t mine = place(a.q_row, a.q_head);
+#pragma unroll 1
+                for (int d = 0; d < D; d += 64) {
+                    uint4 v[8];
+                    rows_in(a.q, mine, d, v);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        uint4 v = make_uint4(0, 0, 0, 0);
-                        if (live) v = *reinterpret_cast<const uint4*>(src + c0 * 2 + i * 8);
-                        r[4 * i] = (__byte_perm(v.x, v.z, 0x5410) & q_and) ^ q_xor; r[4 * i + 1] = (__byte_perm(v.x, v.z, 0x7632) & q_and) ^ q_xor;
-                        r[4 * i + 2] = (__byte_perm(v.y, v.w, 0x5410) & q_and) ^ q_xor; r[4 * i + 3] = (__byte_perm(v.y, v.w, 0x7632) & q_and) ^ q_xor;
+                        const uint4 x = make_uint4((__byte_perm(v[i].x, v[i].z, 0x5410) & q_and) ^ q_xor, (__byte_perm(v[i].x, v[i].z, 0x7632) & q_and) ^ q_xor,
+                                                   (__byte_perm(v[i].y, v[i].w, 0x5410) & q_and) ^ q_xor, (__byte_perm(v[i].y, v[i].w, 0x7632) & q_and) ^ q_xor);
+                        kp_sts(QT ? io + turn(i) : qs0 + q * (KP_M * D * 2) + (d >> 6) * (KP_M * 128) + (warp & 3) * 4096 + turn(i), x);
                     }
-                    __syncwarp();
-                    kp_st32(tmem + lanes + Q0 + q * (D / 2) + c0, r);
+                    if (QT) {
+                        __syncwarp();
+                        uint32_t r[32];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(r + 4 * i) = kp_lds(own + ((i ^ (lane & 7)) << 4));
+                        kp_st32(tmem + lanes + Q0 + q * (D / 2) + d / 2, r);
+                        __syncwarp();
+                    }
                 }
-                kp_wait_st();
-                kp_before();
+                if (QT) { kp_wait_st(); kp_before(); }
+                else asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) kp_arrive(&q_full);
             }
@@ -291,8 +335,8 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
             const int all = a.causal ? min(sq.keys, sq.keys - sq.n + t0 + q * tokens + 1) : sq.keys;
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < tiles && ok; ++j) {
-                const int slot = NQ == 2 ? q : j & 1, k0 = j * KP_N;
-                ok = kp_wait(&s_full[slot], (uint32_t)((NQ == 2 ? j : j >> 1) & 1), &s_abort);
+                const int slot = 2 * q + (j & 1), k0 = j * KP_N;
+                ok = kp_wait(&s_full[slot], (uint32_t)(j >> 1) & 1u, &s_abort);
                 if (!ok) break;
                 kp_after();
                 const uint32_t have = *reinterpret_cast<const uint32_t*>(s_have[j & 7]);
@@ -313,7 +357,7 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
                     const float nm = fmaxf(m, top), f = nm == -INFINITY ? 1.f : kv4_exp2(m - nm);
                     m = nm; l *= f;
                     if (j > 0) {                                              // the outputs so far
-                        if (NQ == 1) ok = kp_wait(&o_done, (uint32_t)(j - 1) & 1, &s_abort);      // (NQ 2: they were done before these scores)
+                        ok = kp_wait(&o_done[q], (uint32_t)(j - 1) & 1u, &s_abort);
                         if (!ok) break;
                         kp_after();
 #pragma unroll 1
@@ -347,30 +391,45 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
                 if (lane == 0) kp_arrive(&p_full[slot]);
             }
             // ---- normalise, gate, round once; eight columns are the dims 0 4 1 5 2 6 3 7 of a word
-            if (tiles > 0 && ok) ok = kp_wait(&o_done, NQ == 1 ? (uint32_t)(tiles - 1) & 1 : 0u, &s_abort);
+            if (tiles > 0 && ok) ok = kp_wait(&o_done[q], (uint32_t)(tiles - 1) & 1u, &s_abort);
             kp_after();
             const float inv = l == 0.f ? 0.f : 1.0f / l;
-            __half* dst = a.out + (int64_t)(sq.q0 + tok) * a.o_row + (int64_t)h * a.o_head;
-            const __half* gate = a.gate ? a.gate + (int64_t)(sq.q0 + tok) * a.g_row + (int64_t)h * a.g_head : nullptr;
+            const int64_t to = place(a.o_row, a.o_head), gates = place(a.g_row, a.g_head);
 #pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 32) {
-                uint32_t o[32];
-                __syncwarp();
-                if (tiles > 0) { kp_ld32(tmem + lanes + q * D + c0, o); kp_wait_ld(); }
-                if (!live) continue;
+            for (int d = 0; d < D; d += 64) {
+                if (a.gate) {
+                    uint4 v[8];
+                    rows_in(a.gate, gates, d, v);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float x[8];
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) x[(k & 1) * 4 + (k >> 1)] = !ok ? __int_as_float(0x7fffffff) : l == 0.f ? 0.f : __uint_as_float(o[8 * i + k]) * inv;
-                    if (gate) {
-                        const uint4 g = *reinterpret_cast<const uint4*>(gate + c0 + 8 * i);
-                        const __half* gh = reinterpret_cast<const __half*>(&g);
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) x[k] *= sigmoid_f(h2f(gh[k]));
-                    }
-                    *reinterpret_cast<uint4*>(dst + c0 + 8 * i) = make_uint4(kv4_pack(x[0], x[1]), kv4_pack(x[2], x[3]), kv4_pack(x[4], x[5]), kv4_pack(x[6], x[7]));
+                    for (int i = 0; i < 8; ++i) kp_sts(io + turn(i), v[i]);
                 }
+                __syncwarp();
+#pragma unroll
+                for (int c0 = 0; c0 < 64; c0 += 32) {
+                    uint32_t o[32];
+                    if (tiles > 0) { kp_ld32(tmem + lanes + q * D + d + c0, o); kp_wait_ld(); }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t at = own + (((c0 / 8 + i) ^ (lane & 7)) << 4);
+                        float x[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) x[(k & 1) * 4 + (k >> 1)] = !ok ? __int_as_float(0x7fffffff) : l == 0.f ? 0.f : __uint_as_float(o[8 * i + k]) * inv;
+                        if (a.gate) {
+                            const uint4 g = kp_lds(at);
+                            const __half* gh = reinterpret_cast<const __half*>(&g);
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) x[k] *= sigmoid_f(h2f(gh[k]));
+                        }
+                        kp_sts(at, make_uint4(kv4_pack(x[0], x[1]), kv4_pack(x[2], x[3]), kv4_pack(x[4], x[5]), kv4_pack(x[6], x[7])));
+                    }
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int64_t at = __shfl_sync(0xffffffffu, to, i * 4 + (lane >> 3));
+                    if (at >= 0) *reinterpret_cast<uint4*>(a.out + at + d + (lane & 7) * 8) = kp_lds(io + turn(i));
+                }
+                __syncwarp();
             }
         }
     }
@@ -393,7 +452,7 @@ static int launch_prompt_t(const Kv4Cache& c, Kv4AttnArgs a, int least, cudaStre
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 64 || !(configured.load(std::memory_order_relaxed) >> dev & 1)) {
-        cudaError_t err = cudaFuncSetAttribute(k_kv4_prompt<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kp_smem<D>);
+        cudaError_t err = cudaFuncSetAttribute(k_kv4_prompt<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kp_smem<D>);
         if (err != cudaSuccess) return (int)err;
         if (dev < 64) configured.fetch_or(1ull << dev);
     }
