@@ -78,7 +78,7 @@ __device__ __forceinline__ void kd_finish(const Kv4AttnArgs& a, int row, int h, 
     if (a.gate) {
         const uint2 g = *reinterpret_cast<const uint2*>(a.gate + row * a.g_row + h * a.g_head + d);
         const float2 g0 = __half22float2(*reinterpret_cast<const __half2*>(&g.x)), g1 = __half22float2(*reinterpret_cast<const __half2*>(&g.y));
-        o.x *= sigmoid_f(g0.x); o.y *= sigmoid_f(g0.y); o.z *= sigmoid_f(g1.x); o.w *= sigmoid_f(g1.y);
+        o.x *= kv4_sigmoid(g0.x); o.y *= kv4_sigmoid(g0.y); o.z *= kv4_sigmoid(g1.x); o.w *= kv4_sigmoid(g1.y);
     }
     const __half2 r0 = __floats2half2_rn(o.x, o.y), r1 = __floats2half2_rn(o.z, o.w);
     uint2 r; r.x = *reinterpret_cast<const uint32_t*>(&r0); r.y = *reinterpret_cast<const uint32_t*>(&r1);

@@ -27,6 +27,8 @@ __device__ __forceinline__ uint32_t kv4_transpose(uint32_t v) {
     return r;
 }
 __device__ __forceinline__ float kv4_exp2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+// 1 / (1 + e^-x), some 2^-21 of itself off: an infinite power makes it 0
+__device__ __forceinline__ float kv4_sigmoid(float x) { return __fdividef(1.0f, 1.0f + fminf(kv4_exp2(x * -1.4426950408889634f), 0x1p126f)); }
 __device__ __forceinline__ uint32_t kv4_pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ __half2 kv4_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
 __device__ __forceinline__ uint32_t kv4_u(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }

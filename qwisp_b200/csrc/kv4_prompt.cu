@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
     static_assert(Q0 + (QT ? NQ * D / 2 : 0) <= 512, "tensor memory");
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    __shared__ __align__(8) uint64_t full[KP_ST], empty[KP_ST], s_full[2 * NQ], p_full[2 * NQ], q_full, o_done[NQ];
+    __shared__ __align__(8) uint64_t full[KP_ST], empty[KP_ST], s_full[2 * NQ], p_full[2 * NQ], q_full, o_done[2 * NQ];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_b, s_tile, s_sum[W];
     __shared__ __align__(4) uint8_t s_have[8][4];                             // whether a tile's blocks of 16 keys exist (softmax is up to four tiles behind)
@@ -143,8 +143,7 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
     const int tiles = (span + KP_N - 1) / KP_N;
     if (tid == 0) {
         for (int i = 0; i < KP_ST; ++i) { mbar_init(&full[i], kp_exp<D>); mbar_init(&empty[i], 1); }
-        for (int i = 0; i < 2 * NQ; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
-        for (int i = 0; i < NQ; ++i) mbar_init(&o_done[i], 1);
+        for (int i = 0; i < 2 * NQ; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
         mbar_init(&q_full, 4 * nq);
         mbar_fence_init();
     }
@@ -164,10 +163,12 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
             constexpr uint32_t ID_S = (1u << 4) | ((uint32_t)(KP_N >> 3) << 17) | ((uint32_t)(KP_M >> 4) << 24);                  // f32 += f16 x f16, K-major B
             constexpr uint32_t ID_O = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(KP_M >> 4) << 24);       // MN-major B
             const uint64_t dk = kp_desc(smem0, 16, 1024), dv = kp_desc(smem0 + KP_ST * TILE, KP_N * 128, 1024);
-            // The whole warp walks the tiles, so that addresses and descriptors stay in uniform registers; one elected lane issues.
+            // The whole warp walks the tiles, so that addresses and descriptors stay in uniform registers; one lane, elected once, issues
+            // everything: MMAs are ordered, and their commits count, by thread.
+            const bool leader = kp_elect();
             const uint64_t dq = kp_desc(qs0, 16, 1024);
             auto scores = [&](int q, int slot, uint64_t keys) {
-                if (kp_elect()) {
+                if (leader) {
                     const uint32_t d = tmem + S0 + (2 * q + slot) * KP_N, x = tmem + Q0 + q * (D / 2);
                     const uint64_t y = dq + (uint32_t)(q * (KP_M * D * 2 >> 4));
 #pragma unroll
@@ -199,13 +200,13 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
                     ok = kp_wait(&p_full[2 * q + (j & 1)], (uint32_t)(j >> 1) & 1u, &s_abort);
                     if (!ok) break;
                     kp_after();
-                    if (kp_elect()) {
+                    if (leader) {
                         const uint32_t d = tmem + q * D, x = tmem + S0 + (2 * q + (j & 1)) * KP_N;
                         kp_mma(d, x, v, ID_O, j > 0 ? 1u : 0u);
 #pragma unroll
                         for (int i = 1; i < KP_N / 16; ++i) kp_mma(d, x + i * 8, v + (uint32_t)(i * (2048 >> 4)), ID_O, 1u);
                         if (q == nq - 1) kp_commit(&empty[st]);
-                        kp_commit(&o_done[q]);
+                        kp_commit(&o_done[2 * q + (j & 1)]);
                     }
                     __syncwarp();
                 }
@@ -307,22 +308,28 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
             if (tiles > 0) {
                 const int64_t mine = place(a.q_row, a.q_head);
 #pragma unroll 1
-                for (int d = 0; d < D; d += 64) {
-                    uint4 v[8];
-                    rows_in(a.q, mine, d, v);
+                for (int d0 = 0; d0 < D; d0 += 128) {                         // (128 dims in flight)
+                    constexpr int AT_ONCE = D == 64 ? 1 : 2;
+                    uint4 v[AT_ONCE][8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint4 x = make_uint4((__byte_perm(v[i].x, v[i].z, 0x5410) & q_and) ^ q_xor, (__byte_perm(v[i].x, v[i].z, 0x7632) & q_and) ^ q_xor,
-                                                   (__byte_perm(v[i].y, v[i].w, 0x5410) & q_and) ^ q_xor, (__byte_perm(v[i].y, v[i].w, 0x7632) & q_and) ^ q_xor);
-                        kp_sts(QT ? io + turn(i) : qs0 + q * (KP_M * D * 2) + (d >> 6) * (KP_M * 128) + (warp & 3) * 4096 + turn(i), x);
-                    }
-                    if (QT) {
-                        __syncwarp();
-                        uint32_t r[32];
+                    for (int k = 0; k < AT_ONCE; ++k) rows_in(a.q, mine, d0 + 64 * k, v[k]);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(r + 4 * i) = kp_lds(own + ((i ^ (lane & 7)) << 4));
-                        kp_st32(tmem + lanes + Q0 + q * (D / 2) + d / 2, r);
-                        __syncwarp();
+                    for (int k = 0; k < AT_ONCE; ++k) {
+                        const int d = d0 + 64 * k;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const uint4 y = v[k][i], x = make_uint4((__byte_perm(y.x, y.z, 0x5410) & q_and) ^ q_xor, (__byte_perm(y.x, y.z, 0x7632) & q_and) ^ q_xor,
+                                                                    (__byte_perm(y.y, y.w, 0x5410) & q_and) ^ q_xor, (__byte_perm(y.y, y.w, 0x7632) & q_and) ^ q_xor);
+                            kp_sts(QT ? io + turn(i) : qs0 + q * (KP_M * D * 2) + (d >> 6) * (KP_M * 128) + (warp & 3) * 4096 + turn(i), x);
+                        }
+                        if (QT) {
+                            __syncwarp();
+                            uint32_t r[32];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(r + 4 * i) = kp_lds(own + ((i ^ (lane & 7)) << 4));
+                            kp_st32(tmem + lanes + Q0 + q * (D / 2) + d / 2, r);
+                            __syncwarp();
+                        }
                     }
                 }
                 if (QT) { kp_wait_st(); kp_before(); }
@@ -357,7 +364,9 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
                     const float nm = fmaxf(m, top), f = nm == -INFINITY ? 1.f : kv4_exp2(m - nm);
                     m = nm; l *= f;
                     if (j > 0) {                                              // the outputs so far
-                        ok = kp_wait(&o_done[q], (uint32_t)(j - 1) & 1u, &s_abort);
+                        // (a parity does not tell a phase from the one two before.  Even and odd tiles have a barrier each, and these scores'
+                        // MMAs were issued, and so are done, behind O += P V of tile j - 2)
+                        ok = kp_wait(&o_done[2 * q + ((j - 1) & 1)], (uint32_t)((j - 1) >> 1) & 1u, &s_abort);
                         if (!ok) break;
                         kp_after();
 #pragma unroll 1
@@ -391,7 +400,7 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
                 if (lane == 0) kp_arrive(&p_full[slot]);
             }
             // ---- normalise, gate, round once; eight columns are the dims 0 4 1 5 2 6 3 7 of a word
-            if (tiles > 0 && ok) ok = kp_wait(&o_done[q], (uint32_t)(tiles - 1) & 1u, &s_abort);
+            if (tiles > 0 && ok) ok = kp_wait(&o_done[2 * q + ((tiles - 1) & 1)], (uint32_t)((tiles - 1) >> 1) & 1u, &s_abort);
             kp_after();
             const float inv = l == 0.f ? 0.f : 1.0f / l;
             const int64_t to = place(a.o_row, a.o_head), gates = place(a.g_row, a.g_head);
@@ -418,7 +427,7 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
                             const uint4 g = kp_lds(at);
                             const __half* gh = reinterpret_cast<const __half*>(&g);
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) x[k] *= sigmoid_f(h2f(gh[k]));
+                            for (int k = 0; k < 8; ++k) x[k] *= kv4_sigmoid(h2f(gh[k]));
                         }
                         kp_sts(at, make_uint4(kv4_pack(x[0], x[1]), kv4_pack(x[2], x[3]), kv4_pack(x[4], x[5]), kv4_pack(x[6], x[7])));
                     }

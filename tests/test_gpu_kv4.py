@@ -465,6 +465,25 @@ def test_scores_far_apart(D, news, keys):
         assert (err <= bound).all(), float((err / bound).max())
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("news,keys", [([1, 1], [900, 300]), ([2] * 3, [700, 64, 333]), ([90, 70], [200, 400]), ([40], [1500])])
+def test_maxima_that_rise_along_the_keys(D, news, keys):
+    """Keys that get longer along the positions, so that rows raise their maxima, and rescale what they have, at tiles of their own; the
+    same bits a hundred times."""
+    cache, table, q, starts = attention_case(D, 8, 2, 32, news, keys)
+    g = gen(6)
+    for b, n in enumerate(keys):
+        p = torch.arange(n, device="cuda")
+        k, v = (torch.randn((n, 2, D), generator=g, device="cuda") for _ in range(2))
+        k *= (1 + 4 * p.double() / n).float()[:, None, None] * (1 + (p % 7 == 3).float())[:, None, None]
+        ops().kv4_append(cache, table[b].long()[p // 32] * 32 + p % 32, None, k.to(F16), v.to(F16))
+    call = lambda: ops().kv4_attention(cache, table, ints(keys), q, ints(starts), max(news))  # noqa: E731
+    first = call()
+    near(first, *attention_reference(cache, table, keys, q, starts, True, D ** -0.5))
+    for _ in range(100):
+        assert torch.equal(call(), first)
+
+
 def test_a_long_tail_of_small_weights_counts():
     """One key far ahead of 30000 others whose weights are 2^-17 each: together they are a fifth of the result."""
     D, page, n = 128, 64, 30000
