@@ -27,6 +27,13 @@ __device__ __forceinline__ uint32_t kv4_transpose(uint32_t v) {
     return r;
 }
 __device__ __forceinline__ float kv4_exp2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+// Pairs of f32 values in one 64-bit register (one instruction, the bits of two), and the larger of three
+typedef unsigned long long kv4_f2;
+__device__ __forceinline__ kv4_f2 kv4_pair(float x, float y) { kv4_f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y)); return r; }
+__device__ __forceinline__ float2 kv4_unpair(kv4_f2 v) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v)); return r; }
+__device__ __forceinline__ kv4_f2 kv4_fma2(kv4_f2 a, kv4_f2 b, kv4_f2 c) { kv4_f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ kv4_f2 kv4_add2(kv4_f2 a, kv4_f2 b) { kv4_f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ float kv4_max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 // 1 / (1 + e^-x), some 2^-21 of itself off: an infinite power makes it 0
 __device__ __forceinline__ float kv4_sigmoid(float x) { return __fdividef(1.0f, 1.0f + fminf(kv4_exp2(x * -1.4426950408889634f), 0x1p126f)); }
 __device__ __forceinline__ uint32_t kv4_pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }

@@ -298,11 +298,11 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
             auto place = [&](int64_t by_row, int64_t by_head) { return live ? (int64_t)(sq.q0 + tok) * by_row + (int64_t)h * by_head : (int64_t)-1; };
             // 64 dims of the warp's rows, eight lanes a row: 128 bytes at a time
             auto rows_in = [&](const __half* src, int64_t mine, int d, uint4 v[8]) {
+                // (a row that there is none of reads the first, so that no load is behind a branch: eight in flight, not one)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int64_t at = __shfl_sync(0xffffffffu, mine, i * 4 + (lane >> 3));
-                    v[i] = at >= 0 ? *reinterpret_cast<const uint4*>(src + at + d + (lane & 7) * 8) : make_uint4(0, 0, 0, 0);
-                }
+                for (int i = 0; i < 8; ++i) v[i] = __ldcg(reinterpret_cast<const uint4*>(src + max(__shfl_sync(0xffffffffu, mine, i * 4 + (lane >> 3)), (int64_t)0) + d + (lane & 7) * 8));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) if (__shfl_sync(0xffffffffu, mine, i * 4 + (lane >> 3)) < 0) v[i] = make_uint4(0, 0, 0, 0);
             };
             auto turn = [&](int i) { const int r = i * 4 + (lane >> 3); return (uint32_t)(r * 128 + (((lane & 7) ^ (r & 7)) << 4)); };
             if (tiles > 0) {
@@ -358,7 +358,11 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
                 }
                 float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int i = 4; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+                for (int i = 4; i < 60; i += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mx[k] = kv4_max3(mx[k], s[i + k], s[i + 4 + k]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], s[60 + k]);
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale;
                 if (__any_sync(0xffffffffu, top > m + KP_SLACK)) {
                     const float nm = fmaxf(m, top), f = nm == -INFINITY ? 1.f : kv4_exp2(m - nm);
@@ -381,19 +385,22 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
                     }
                 }
                 const float base = KP_UP - (m == -INFINITY ? 0.f : m);
-                float sum[2] = {0.f, 0.f};
+                kv4_f2 sum[2] = {0, 0};
+                const kv4_f2 scale2 = kv4_pair(a.scale, a.scale), base2 = kv4_pair(base, base);
 #pragma unroll
                 for (int i0 = 0; i0 < 32; i0 += 16) {
                     uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float x = kv4_exp2(fmaf(s[2 * (i0 + i)], a.scale, base)), y = kv4_exp2(fmaf(s[2 * (i0 + i) + 1], a.scale, base));
-                        sum[0] += x; sum[1] += y;
+                        const float2 t = kv4_unpair(kv4_fma2(kv4_pair(s[2 * (i0 + i)], s[2 * (i0 + i) + 1]), scale2, base2));
+                        const float x = kv4_exp2(t.x), y = kv4_exp2(t.y);
+                        sum[i & 1] = kv4_add2(sum[i & 1], kv4_pair(x, y));
                         p[i] = kv4_pack(x, y);
                     }
                     kp_st16(tmem + lanes + S0 + slot * KP_N + i0, p);
                 }
-                l += sum[0] + sum[1];
+                const float2 sums = kv4_unpair(kv4_add2(sum[0], sum[1]));
+                l += sums.x + sums.y;
                 kp_wait_st();
                 kp_before();
                 __syncwarp();
