@@ -216,20 +216,16 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
         }
     } else if (warp < SW0 || warp >= SW0 + 4 * NQ) {
         // ------------------------------------------------------------ expand: keys PER e .. of every tile
-        // Pieces of 32 dims of a key, NP a lane: K first, then V.  Where a lane's pieces lie in a block and in a tile does not change.
-        constexpr int CH = D / 32, PER = KP_N / kp_exp<D>, NP = CH * PER / 16;
+        // Pieces of 32 dims of a key, NC of K and of V a lane, half of the head apart.  Where a lane's pieces lie in a block and in a tile does
+        // not change: a pointer for each, and constants from there.
+        constexpr int CH = D / 32, PER = KP_N / kp_exp<D>, NC = CH * PER / 32, HALF = CH / 2;      // HALF: pieces of half a head
         const int e = warp < SW0 ? warp - 1 : warp - (SW0 + 4 * NQ) + SW0 - 1, key = lane & (PER - 1), at = (e * PER + key) % KV4_B;      // at: position in its block of 16
-        const int page_blocks = c.page_size / KV4_B;
+        const int page_blocks = c.page_size / KV4_B, ch = lane / PER;
         const int* table = a.table + (int64_t)b * a.table_stride;
-        int code_at[NP], sb_at[NP]; uint32_t to[NP];
+        const int code_at = (int)kv4_swz((uint32_t)(at * (D / 2) + ch * 16)), sb_at = 16 * D + ((ch >> 1) * 32 + at) * 2;
+        uint32_t to[4];                                                       // (a row of 64 dims: 128 bytes, its 16-byte pieces XORed with the key)
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const int x = lane + 32 * i, v = x / (PER * CH), ch = x / PER % CH;
-            code_at[i] = v * 8 * D + (int)kv4_swz((uint32_t)(at * (D / 2) + ch * 16));
-            sb_at[i] = (16 + v) * D + ((ch >> 1) * 32 + at) * 2;
-            // (a row of 64 dims: 128 bytes, its 16-byte pieces XORed with the key)
-            to[i] = smem0 + v * KP_ST * TILE + (ch >> 1) * (KP_N * 128) + (e * PER + key) * 128 + ((((ch & 1) << 2) ^ (key & 7)) << 4);
-        }
+        for (int x = 0; x < 4; ++x) to[x] = (ch >> 1) * (KP_N * 128) + (e * PER + key) * 128 + (((((ch & 1) << 2) + x) ^ (key & 7)) << 4);
         unsigned long long page_at = 0;                                       // the block of tile (j & ~31) + lane, 0: there is none
         auto block_of = [&](int j) -> const unsigned char* {
             if ((j & 31) == 0) {
@@ -242,36 +238,51 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
             }
             return (const unsigned char*)__shfl_sync(0xffffffffu, page_at, j & 31);
         };
-        struct Raw { uint4 code[NP]; __half s[NP], b[NP]; bool have; };
+        struct Raw { uint4 code[2][NC]; __half s[2][NC], b[2][NC]; bool have; };
         auto fetch = [&](int j, Raw& r) {
             const unsigned char* p = j < tiles ? block_of(j) : nullptr;
             r.have = p != nullptr;
+            auto load = [&] {
+                const unsigned char *code = p + code_at, *other = p + (code_at ^ (HALF * 16)), *sb = p + sb_at;
 #pragma unroll
-            for (int i = 0; i < NP; ++i) { r.code[i] = make_uint4(0, 0, 0, 0); r.s[i] = __ushort_as_half(0); r.b[i] = __ushort_as_half(0); }
-            if (p && j * KP_N + e * PER + key < sq.keys) {                      // (what lies behind the keys stays zero)
+                for (int v = 0; v < 2; ++v)
 #pragma unroll
-                for (int i = 0; i < NP; ++i) {
-                    r.code[i] = *reinterpret_cast<const uint4*>(p + code_at[i]);
-                    const __half* sb = reinterpret_cast<const __half*>(p + sb_at[i]);
-                    r.s[i] = sb[0]; r.b[i] = sb[16];
-                }
+                    for (int k = 0; k < NC; ++k) {
+                        r.code[v][k] = *reinterpret_cast<const uint4*>((k ? other : code) + v * 8 * D);
+                        const __half* h = reinterpret_cast<const __half*>(sb + v * D + k * (HALF / 2) * 64);
+                        r.s[v][k] = h[0]; r.b[v][k] = h[16];
+                    }
+            };
+            if (p && (j + 1) * KP_N <= sq.keys) load();
+            else {                                                            // the last tile, or no page: what lies behind the keys is zero
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+#pragma unroll
+                    for (int k = 0; k < NC; ++k) { r.code[v][k] = make_uint4(0, 0, 0, 0); r.s[v][k] = r.b[v][k] = __ushort_as_half(0); }
+                if (p && j * KP_N + e * PER + key < sq.keys) load();
+                __syncwarp();
             }
         };
         int st = 0; uint32_t ph = 1;                                          // (a fresh barrier passes at 1)
         auto work = [&](int j, const Raw& now) {
             ok = kp_wait(&empty[st], ph, &s_abort);
             if (!ok) return;
+            uint32_t at_x[4];
 #pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const __half2 s = __half2half2(now.s[i]), bi = __half2half2(now.b[i]);
-                const uint32_t w[4] = {now.code[i].x, now.code[i].y, now.code[i].z, now.code[i].w}, row = to[i] + st * TILE;
+            for (int x = 0; x < 4; ++x) at_x[x] = to[x] + st * TILE;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    uint32_t o[4];
-                    kv4_expand(w[x], s, bi, o);
-                    kp_sts(row ^ (uint32_t)(x << 4), make_uint4(o[0], o[1], o[2], o[3]));
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+                for (int k = 0; k < NC; ++k) {
+                    const __half2 s = __half2half2(now.s[v][k]), bi = __half2half2(now.b[v][k]);
+                    const uint32_t w[4] = {now.code[v][k].x, now.code[v][k].y, now.code[v][k].z, now.code[v][k].w};
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        uint32_t o[4];
+                        kv4_expand(w[x], s, bi, o);
+                        *reinterpret_cast<uint4*>(smem + at_x[x] + (v * KP_ST * TILE + k * (HALF / 2) * (KP_N * 128))) = make_uint4(o[0], o[1], o[2], o[3]);
+                    }
                 }
-            }
             if (e * PER % KV4_B == 0 && lane == 0) s_have[j & 7][e * PER / KV4_B] = now.have;      // (read by softmax behind the scores, which wait for this)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -393,9 +404,9 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const float2 t = kv4_unpair(kv4_fma2(kv4_pair(s[2 * (i0 + i)], s[2 * (i0 + i) + 1]), scale2, base2));
-                        const float x = kv4_exp2(t.x), y = kv4_exp2(t.y);
-                        sum[i & 1] = kv4_add2(sum[i & 1], kv4_pair(x, y));
-                        p[i] = kv4_pack(x, y);
+                        const float2 e = make_float2(kv4_exp2(t.x), kv4_exp2(t.y));
+                        sum[i & 1] = kv4_add2(sum[i & 1], kv4_pair(e.x, e.y));
+                        p[i] = kv4_pack(e.x, e.y);
                     }
                     kp_st16(tmem + lanes + S0 + slot * KP_N + i0, p);
                 }
