@@ -357,6 +357,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32) k_kv4_join(Kv4Cache c, Kv4AttnA
     __shared__ int s_ws[KD_WARPS];
     __shared__ __align__(16) float s_o[KD_WARPS][D];
     const int r = blockIdx.x, head = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_launch_dependents();
     kd_prefix(c, a, most, s_pre, s_ws);
     const KdSeq sq = kd_seq(c, a, b, most);
     pdl_wait();                              // (every CTA: what follows this kernel in the stream also follows the one before)
@@ -445,7 +446,7 @@ static int launch_attn(const Kv4Cache& c, const Kv4AttnArgs& a, cudaStream_t st)
     const int tile = many ? 16 : a.max_q * a.G;
     if (a.G <= 16) rc = tile > 8 ? launch_decode<D, 2>(c, a, 16, st) : launch_decode<D, 1>(c, a, 8, st);
     if (rc || !many) return rc;
-    return launch_kv4_prompt(c, a, a.G <= 16 ? 16 : 0, st);
+    return launch_kv4_prompt(c, a, a.G <= 16 ? 16 : 0, st, a.G <= 16);
 }
 int launch_kv4_attn(const Kv4Cache& c, const Kv4AttnArgs& a, cudaStream_t st) {
     return c.D == 64 ? launch_attn<64>(c, a, st) : c.D == 128 ? launch_attn<128>(c, a, st) : launch_attn<256>(c, a, st);

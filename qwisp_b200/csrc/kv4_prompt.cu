@@ -82,14 +82,17 @@ __device__ __forceinline__ bool kp_elect() {
 }
 // Bounded wait of a whole warp.  The first that runs out raises the CTA's abort word, and every later one gives up soon; a role then leaves
 // its loop (nothing in the CTA waits for it unboundedly) and the rows come out as NaN.
-__device__ __forceinline__ bool kp_wait(uint64_t* b, uint32_t parity, volatile int* abort_word) {
-    bool ok = mbar_try_wait(b, parity);
-    for (int i = 0; !ok && i < KP_LIMIT; ++i) {
-        ok = mbar_try_wait(b, parity);
+__device__ __forceinline__ bool kp_wait_one(uint64_t* b, uint32_t parity, volatile int* abort_word) {      // by one thread
+    if (mbar_try_wait(b, parity)) return true;
+    for (int i = 0; i < KP_LIMIT; ++i) {
+        if (mbar_try_wait(b, parity)) return true;
         if ((i & 255) == 255 && *abort_word) break;
     }
-    if (!ok) *abort_word = 1;
-    return __all_sync(0xffffffffu, ok);
+    *abort_word = 1;
+    return false;
+}
+__device__ __forceinline__ bool kp_wait(uint64_t* b, uint32_t parity, volatile int* abort_word) {          // by a whole warp
+    return __all_sync(0xffffffffu, kp_wait_one(b, parity, abort_word));
 }
 
 struct KpSeq { int q0, rows, n, keys; };
@@ -131,8 +134,10 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
         __syncthreads();
         if (s_b >= 0) break;
     }
+    // (Launched ahead of the end of the kernels for few rows, with whose requests it shares nothing.  Every thread waits for them before it
+    // leaves, so that what follows this kernel in the stream follows those too.)
     const int b = s_b;
-    if (b < 0) return;
+    if (b < 0) { pdl_wait(); return; }
     KpSeq sq;
     sq.q0 = a.q_start[b]; sq.n = a.q_start[b + 1] - sq.q0; sq.rows = min(min(sq.n, a.max_q), a.rows - sq.q0);
     sq.keys = min(max(a.kv_len[b], 0), a.table_width * c.page_size);
@@ -163,12 +168,12 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
             constexpr uint32_t ID_S = (1u << 4) | ((uint32_t)(KP_N >> 3) << 17) | ((uint32_t)(KP_M >> 4) << 24);                  // f32 += f16 x f16, K-major B
             constexpr uint32_t ID_O = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(KP_M >> 4) << 24);       // MN-major B
             const uint64_t dk = kp_desc(smem0, 16, 1024), dv = kp_desc(smem0 + KP_ST * TILE, KP_N * 128, 1024);
-            // The whole warp walks the tiles, so that addresses and descriptors stay in uniform registers; one lane, elected once, issues
-            // everything: MMAs are ordered, and their commits count, by thread.
-            const bool leader = kp_elect();
+            // One lane, elected once, does all of it: MMAs are ordered, and their commits count, by thread.  (With the whole warp walking the
+            // tiles, votes and meetings around each wait cost more than the addresses that uniform registers saved.)
+            if (kp_elect()) {
             const uint64_t dq = kp_desc(qs0, 16, 1024);
             auto scores = [&](int q, int slot, uint64_t keys) {
-                if (leader) {
+                {
                     const uint32_t d = tmem + S0 + (2 * q + slot) * KP_N, x = tmem + Q0 + q * (D / 2);
                     const uint64_t y = dq + (uint32_t)(q * (KP_M * D * 2 >> 4));
 #pragma unroll
@@ -179,15 +184,14 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
                     }
                     kp_commit(&s_full[2 * q + slot]);
                 }
-                __syncwarp();
             };
-            ok = kp_wait(&q_full, 0, &s_abort) && kp_wait(&full[0], 0, &s_abort);
+            ok = kp_wait_one(&q_full, 0, &s_abort) && kp_wait_one(&full[0], 0, &s_abort);
             kp_after();
             if (ok) for (int q = 0; q < nq; ++q) scores(q, 0, dk);
             int st = 0, nst = 1; uint32_t nph = 0;                            // stage of tile j and of the next, phase of the next one's
             for (int j = 0; j < tiles && ok; ++j) {
                 const bool more = j + 1 < tiles;
-                if (more) ok = kp_wait(&full[nst], nph, &s_abort) && ok;
+                if (more) ok = kp_wait_one(&full[nst], nph, &s_abort) && ok;
                 kp_after();
                 const uint64_t kn = dk + (uint32_t)(nst * (TILE >> 4)), v = dv + (uint32_t)(st * (TILE >> 4));
                 if (more && ok) {
@@ -197,10 +201,10 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
 #pragma unroll
                 for (int q = 0; q < NQ; ++q) {
                     if (q >= nq || !ok) break;
-                    ok = kp_wait(&p_full[2 * q + (j & 1)], (uint32_t)(j >> 1) & 1u, &s_abort);
+                    ok = kp_wait_one(&p_full[2 * q + (j & 1)], (uint32_t)(j >> 1) & 1u, &s_abort);
                     if (!ok) break;
                     kp_after();
-                    if (leader) {
+                    {
                         const uint32_t d = tmem + q * D, x = tmem + S0 + (2 * q + (j & 1)) * KP_N;
                         kp_mma(d, x, v, ID_O, j > 0 ? 1u : 0u);
 #pragma unroll
@@ -208,10 +212,10 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
                         if (q == nq - 1) kp_commit(&empty[st]);
                         kp_commit(&o_done[2 * q + (j & 1)]);
                     }
-                    __syncwarp();
                 }
                 st = nst;
                 if (++nst == KP_ST) { nst = 0; nph ^= 1u; }
+            }
             }
         }
     } else if (warp < SW0 || warp >= SW0 + 4 * NQ) {
@@ -468,10 +472,11 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
     __syncthreads();
     __syncwarp();
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    pdl_wait();
 }
 
 template <int D>
-static int launch_prompt_t(const Kv4Cache& c, Kv4AttnArgs a, int least, cudaStream_t st) {
+static int launch_prompt_t(const Kv4Cache& c, Kv4AttnArgs a, int least, cudaStream_t st, bool pdl) {
     // a scale below zero, or zero, goes into the queries: the maximum of the scores is that of the scaled ones then
     const uint32_t q_and = a.scale == 0.f ? 0u : 0xffffffffu, q_xor = a.scale < 0.f ? 0x80008000u : 0u;
     a.scale = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
@@ -486,11 +491,11 @@ static int launch_prompt_t(const Kv4Cache& c, Kv4AttnArgs a, int least, cudaStre
     const int per_cta = KP_M / a.G * kp_nq<D>;
     const long long most = (long long)a.rows / per_cta + a.batch;             // (a request's last tile may be short)
     int rc = 0;
-    profile_launch("k_kv4_prompt", st, [&] { return rc = launch_pdl(false, k_kv4_prompt<D>, dim3((unsigned)most, (unsigned)c.KV), kp_threads<D>, kp_smem<D>, st, c, a, least, q_and, q_xor); });
+    profile_launch("k_kv4_prompt", st, [&] { return rc = launch_pdl(pdl, k_kv4_prompt<D>, dim3((unsigned)most, (unsigned)c.KV), kp_threads<D>, kp_smem<D>, st, c, a, least, q_and, q_xor); });
     return rc;
 }
-int launch_kv4_prompt(const Kv4Cache& c, const Kv4AttnArgs& a, int least, cudaStream_t st) {
-    return c.D == 64 ? launch_prompt_t<64>(c, a, least, st) : c.D == 128 ? launch_prompt_t<128>(c, a, least, st) : launch_prompt_t<256>(c, a, least, st);
+int launch_kv4_prompt(const Kv4Cache& c, const Kv4AttnArgs& a, int least, cudaStream_t st, bool pdl) {
+    return c.D == 64 ? launch_prompt_t<64>(c, a, least, st, pdl) : c.D == 128 ? launch_prompt_t<128>(c, a, least, st, pdl) : launch_prompt_t<256>(c, a, least, st, pdl);
 }
 
 }  // namespace sl
