@@ -422,17 +422,18 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
                 if (lane == 0) kp_arrive(&p_full[slot]);
             }
             // ---- normalise, gate, round once; eight columns are the dims 0 4 1 5 2 6 3 7 of a word
+            const int64_t to = place(a.o_row, a.o_head), gates = place(a.g_row, a.g_head);
+            uint4 gate[8];
+            if (a.gate) rows_in(a.gate, gates, 0, gate);
             if (tiles > 0 && ok) ok = kp_wait(&o_done[2 * q + ((tiles - 1) & 1)], (uint32_t)((tiles - 1) >> 1) & 1u, &s_abort);
             kp_after();
             const float inv = l == 0.f ? 0.f : 1.0f / l;
-            const int64_t to = place(a.o_row, a.o_head), gates = place(a.g_row, a.g_head);
 #pragma unroll 1
             for (int d = 0; d < D; d += 64) {
                 if (a.gate) {
-                    uint4 v[8];
-                    rows_in(a.gate, gates, d, v);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) kp_sts(io + turn(i), v[i]);
+                    for (int i = 0; i < 8; ++i) kp_sts(io + turn(i), gate[i]);
+                    if (d + 64 < D) rows_in(a.gate, gates, d + 64, gate);     // (the next dims' on their way)
                 }
                 __syncwarp();
 #pragma unroll
