@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv
     int u = min((long long)blockIdx.x * per, (long long)total);
     const int u1 = min(u + per, total);
     if (u >= u1) return;
-    unsigned char* ring = smem + warp * S * BB;
+    unsigned char* ring = smem + warp * S * U * BB;
     const uint32_t ring_u = smem_u32(ring);
     // ldmatrix: lanes 0-7 the rows of keys 0-7, 8-15 of keys 8-15, 16-31 the same of the next piece
     uint32_t lm[CH / 2];

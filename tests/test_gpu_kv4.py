@@ -378,7 +378,23 @@ def test_attention(case, causal, gated):
     cache, table, q, starts = attention_case(D, NH, KV, page, news, keys)
     gate = torch.randn(q.shape, generator=gen(9), device="cuda").mul_(2).to(F16) if gated else None
     got = ops().kv4_attention(cache, table, ints(keys), q, ints(starts), max(news), causal=causal, gate=gate)
-    near(got, *attention_reference(cache, table, keys, q, starts, causal, D ** -0.5, gate))
+    want = attention_reference(cache, table, keys, q, starts, causal, D ** -0.5, gate)
+    near(got, *want)
+    # the same with a table made for far longer caches, whose work is dealt out in another way
+    wide = torch.nn.functional.pad(table, (0, 70000 // page - table.shape[1]), value=-1)
+    near(ops().kv4_attention(cache, wide, ints(keys), q, ints(starts), max(news), causal=causal, gate=gate), *want)
+
+
+@pytest.mark.parametrize("D,NH,KV,new", [(64, 32, 8, 1), (128, 32, 8, 1), (128, 32, 8, 3), (256, 16, 4, 1), (256, 32, 4, 2)])
+def test_long_caches_of_many_requests(D, NH, KV, new):
+    """So many key blocks that every warp walks its ring many times over, and the same bits again and again."""
+    keys = [new + (i * 977) % 3301 for i in range(48)]
+    news = [new] * len(keys)
+    cache, table, q, starts = attention_case(D, NH, KV, 64, news, keys)
+    first = ops().kv4_attention(cache, table, ints(keys), q, ints(starts), new)
+    near(first, *attention_reference(cache, table, keys, q, starts, True, D ** -0.5))
+    for _ in range(20):
+        assert torch.equal(ops().kv4_attention(cache, table, ints(keys), q, ints(starts), new), first)
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
@@ -477,11 +493,12 @@ def test_maxima_that_rise_along_the_keys(D, news, keys):
         k, v = (torch.randn((n, 2, D), generator=g, device="cuda") for _ in range(2))
         k *= (1 + 4 * p.double() / n).float()[:, None, None] * (1 + (p % 7 == 3).float())[:, None, None]
         ops().kv4_append(cache, table[b].long()[p // 32] * 32 + p % 32, None, k.to(F16), v.to(F16))
-    call = lambda: ops().kv4_attention(cache, table, ints(keys), q, ints(starts), max(news))  # noqa: E731
-    first = call()
-    near(first, *attention_reference(cache, table, keys, q, starts, True, D ** -0.5))
-    for _ in range(100):
-        assert torch.equal(call(), first)
+    for t in (table, torch.nn.functional.pad(table, (0, 1000), value=-1)):
+        call = lambda: ops().kv4_attention(cache, t, ints(keys), q, ints(starts), max(news))  # noqa: E731,B023
+        first = call()
+        near(first, *attention_reference(cache, t, keys, q, starts, True, D ** -0.5))
+        for _ in range(100):
+            assert torch.equal(call(), first)
 
 
 def test_a_long_tail_of_small_weights_counts():
