@@ -19,7 +19,10 @@ namespace sl {
 // four dims of two neighbouring keys for V; both expand to operand registers as they are, and the order of dims inside a step is
 // the queries' (the outputs') to follow.  The running maximum is raised only when a score exceeds it by 2^6; the weights are
 // carried times 2^8, so that fp16 holds them from 2^-32 of the largest on.
-constexpr int KD_WARPS = 4, KD_MAX_BATCH = 4096;
+//
+// CL: for few (request, kv head) pairs of short caches a cluster of eight CTAs takes each, an eighth of its blocks a CTA, and adds the sums up
+// through one another's shared memory: no look at the other requests, no second kernel.
+constexpr int KD_WARPS = 4, KD_MAX_BATCH = 4096, KD_CL = 8;
 template <int D, int NT> constexpr int kd_step = D == 256 || NT == 2 ? 1 : 2;                              // blocks a warp takes at a time
 template <int D> constexpr int kd_stages = D == 256 ? 3 : D == 128 ? 4 : 6;                               // blocks of a warp's ring
 template <int D, int NT> constexpr int kd_ctas = D == 256 ? 2 : NT == 1 ? 4 : 3;                          // CTAs of a multiprocessor
@@ -89,23 +92,44 @@ template <int D, int R> __device__ __forceinline__ float* kd_part(const Kv4AttnA
     return (float*)a.ws + ((size_t)cta * 2 + place) * R * (D + 2);
 }
 
-template <int D, int NT>
+__device__ __forceinline__ void kd_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t kd_peer(const void* p, int rank) {        // the same place in the shared memory of a CTA of the cluster
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+    return r;
+}
+
+template <int D, int NT, bool CL>
 __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv4Cache c, Kv4AttnArgs a, int most, int least) {
     constexpr int R = 8 * NT, U = kd_step<D, NT>, S = kd_stages<D> / U, CH = D / 32, BB = kv4_block_bytes(D), PIECES = BB / 16;
     extern __shared__ __align__(128) unsigned char smem[];
     float* s_o = reinterpret_cast<float*>(smem);                            // [warps][8 rows][D + 4], where the rings were
     int* s_pre = reinterpret_cast<int*>(smem + kd_ring<D>);
-    static_assert(kd_ring<D> >= (size_t)KD_WARPS * 8 * (D + 4) * 4, "");
+    float* s_c = s_o + KD_WARPS * 8 * (D + 4);                               // CL: [R][D], the CTA's sums
+    static_assert(kd_ring<D> >= (size_t)(KD_WARPS * 8 * (D + 4) + R * D) * 4, "");
+    __shared__ float2 s_ml[CL ? R : 1];                                       // CL: their (max, norm)
     __shared__ float s_m[KD_WARPS][R], s_l[KD_WARPS][R];
     __shared__ int s_ws[KD_WARPS];
     __shared__ uint4 s_q[NT * CH][32];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
     pdl_launch_dependents();
-    kd_prefix(c, a, most, s_pre, s_ws);
-    const int total = s_pre[a.batch], per = kd_run(total, gridDim.x, least);
-    int u = min((long long)blockIdx.x * per, (long long)total);
-    const int u1 = min(u + per, total);
-    if (u >= u1) return;
+    int u = 0, u1 = 0, b = blockIdx.y;
+    KdSeq sq;
+    if (CL) {
+        sq = kd_seq(c, a, b, most);
+        if (!sq.units) return;                                                // (the whole cluster)
+    } else {
+        kd_prefix(c, a, most, s_pre, s_ws);
+        const int total = s_pre[a.batch], per = kd_run(total, gridDim.x, least);
+        u = min((long long)blockIdx.x * per, (long long)total);
+        u1 = min(u + per, total);
+        if (u >= u1) return;
+        b = kd_find(s_pre, a.batch, u);
+        sq = kd_seq(c, a, b, most);
+    }
     unsigned char* ring = smem + warp * S * U * BB;
     const uint32_t ring_u = smem_u32(ring);
     // ldmatrix: lanes 0-7 the rows of keys 0-7, 8-15 of keys 8-15, 16-31 the same of the next piece
@@ -113,10 +137,16 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv
 #pragma unroll
     for (int i = 0; i < CH / 2; ++i) lm[i] = kv4_swz((uint32_t)((lane & 15) * (D / 2) + (2 * i + (lane >> 4)) * 16));
     const int page_blocks = c.page_size / KV4_B;
-    int b = kd_find(s_pre, a.batch, u);
-    KdSeq sq = kd_seq(c, a, b, most);
-    while (u < u1) {
-        const int rel = u - s_pre[b], head = rel / sq.units, j0 = rel % sq.units, j1 = min(sq.units, j0 + (u1 - u));
+    while (CL || u < u1) {
+        int head, j0, j1;                                                     // blocks j0 .. of a head
+        if (CL) {
+            const int per = ((sq.units + KD_CL - 1) / KD_CL + U - 1) / U * U;
+            head = blockIdx.x / KD_CL;
+            j0 = min((int)(blockIdx.x % KD_CL) * per, sq.units); j1 = min(j0 + per, sq.units);
+        } else {
+            const int rel = u - s_pre[b];
+            head = rel / sq.units; j0 = rel % sq.units; j1 = min(sq.units, j0 + (u1 - u));
+        }
         const bool whole = j0 == 0 && j1 == sq.units;
         const int n = a.q_start[b + 1] - sq.q0, live = sq.rows * a.G;        // rows of the tile that exist
         // ---- queries: B operands, row g of each N tile; dims 32 i + 8 t .. of piece i in the order that the codes expand in
@@ -336,13 +366,43 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv
                     sum = fmaf(s_l[w][rr], f, sum);
                     v.x = fmaf(y.x, f, v.x); v.y = fmaf(y.y, f, v.y); v.z = fmaf(y.z, f, v.z); v.w = fmaf(y.w, f, v.w);
                 }
-                if (whole) kd_finish(a, sq.q0 + rr / a.G, head * a.G + rr % a.G, d, v, sum);
+                if (CL) {
+                    *reinterpret_cast<float4*>(s_c + rr * D + d) = v;
+                    if (d == 0) s_ml[rr] = make_float2(top, sum);
+                } else if (whole) kd_finish(a, sq.q0 + rr / a.G, head * a.G + rr % a.G, d, v, sum);
                 else {
                     *reinterpret_cast<float4*>(part + (size_t)rr * D + d) = v;
                     if (d == 0) *reinterpret_cast<float2*>(part + (size_t)R * D + 2 * rr) = make_float2(top, sum);
                 }
             }
             __syncthreads();
+        }
+        if (CL) {                                                             // four dims a thread of the cluster
+            kd_cluster_sync();
+            const int x = (int)(blockIdx.x % KD_CL) * (KD_WARPS * 32) + tid, r = x / (D / 4), d = x % (D / 4) * 4;
+            static_assert(R * D / 4 <= KD_CL * KD_WARPS * 32, "");
+            if (r < live) {
+                float2 ml[KD_CL]; float4 y[KD_CL];
+#pragma unroll
+                for (int i = 0; i < KD_CL; ++i) {
+                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml[i].x), "=f"(ml[i].y) : "r"(kd_peer(&s_ml[CL ? r : 0], i)) : "memory");
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(y[i].x), "=f"(y[i].y), "=f"(y[i].z), "=f"(y[i].w) : "r"(kd_peer(s_c + r * D + d, i)) : "memory");
+                }
+                float top = -INFINITY, sum = 0.f;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int i = 0; i < KD_CL; ++i) top = fmaxf(top, ml[i].x);
+#pragma unroll
+                for (int i = 0; i < KD_CL; ++i) {
+                    const float f = ml[i].x == -INFINITY ? 0.f : kv4_exp2(ml[i].x - top);
+                    sum = fmaf(ml[i].y, f, sum);
+                    v.x = fmaf(y[i].x, f, v.x); v.y = fmaf(y[i].y, f, v.y); v.z = fmaf(y[i].z, f, v.z); v.w = fmaf(y[i].w, f, v.w);
+                }
+                kd_finish(a, sq.q0 + r / a.G, head * a.G + r % a.G, d, v, sum);
+            }
+            __syncwarp();
+            kd_cluster_sync();                                                // (nobody leaves while its shared memory is read)
+            return;
         }
         u += j1 - j0;
         if (u < u1 && u >= s_pre[b + 1]) { b = kd_find(s_pre, a.batch, u); sq = kd_seq(c, a, b, most); }
@@ -412,21 +472,38 @@ __global__ void __launch_bounds__(KD_WARPS * 32) k_kv4_join(Kv4Cache c, Kv4AttnA
     kd_finish(a, sq.q0 + r / a.G, head * a.G + r % a.G, d, o, sum);
 }
 constexpr int KD_LEAST = 8;              // units a CTA takes at least
+// Positions x dims of a table's row up to which clusters are taken.  GPU time of a call by clusters | evenly dealt out, us (the call as a program
+// waits for it, launches and all, in brackets): 1 request, 32/8 heads of 128, 1001 positions: 8.2 | 12.3; 4001: 10.3 | 13.3; 8101: 14.4 | 16.4; 16/2
+// of 256, 513: 8.2 | 14.3; 2048: 10.3 | 11.3; 4096: 14.4 | 12.3 [14.7 | 17.5]; 8101: 20.5 | 16.4 [20.6 | 17.3]; 8/1 of 64, 16001: 16.4 | 13.6 [16.5 | 18.9].
+constexpr long long KD_CL_SPAN = 8192 * 128;
+template <int D, int NT, bool CL>
+static int decode_ready(int smem) {      // shared memory, once for each device
+    static std::atomic<unsigned long long> configured{0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 64 && configured.load(std::memory_order_relaxed) >> dev & 1) return 0;
+    const cudaError_t err = cudaFuncSetAttribute(k_kv4_decode<D, NT, CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (err == cudaSuccess && dev < 64) configured.fetch_or(1ull << dev);
+    return (int)err;
+}
 template <int D, int NT>
 static int launch_decode(const Kv4Cache& c, Kv4AttnArgs a, int most, cudaStream_t st) {
     a.scale *= 1.4426950408889634f;
     const int ctas = sm_count() * kd_ctas<D, NT>;
-    const size_t smem = kd_smem<D>(a.batch);
-    static std::atomic<unsigned long long> configured{0};                     // devices
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev >= 64 || !(configured.load(std::memory_order_relaxed) >> dev & 1)) {
-        cudaError_t err = cudaFuncSetAttribute(k_kv4_decode<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kd_smem<D>(KD_MAX_BATCH));
-        if (err != cudaSuccess) return (int)err;
-        if (dev < 64) configured.fetch_or(1ull << dev);
-    }
     int rc = 0;
-    profile_launch("k_kv4_decode", st, [&] { return rc = launch_pdl(false, k_kv4_decode<D, NT>, dim3((unsigned)ctas), KD_WARPS * 32, smem, st, c, a, most, KD_LEAST); });
+    if ((long long)a.batch * c.KV * KD_CL <= ctas && (long long)a.table_width * c.page_size * D <= KD_CL_SPAN) {
+        if ((rc = decode_ready<D, NT, true>((int)kd_ring<D>))) return rc;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(c.KV * KD_CL), (unsigned)a.batch); cfg.blockDim = dim3(KD_WARPS * 32); cfg.dynamicSmemBytes = kd_ring<D>; cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = KD_CL; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr; cfg.numAttrs = 1;
+        profile_launch("k_kv4_decode", st, [&] { return rc = (int)cudaLaunchKernelEx(&cfg, k_kv4_decode<D, NT, true>, c, a, most, 0); });
+        return rc;
+    }
+    if ((rc = decode_ready<D, NT, false>((int)kd_smem<D>(KD_MAX_BATCH)))) return rc;
+    profile_launch("k_kv4_decode", st, [&] { return rc = launch_pdl(false, k_kv4_decode<D, NT, false>, dim3((unsigned)ctas), KD_WARPS * 32, kd_smem<D>(a.batch), st, c, a, most, KD_LEAST); });
     if (rc) return rc;
     profile_launch("k_kv4_join", st, [&] { return rc = launch_pdl(true, k_kv4_join<D, NT>, dim3((unsigned)(a.G * (a.max_q < most / a.G ? a.max_q : most / a.G)), (unsigned)c.KV, (unsigned)a.batch), KD_WARPS * 32, (size_t)(a.batch + 1) * 4, st, c, a, most, KD_LEAST, ctas); });
     return rc;
