@@ -22,7 +22,7 @@ namespace sl {
 //
 // CL: for few (request, kv head) pairs of short caches a cluster of eight CTAs takes each, an eighth of its blocks a CTA, and adds the sums up
 // through one another's shared memory: no look at the other requests, no second kernel.
-constexpr int KD_WARPS = 4, KD_MAX_BATCH = 4096, KD_CL = 8;
+constexpr int KD_WARPS = 4, KD_MAX_BATCH = 4096;
 template <int D, int NT> constexpr int kd_step = D == 256 || NT == 2 ? 1 : 2;                              // blocks a warp takes at a time
 template <int D> constexpr int kd_stages = D == 256 ? 3 : D == 128 ? 4 : 6;                               // blocks of a warp's ring
 template <int D, int NT> constexpr int kd_ctas = D == 256 ? 2 : NT == 1 ? 4 : 3;                          // CTAs of a multiprocessor
@@ -102,7 +102,7 @@ __device__ __forceinline__ uint32_t kd_peer(const void* p, int rank) {        //
     return r;
 }
 
-template <int D, int NT, bool CL>
+template <int D, int NT, int CL>
 __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv4Cache c, Kv4AttnArgs a, int most, int least) {
     constexpr int R = 8 * NT, U = kd_step<D, NT>, S = kd_stages<D> / U, CH = D / 32, BB = kv4_block_bytes(D), PIECES = BB / 16;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -139,10 +139,10 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv
     const int page_blocks = c.page_size / KV4_B;
     while (CL || u < u1) {
         int head, j0, j1;                                                     // blocks j0 .. of a head
-        if (CL) {
-            const int per = ((sq.units + KD_CL - 1) / KD_CL + U - 1) / U * U;
-            head = blockIdx.x / KD_CL;
-            j0 = min((int)(blockIdx.x % KD_CL) * per, sq.units); j1 = min(j0 + per, sq.units);
+        if constexpr (CL != 0) {
+            const int per = ((sq.units + CL - 1) / CL + U - 1) / U * U;
+            head = blockIdx.x / CL;
+            j0 = min((int)(blockIdx.x % CL) * per, sq.units); j1 = min(j0 + per, sq.units);
         } else {
             const int rel = u - s_pre[b];
             head = rel / sq.units; j0 = rel % sq.units; j1 = min(sq.units, j0 + (u1 - u));
@@ -377,23 +377,22 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv
             }
             __syncthreads();
         }
-        if (CL) {                                                             // four dims a thread of the cluster
+        if constexpr (CL != 0) {
             kd_cluster_sync();
-            const int x = (int)(blockIdx.x % KD_CL) * (KD_WARPS * 32) + tid, r = x / (D / 4), d = x % (D / 4) * 4;
-            static_assert(R * D / 4 <= KD_CL * KD_WARPS * 32, "");
-            if (r < live) {
-                float2 ml[KD_CL]; float4 y[KD_CL];
+            for (int x = (int)(blockIdx.x % CL) * (KD_WARPS * 32) + tid; x < live * (D / 4); x += CL * KD_WARPS * 32) {      // four dims a thread
+                const int r = x / (D / 4), d = x % (D / 4) * 4;
+                float2 ml[CL]; float4 y[CL];
 #pragma unroll
-                for (int i = 0; i < KD_CL; ++i) {
-                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml[i].x), "=f"(ml[i].y) : "r"(kd_peer(&s_ml[CL ? r : 0], i)) : "memory");
+                for (int i = 0; i < CL; ++i) {
+                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml[i].x), "=f"(ml[i].y) : "r"(kd_peer(&s_ml[r], i)) : "memory");
                     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(y[i].x), "=f"(y[i].y), "=f"(y[i].z), "=f"(y[i].w) : "r"(kd_peer(s_c + r * D + d, i)) : "memory");
                 }
                 float top = -INFINITY, sum = 0.f;
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int i = 0; i < KD_CL; ++i) top = fmaxf(top, ml[i].x);
+                for (int i = 0; i < CL; ++i) top = fmaxf(top, ml[i].x);
 #pragma unroll
-                for (int i = 0; i < KD_CL; ++i) {
+                for (int i = 0; i < CL; ++i) {
                     const float f = ml[i].x == -INFINITY ? 0.f : kv4_exp2(ml[i].x - top);
                     sum = fmaf(ml[i].y, f, sum);
                     v.x = fmaf(y[i].x, f, v.x); v.y = fmaf(y[i].y, f, v.y); v.z = fmaf(y[i].z, f, v.z); v.w = fmaf(y[i].w, f, v.w);
@@ -475,8 +474,8 @@ constexpr int KD_LEAST = 8;              // units a CTA takes at least
 // Positions x dims of a table's row up to which clusters are taken.  GPU time of a call by clusters | evenly dealt out, us (the call as a program
 // waits for it, launches and all, in brackets): 1 request, 32/8 heads of 128, 1001 positions: 8.2 | 12.3; 4001: 10.3 | 13.3; 8101: 14.4 | 16.4; 16/2
 // of 256, 513: 8.2 | 14.3; 2048: 10.3 | 11.3; 4096: 14.4 | 12.3 [14.7 | 17.5]; 8101: 20.5 | 16.4 [20.6 | 17.3]; 8/1 of 64, 16001: 16.4 | 13.6 [16.5 | 18.9].
-constexpr long long KD_CL_SPAN = 8192 * 128;
-template <int D, int NT, bool CL>
+constexpr long long KD_CL_SPAN = 1024 * 128;
+template <int D, int NT, int CL>
 static int decode_ready(int smem) {      // shared memory, once for each device
     static std::atomic<unsigned long long> configured{0};
     int dev = 0;
@@ -486,24 +485,31 @@ static int decode_ready(int smem) {      // shared memory, once for each device
     if (err == cudaSuccess && dev < 64) configured.fetch_or(1ull << dev);
     return (int)err;
 }
+template <int D, int NT, int CL>
+static int launch_cluster(const Kv4Cache& c, const Kv4AttnArgs& a, int most, cudaStream_t st) {
+    int rc = decode_ready<D, NT, CL>((int)kd_ring<D>);
+    if (rc) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(c.KV * CL), (unsigned)a.batch); cfg.blockDim = dim3(KD_WARPS * 32); cfg.dynamicSmemBytes = kd_ring<D>; cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CL; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    profile_launch("k_kv4_decode", st, [&] { return rc = (int)cudaLaunchKernelEx(&cfg, k_kv4_decode<D, NT, CL>, c, a, most, 0); });
+    return rc;
+}
 template <int D, int NT>
 static int launch_decode(const Kv4Cache& c, Kv4AttnArgs a, int most, cudaStream_t st) {
     a.scale *= 1.4426950408889634f;
     const int ctas = sm_count() * kd_ctas<D, NT>;
     int rc = 0;
-    if ((long long)a.batch * c.KV * KD_CL <= ctas && (long long)a.table_width * c.page_size * D <= KD_CL_SPAN) {
-        if ((rc = decode_ready<D, NT, true>((int)kd_ring<D>))) return rc;
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)(c.KV * KD_CL), (unsigned)a.batch); cfg.blockDim = dim3(KD_WARPS * 32); cfg.dynamicSmemBytes = kd_ring<D>; cfg.stream = st;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = KD_CL; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr; cfg.numAttrs = 1;
-        profile_launch("k_kv4_decode", st, [&] { return rc = (int)cudaLaunchKernelEx(&cfg, k_kv4_decode<D, NT, true>, c, a, most, 0); });
-        return rc;
-    }
-    if ((rc = decode_ready<D, NT, false>((int)kd_smem<D>(KD_MAX_BATCH)))) return rc;
-    profile_launch("k_kv4_decode", st, [&] { return rc = launch_pdl(false, k_kv4_decode<D, NT, false>, dim3((unsigned)ctas), KD_WARPS * 32, kd_smem<D>(a.batch), st, c, a, most, KD_LEAST); });
+    const long long pairs = (long long)a.batch * c.KV, span = (long long)a.table_width * c.page_size * D;
+    if (pairs * 8 <= ctas && span <= 8 * KD_CL_SPAN) return launch_cluster<D, NT, 8>(c, a, most, st);
+    if (pairs * 4 <= ctas && span <= 4 * KD_CL_SPAN) return launch_cluster<D, NT, 4>(c, a, most, st);
+    if (pairs * 2 <= ctas && span <= 2 * KD_CL_SPAN) return launch_cluster<D, NT, 2>(c, a, most, st);
+    if (pairs <= ctas && span <= KD_CL_SPAN) return launch_cluster<D, NT, 1>(c, a, most, st);
+    if ((rc = decode_ready<D, NT, 0>((int)kd_smem<D>(KD_MAX_BATCH)))) return rc;
+    profile_launch("k_kv4_decode", st, [&] { return rc = launch_pdl(false, k_kv4_decode<D, NT, 0>, dim3((unsigned)ctas), KD_WARPS * 32, kd_smem<D>(a.batch), st, c, a, most, KD_LEAST); });
     if (rc) return rc;
     profile_launch("k_kv4_join", st, [&] { return rc = launch_pdl(true, k_kv4_join<D, NT>, dim3((unsigned)(a.G * (a.max_q < most / a.G ? a.max_q : most / a.G)), (unsigned)c.KV, (unsigned)a.batch), KD_WARPS * 32, (size_t)(a.batch + 1) * 4, st, c, a, most, KD_LEAST, ctas); });
     return rc;
