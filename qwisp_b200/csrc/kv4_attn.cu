@@ -87,9 +87,9 @@ __device__ __forceinline__ void kd_finish(const Kv4AttnArgs& a, int row, int h, 
     uint2 r; r.x = *reinterpret_cast<const uint32_t*>(&r0); r.y = *reinterpret_cast<const uint32_t*>(&r1);
     *reinterpret_cast<uint2*>(a.out + row * a.o_row + h * a.o_head + d) = r;
 }
-// Partial sums of a CTA: two places (the item that began before its run, the one that goes on behind it), each [R][D] sums and [R] (max, norm).
+// The workspace: the exclusive sums of the units, then the partial sums of a CTA: two places (the item that began before its run, the one that goes on behind it), each [R][D] sums and [R] (max, norm).
 template <int D, int R> __device__ __forceinline__ float* kd_part(const Kv4AttnArgs& a, int cta, int place) {
-    return (float*)a.ws + ((size_t)cta * 2 + place) * R * (D + 2);
+    return (float*)a.ws + (a.batch + 4) / 4 * 4 + ((size_t)cta * 2 + place) * R * (D + 2);
 }
 
 __device__ __forceinline__ void kd_cluster_sync() {
@@ -123,6 +123,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv
         if (!sq.units) return;                                                // (the whole cluster)
     } else {
         kd_prefix(c, a, most, s_pre, s_ws);
+        if (blockIdx.x == 0) for (int x = tid; x <= a.batch; x += KD_WARPS * 32) ((int*)a.ws)[x] = s_pre[x];      // (for k_kv4_join)
         const int total = s_pre[a.batch], per = kd_run(total, gridDim.x, least);
         u = min((long long)blockIdx.x * per, (long long)total);
         u1 = min(u + per, total);
@@ -149,6 +150,39 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv
         }
         const bool whole = j0 == 0 && j1 == sq.units;
         const int n = a.q_start[b + 1] - sq.q0, live = sq.rows * a.G;        // rows of the tile that exist
+        // ---- the warp's steps of U blocks: warp, + 4, .. of the item's; 32 blocks looked up at a time, a lane each
+        const int mine = max(0, ((j1 - j0 + U - 1) / U - warp + KD_WARPS - 1) / KD_WARPS);
+        const int* table = a.table + (int64_t)b * a.table_stride;
+        auto look = [&](int it) {                                             // the page of the lane's block of the 32 from step `it` on
+            const int j = j0 + (warp + (it + lane / U) * KD_WARPS) * U + lane % U;
+            return j < j1 ? table[j / page_blocks] : -1;
+        };
+        unsigned long long addr = 0;
+        int ahead = look(0);
+        unsigned absent = 0;                                                  // blocks of the ring that there are none of
+        auto issue = [&](int it) {
+            if (it < mine) {
+                if (it % (32 / U) == 0) {
+                    const int j = j0 + (warp + (it + lane / U) * KD_WARPS) * U + lane % U;
+                    addr = ahead >= 0 && ahead < c.pages ? (unsigned long long)kv4_block(c, ahead, head, j % page_blocks) : 0;
+                } else if (it % (32 / U) == 32 / U / 2) ahead = look(it + 32 / U / 2);
+#pragma unroll
+                for (int x = 0; x < U; ++x) {
+                    const unsigned char* src = (const unsigned char*)__shfl_sync(0xffffffffu, addr, it % (32 / U) * U + x);
+                    const int st = it % S * U + x;
+                    absent &= ~(1u << st);
+                    if (src) {
+                        const uint32_t dst = ring_u + st * BB + lane * 16;
+                        src += lane * 16;
+#pragma unroll
+                        for (int i = 0; i < (PIECES + 31) / 32; ++i) if (i < PIECES / 32 || lane < PIECES % 32) kv4_cp16(dst + i * 512, src + i * 512);
+                    } else absent |= 1u << st;
+                }
+            }
+            kv4_commit();
+        };
+#pragma unroll
+        for (int it = 0; it < S - 1; ++it) issue(it);
         // ---- queries: B operands, row g of each N tile; dims 32 i + 8 t .. of piece i in the order that the codes expand in
         for (int x = warp; x < NT * CH; x += KD_WARPS) {
             const int nt = x / CH, ch = x % CH, r = nt * 8 + g, i = r / a.G;
@@ -173,38 +207,6 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv
                 for (int i = 0; i < 8; ++i) o[nt][ch][i >> 2][i & 3] = 0.f;
             base[nt][0] = base[nt][1] = INFINITY; l[nt][0] = l[nt][1] = 0.f;
         }
-        // ---- the warp's steps of U blocks: warp, + 4, .. of the item's; 32 blocks looked up at a time, a lane each
-        const int mine = max(0, ((j1 - j0 + U - 1) / U - warp + KD_WARPS - 1) / KD_WARPS);
-        const int* table = a.table + (int64_t)b * a.table_stride;
-        unsigned long long addr = 0;
-        unsigned absent = 0;                                                  // blocks of the ring that there are none of
-        auto issue = [&](int it) {
-            if (it < mine) {
-                if (it % (32 / U) == 0) {
-                    const int j = j0 + (warp + (it + lane / U) * KD_WARPS) * U + lane % U;
-                    addr = 0;
-                    if (j < j1) {
-                        const int page = table[j / page_blocks];
-                        if (page >= 0 && page < c.pages) addr = (unsigned long long)kv4_block(c, page, head, j % page_blocks);
-                    }
-                }
-#pragma unroll
-                for (int x = 0; x < U; ++x) {
-                    const unsigned char* src = (const unsigned char*)__shfl_sync(0xffffffffu, addr, it % (32 / U) * U + x);
-                    const int st = it % S * U + x;
-                    absent &= ~(1u << st);
-                    if (src) {
-                        const uint32_t dst = ring_u + st * BB + lane * 16;
-                        src += lane * 16;
-#pragma unroll
-                        for (int i = 0; i < (PIECES + 31) / 32; ++i) if (i < PIECES / 32 || lane < PIECES % 32) kv4_cp16(dst + i * 512, src + i * 512);
-                    } else absent |= 1u << st;
-                }
-            }
-            kv4_commit();
-        };
-#pragma unroll
-        for (int it = 0; it < S - 1; ++it) issue(it);
 #pragma unroll 1
         for (int it = 0; it < mine; ++it) {
             kv4_wait<S - 2>();
@@ -412,48 +414,47 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv
 template <int D, int NT>
 __global__ void __launch_bounds__(KD_WARPS * 32) k_kv4_join(Kv4Cache c, Kv4AttnArgs a, int most, int least, int ctas) {
     constexpr int R = 8 * NT, V = D / 32;
-    extern __shared__ int s_pre[];
-    __shared__ int s_ws[KD_WARPS];
     __shared__ __align__(16) float s_o[KD_WARPS][D];
     const int r = blockIdx.x, head = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_launch_dependents();
-    kd_prefix(c, a, most, s_pre, s_ws);
     const KdSeq sq = kd_seq(c, a, b, most);
     pdl_wait();                              // (every CTA: what follows this kernel in the stream also follows the one before)
     if (r >= sq.rows * a.G) return;
-    const int per = kd_run(s_pre[a.batch], ctas, least), u0 = s_pre[b] + head * sq.units, c0 = u0 / per, n = (u0 + sq.units - 1) / per - c0 + 1;
+    const int* pre = (const int*)a.ws;
+    const int per = kd_run(pre[a.batch], ctas, least), u0 = pre[b] + head * sq.units, c0 = u0 / per, n = (u0 + sq.units - 1) / per - c0 + 1;
     if (n == 1) return;
     // piece i: the first CTA's item goes on behind its run, the others' began before theirs
     auto part = [&](int i) { return kd_part<D, R>(a, c0 + i, i > 0 ? 0 : 1); };
     auto ml_of = [&](int i) { return i < n ? *reinterpret_cast<const float2*>(part(i) + (size_t)R * D + 2 * r) : make_float2(-INFINITY, 0.f); };
+    float y[8][V];
+    auto sums = [&](int i0) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = i0 + warp + 4 * k;
+            const float* src = part(i) + (size_t)r * D + lane * V;
+#pragma unroll
+            for (int x = 0; x < V; x += 2) {
+                float2 t = make_float2(0.f, 0.f);
+                if (i < n) t = *reinterpret_cast<const float2*>(src + x);
+                y[k][x] = t.x; y[k][x + 1] = t.y;
+            }
+        }
+    };
     float2 ml = ml_of(lane);
+    sums(0);
     float top = ml.x;
     for (int i = 32; i < n; i += 32) top = fmaxf(top, ml_of(i + lane).x);
     top = warp_max(top);
     float v[V] = {}, sum = 0.f;
     for (int i0 = 0; i0 < n; i0 += 32) {
-        if (i0) ml = ml_of(i0 + lane);
+        if (i0) { ml = ml_of(i0 + lane); sums(i0); }
         const float f = ml.x == -INFINITY ? 0.f : kv4_exp2(ml.x - top);
         sum = fmaf(ml.y, f, sum);
-        {
-            float y[8][V];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int i = warp + 4 * k;
-                const float* src = part(i0 + i) + (size_t)r * D + lane * V;
+        for (int k = 0; k < 8; ++k) {
+            const float fk = __shfl_sync(0xffffffffu, f, warp + 4 * k);
 #pragma unroll
-                for (int x = 0; x < V; x += 2) {
-                    float2 t = make_float2(0.f, 0.f);
-                    if (i0 + i < n) t = *reinterpret_cast<const float2*>(src + x);
-                    y[k][x] = t.x; y[k][x + 1] = t.y;
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float fk = __shfl_sync(0xffffffffu, f, warp + 4 * k);
-#pragma unroll
-                for (int x = 0; x < V; ++x) v[x] = fmaf(y[k][x], fk, v[x]);
-            }
+            for (int x = 0; x < V; ++x) v[x] = fmaf(y[k][x], fk, v[x]);
         }
     }
     sum = warp_sum(sum);
@@ -511,16 +512,16 @@ static int launch_decode(const Kv4Cache& c, Kv4AttnArgs a, int most, cudaStream_
     if ((rc = decode_ready<D, NT, 0>((int)kd_smem<D>(KD_MAX_BATCH)))) return rc;
     profile_launch("k_kv4_decode", st, [&] { return rc = launch_pdl(false, k_kv4_decode<D, NT, 0>, dim3((unsigned)ctas), KD_WARPS * 32, kd_smem<D>(a.batch), st, c, a, most, KD_LEAST); });
     if (rc) return rc;
-    profile_launch("k_kv4_join", st, [&] { return rc = launch_pdl(true, k_kv4_join<D, NT>, dim3((unsigned)(a.G * (a.max_q < most / a.G ? a.max_q : most / a.G)), (unsigned)c.KV, (unsigned)a.batch), KD_WARPS * 32, (size_t)(a.batch + 1) * 4, st, c, a, most, KD_LEAST, ctas); });
+    profile_launch("k_kv4_join", st, [&] { return rc = launch_pdl(true, k_kv4_join<D, NT>, dim3((unsigned)(a.G * (a.max_q < most / a.G ? a.max_q : most / a.G)), (unsigned)c.KV, (unsigned)a.batch), KD_WARPS * 32, 0, st, c, a, most, KD_LEAST, ctas); });
     return rc;
 }
 
 template <int D>
 static size_t decode_workspace(int rows) { return rows > 8 ? (size_t)sm_count() * kd_ctas<D, 2> * 2 * 16 * (D + 2) * 4 : (size_t)sm_count() * kd_ctas<D, 1> * 2 * 8 * (D + 2) * 4; }
 size_t kv4_attn_workspace(int D, int G, int KV, int batch, int max_q, int rows) {
-    (void)KV; (void)batch; (void)rows;
+    (void)KV; (void)rows;
     const int tile = max_q > 16 / G ? 16 : max_q * G;
-    return D == 64 ? decode_workspace<64>(tile) : D == 128 ? decode_workspace<128>(tile) : decode_workspace<256>(tile);
+    return (size_t)(batch + 4) / 4 * 16 + (D == 64 ? decode_workspace<64>(tile) : D == 128 ? decode_workspace<128>(tile) : decode_workspace<256>(tile));
 }
 template <int D>
 static int launch_attn(const Kv4Cache& c, const Kv4AttnArgs& a, cudaStream_t st) {
