@@ -92,16 +92,6 @@ template <int D, int R> __device__ __forceinline__ float* kd_part(const Kv4AttnA
     return (float*)a.ws + (a.batch + 4) / 4 * 4 + ((size_t)cta * 2 + place) * R * (D + 2);
 }
 
-__device__ __forceinline__ void kd_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t kd_peer(const void* p, int rank) {        // the same place in the shared memory of a CTA of the cluster
-    uint32_t r;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
-    return r;
-}
-
 template <int D, int NT, int CL>
 __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv4Cache c, Kv4AttnArgs a, int most, int least) {
     constexpr int R = 8 * NT, U = kd_step<D, NT>, S = kd_stages<D> / U, CH = D / 32, BB = kv4_block_bytes(D), PIECES = BB / 16;
@@ -380,14 +370,14 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv
             __syncthreads();
         }
         if constexpr (CL != 0) {
-            kd_cluster_sync();
+            kv4_cluster_sync();
             for (int x = (int)(blockIdx.x % CL) * (KD_WARPS * 32) + tid; x < live * (D / 4); x += CL * KD_WARPS * 32) {      // four dims a thread
                 const int r = x / (D / 4), d = x % (D / 4) * 4;
                 float2 ml[CL]; float4 y[CL];
 #pragma unroll
                 for (int i = 0; i < CL; ++i) {
-                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml[i].x), "=f"(ml[i].y) : "r"(kd_peer(&s_ml[r], i)) : "memory");
-                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(y[i].x), "=f"(y[i].y), "=f"(y[i].z), "=f"(y[i].w) : "r"(kd_peer(s_c + r * D + d, i)) : "memory");
+                    ml[i] = kv4_peer2(kv4_peer(smem_u32(&s_ml[r]), i));
+                    y[i] = kv4_peer4(kv4_peer(smem_u32(s_c + r * D + d), i));
                 }
                 float top = -INFINITY, sum = 0.f;
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -402,7 +392,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv
                 kd_finish(a, sq.q0 + r / a.G, head * a.G + r % a.G, d, v, sum);
             }
             __syncwarp();
-            kd_cluster_sync();                                                // (nobody leaves while its shared memory is read)
+            kv4_cluster_sync();                                                // (nobody leaves while its shared memory is read)
             return;
         }
         u += j1 - j0;

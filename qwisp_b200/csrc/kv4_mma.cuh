@@ -55,4 +55,25 @@ __device__ __forceinline__ void kv4_expand(uint32_t w, __half2 s, __half2 b, uin
     o[3] = kv4_u(__hfma2(kv4_codes<0x00f000f0u, 0x54005400u>(v), s, b));
 }
 
+// ---- the other CTAs of a cluster: a meeting of all of their threads, and places in their shared memory
+__device__ __forceinline__ void kv4_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t kv4_peer(uint32_t own, int rank) {        // where CTA `rank` has what this one has at `own`
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(own), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float2 kv4_peer2(uint32_t p) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 kv4_peer4(uint32_t p) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(p) : "memory");
+    return v;
+}
+
 }  // namespace sl

@@ -18,15 +18,15 @@
 namespace sl {
 
 constexpr int KP_M = 128, KP_N = 64, KP_ST = 3;
-template <int D> constexpr int kp_nq = D == 256 ? 1 : 2;
-template <int D> constexpr int kp_exp = D == 256 ? 8 : 4;                     // expanding warps: 13 warps in all, 128 registers a thread
-template <int D> constexpr int kp_threads = (1 + kp_exp<D> + 4 * kp_nq<D>) * 32;
+// (D, NQ): two tiles a CTA; D 256: one, whose outputs alone take half of tensor memory
+template <int D> constexpr int kp_exp = D == 256 ? 8 : 4;                     // expanding warps
+template <int D, int NQ> constexpr int kp_threads = (1 + kp_exp<D> + 4 * NQ) * 32;
 template <int D> constexpr int kp_tile = KP_N * D * 2;                        // bytes of a tile of keys or values
-template <int D> constexpr bool kp_qt = D != 128;                            // queries in tensor memory (two tiles of 128 dims: outputs and scores fill it)
-template <int D> constexpr int kp_io = 4 * kp_nq<D> * 4096;                  // where a softmax warp turns 32 rows of 64 dims
-template <int D> constexpr int kp_bytes = 2 * KP_ST * kp_tile<D> + kp_io<D> + (kp_qt<D> ? 0 : kp_nq<D> * KP_M * D * 2);
+template <int D> constexpr bool kp_qt = D != 128;                            // queries in tensor memory (128 dims: outputs and scores fill it)
+template <int D, int NQ> constexpr int kp_io = 4 * NQ * 4096;      // where a softmax warp turns 32 rows of 64 dims
+template <int D, int NQ> constexpr int kp_bytes = 2 * KP_ST * kp_tile<D> + kp_io<D, NQ> + (kp_qt<D> ? 0 : NQ * KP_M * D * 2);
 // (more than half of a multiprocessor's: a second CTA would wait for the first one's tensor memory)
-template <int D> constexpr int kp_smem = (kp_bytes<D> > 120 * 1024 ? kp_bytes<D> : 120 * 1024) + 1024;
+template <int D, int NQ> constexpr int kp_smem = (kp_bytes<D, NQ> > 120 * 1024 ? kp_bytes<D, NQ> : 120 * 1024) + 1024;
 constexpr int KP_LIMIT = 1 << 22;                                            // polls of a wait (up to 4 us each)
 constexpr float KP_UP = 8.0f, KP_SLACK = 6.0f;
 
@@ -95,22 +95,27 @@ __device__ __forceinline__ bool kp_wait(uint64_t* b, uint32_t parity, volatile i
     return __all_sync(0xffffffffu, kp_wait_one(b, parity, abort_word));
 }
 
+// CTAs (clusters) of a kv head at most: a request's last tile may be short
+template <int D, int NQ> static long long kp_items(const Kv4AttnArgs& a) { return (long long)a.rows / (KP_M / a.G * NQ) + a.batch; }
+constexpr int KP_SPLIT = 256;                                                // keys a CTA of a cluster has at least, of a table's span
 struct KpSeq { int q0, rows, n, keys; };
 
-template <int D>
-__global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4AttnArgs a, int least, uint32_t q_and, uint32_t q_xor) {
-    constexpr int NQ = kp_nq<D>, TILE = kp_tile<D>, NT = kp_threads<D>, W = NT / 32, SW0 = 4;      // softmax warps start at SW0
+template <int D, int NQ, int CL>
+__global__ void __launch_bounds__(kp_threads<D, NQ>, 1) k_kv4_prompt(Kv4Cache c, Kv4AttnArgs a, int least, uint32_t q_and, uint32_t q_xor) {
+    constexpr int TILE = kp_tile<D>, NT = kp_threads<D, NQ>, W = NT / 32, SW0 = 4;      // softmax warps start at SW0
     constexpr bool QT = kp_qt<D>;
-    constexpr uint32_t S0 = NQ * D, Q0 = S0 + NQ * 2 * KP_N;                  // columns of tensor memory: outputs, scores (two of each tile), queries
+    constexpr uint32_t S0 = NQ * D, Q0 = S0 + NQ * 2 * KP_N;      // of tensor memory: outputs, scores (two of each tile), queries
     static_assert(Q0 + (QT ? NQ * D / 2 : 0) <= 512, "tensor memory");
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ __align__(8) uint64_t full[KP_ST], empty[KP_ST], s_full[2 * NQ], p_full[2 * NQ], q_full, o_done[2 * NQ];
     __shared__ uint32_t s_tmem;
+    __shared__ float2 s_ml[CL > 1 ? NQ * KP_M : 1];                           // CL > 1: the rows' (maximum, sum)
+    static_assert(CL == 1 || NQ * KP_M * D * 4 <= kp_smem<D, NQ> - 1024, "");
     __shared__ int s_abort, s_b, s_tile, s_sum[W];
     __shared__ __align__(4) uint8_t s_have[8][4];                             // whether a tile's blocks of 16 keys exist (softmax is up to four tiles behind)
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    const int tokens = KP_M / a.G, per_cta = tokens * NQ, head = blockIdx.y;
+    const int tokens = KP_M / a.G, per_cta = tokens * NQ, head = blockIdx.y, item = (int)blockIdx.x / CL;
     // ---- which request, and which of its tiles: the longest of a request first
     if (tid == 0) { s_b = -1; s_abort = 0; }
     __syncthreads();
@@ -129,7 +134,7 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
         int all = 0;
         x += base;
         for (int w = 0; w < W; ++w) { if (w < warp) x += s_sum[w]; all += s_sum[w]; }
-        if ((int)blockIdx.x < x && (int)blockIdx.x >= x - own) { s_b = b; s_tile = x - 1 - (int)blockIdx.x; }
+        if (item < x && item >= x - own) { s_b = b; s_tile = x - 1 - item; }
         base += all;
         __syncthreads();
         if (s_b >= 0) break;
@@ -145,7 +150,9 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
     const int nq = NQ == 1 || t0 + tokens >= sq.rows ? 1 : 2;                 // tiles that have rows
     const int last = min(t0 + per_cta, sq.rows) - 1;
     const int span = a.causal ? min(sq.keys, max(0, sq.keys - sq.n + last + 1)) : sq.keys;
-    const int tiles = (span + KP_N - 1) / KP_N;
+    // keys KP_N j0 .. : all of them, or the cluster's CTAs share them out
+    const int all_tiles = (span + KP_N - 1) / KP_N, per = (all_tiles + CL - 1) / CL, j0 = CL == 1 ? 0 : min((int)(blockIdx.x % CL) * per, all_tiles);
+    const int tiles = CL == 1 ? all_tiles : min(per, all_tiles - j0);
     if (tid == 0) {
         for (int i = 0; i < KP_ST; ++i) { mbar_init(&full[i], kp_exp<D>); mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2 * NQ; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
@@ -160,7 +167,7 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
     kp_before();
     __syncthreads();
     kp_after();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0), smem0 = smem_u32(smem), io0 = smem0 + 2 * KP_ST * TILE, qs0 = io0 + kp_io<D>;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0), smem0 = smem_u32(smem), io0 = smem0 + 2 * KP_ST * TILE, qs0 = io0 + kp_io<D, NQ>;
     bool ok = true;
     if (warp == 0) {
         // ------------------------------------------------------------ mma
@@ -233,7 +240,7 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
         unsigned long long page_at = 0;                                       // the block of tile (j & ~31) + lane, 0: there is none
         auto block_of = [&](int j) -> const unsigned char* {
             if ((j & 31) == 0) {
-                const int blk = (j + lane) * (KP_N / KV4_B) + e * PER / KV4_B, pg = blk / page_blocks;
+                const int blk = (j0 + j + lane) * (KP_N / KV4_B) + e * PER / KV4_B, pg = blk / page_blocks;
                 page_at = 0;
                 if (j + lane < tiles && blk * KV4_B < sq.keys) {
                     const int page = table[pg];
@@ -257,13 +264,13 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
                         r.s[v][k] = h[0]; r.b[v][k] = h[16];
                     }
             };
-            if (p && (j + 1) * KP_N <= sq.keys) load();
+            if (p && (j0 + j + 1) * KP_N <= sq.keys) load();
             else {                                                            // the last tile, or no page: what lies behind the keys is zero
 #pragma unroll
                 for (int v = 0; v < 2; ++v)
 #pragma unroll
                     for (int k = 0; k < NC; ++k) { r.code[v][k] = make_uint4(0, 0, 0, 0); r.s[v][k] = r.b[v][k] = __ushort_as_half(0); }
-                if (p && j * KP_N + e * PER + key < sq.keys) load();
+                if (p && (j0 + j) * KP_N + e * PER + key < sq.keys) load();
                 __syncwarp();
             }
         };
@@ -357,7 +364,7 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
             const int all = a.causal ? min(sq.keys, sq.keys - sq.n + t0 + q * tokens + 1) : sq.keys;
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < tiles && ok; ++j) {
-                const int slot = 2 * q + (j & 1), k0 = j * KP_N;
+                const int slot = 2 * q + (j & 1), k0 = (j0 + j) * KP_N;
                 ok = kp_wait(&s_full[slot], (uint32_t)(j >> 1) & 1u, &s_abort);
                 if (!ok) break;
                 kp_after();
@@ -421,6 +428,21 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
                 __syncwarp();
                 if (lane == 0) kp_arrive(&p_full[slot]);
             }
+            if constexpr (CL > 1) {
+                // ---- the sums as they are, 16-byte pieces XORed with the row, over the ring and the queries (whose last readers were these MMAs)
+                for (int i = 0; i < nq; ++i) if (tiles > 0 && ok) ok = kp_wait(&o_done[2 * i + ((tiles - 1) & 1)], (uint32_t)((tiles - 1) >> 1) & 1u, &s_abort);
+                kp_after();
+                s_ml[q * KP_M + row] = make_float2(m, ok ? l : __int_as_float(0x7fffffff));
+                const uint32_t mine = smem0 + (q * KP_M + row) * (D * 4);
+#pragma unroll 1
+                for (int d = 0; d < D; d += 32) {
+                    uint32_t o[32];
+                    if (tiles > 0) { kp_ld32(tmem + lanes + q * D + d, o); kp_wait_ld(); }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        kp_sts(mine + (((d / 4 + i) ^ (row & 7)) << 4), tiles > 0 && ok ? make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]) : make_uint4(0, 0, 0, 0));
+                }
+            } else {
             // ---- normalise, gate, round once; eight columns are the dims 0 4 1 5 2 6 3 7 of a word
             const int64_t to = place(a.o_row, a.o_head), gates = place(a.g_row, a.g_head);
             uint4 gate[8];
@@ -463,6 +485,7 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
                 }
                 __syncwarp();
             }
+            }
         }
     }
     if (!ok) {                                 // MMAs of this CTA may still be running: outlast them before tensor memory is given back
@@ -471,12 +494,49 @@ __global__ void __launch_bounds__(kp_threads<D>, 1) k_kv4_prompt(Kv4Cache c, Kv4
     }
     kp_before();
     __syncthreads();
+    if constexpr (CL > 1) {
+        // ---- each CTA adds up every CL-th row, eight columns a thread
+        __syncwarp();
+        kv4_cluster_sync();
+        for (int x = tid; x < NQ * KP_M / CL * (D / 8); x += NT) {
+            const int r = x / (D / 8) * CL + (int)(blockIdx.x % CL), d = x % (D / 8) * 8, q = r / KP_M, row = r % KP_M, tok = t0 + q * tokens + row / a.G, h = head * a.G + row % a.G;
+            if (q >= nq || row >= tokens * a.G || tok >= sq.rows) continue;
+            const int64_t at_row = sq.q0 + tok;
+            uint4 g = make_uint4(0, 0, 0, 0);
+            if (a.gate) g = __ldcg(reinterpret_cast<const uint4*>(a.gate + at_row * a.g_row + h * a.g_head + d));
+            const uint32_t p0 = smem0 + r * (D * 4) + (((d / 4) ^ (r & 7)) << 4), p1 = smem0 + r * (D * 4) + (((d / 4 + 1) ^ (r & 7)) << 4);
+            float2 ml[CL];
+            float top = -INFINITY, l = 0.f, v[8] = {};
+#pragma unroll
+            for (int i = 0; i < CL; ++i) { ml[i] = kv4_peer2(kv4_peer(smem_u32(&s_ml[CL > 1 ? r : 0]), i)); top = fmaxf(top, ml[i].x); }
+#pragma unroll
+            for (int i = 0; i < CL; ++i) {
+                const float4 y0 = kv4_peer4(kv4_peer(p0, i)), y1 = kv4_peer4(kv4_peer(p1, i));
+                const float f = ml[i].x == -INFINITY ? 0.f : kv4_exp2(ml[i].x - top);
+                l = fmaf(ml[i].y, f, l);
+                v[0] = fmaf(y0.x, f, v[0]); v[1] = fmaf(y0.y, f, v[1]); v[2] = fmaf(y0.z, f, v[2]); v[3] = fmaf(y0.w, f, v[3]);
+                v[4] = fmaf(y1.x, f, v[4]); v[5] = fmaf(y1.y, f, v[5]); v[6] = fmaf(y1.z, f, v[6]); v[7] = fmaf(y1.w, f, v[7]);
+            }
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            float y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[(k & 1) * 4 + (k >> 1)] = v[k] * inv;
+            if (a.gate) {
+                const __half* gh = reinterpret_cast<const __half*>(&g);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) y[k] *= kv4_sigmoid(h2f(gh[k]));
+            }
+            *reinterpret_cast<uint4*>(a.out + at_row * a.o_row + h * a.o_head + d) = make_uint4(kv4_pack(y[0], y[1]), kv4_pack(y[2], y[3]), kv4_pack(y[4], y[5]), kv4_pack(y[6], y[7]));
+        }
+        __syncwarp();
+        kv4_cluster_sync();                                                   // (nobody leaves while its shared memory is read)
+    }
     __syncwarp();
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     pdl_wait();
 }
 
-template <int D>
+template <int D, int NQ, int CL>
 static int launch_prompt_t(const Kv4Cache& c, Kv4AttnArgs a, int least, cudaStream_t st, bool pdl) {
     // a scale below zero, or zero, goes into the queries: the maximum of the scores is that of the scaled ones then
     const uint32_t q_and = a.scale == 0.f ? 0u : 0xffffffffu, q_xor = a.scale < 0.f ? 0x80008000u : 0u;
@@ -485,18 +545,32 @@ static int launch_prompt_t(const Kv4Cache& c, Kv4AttnArgs a, int least, cudaStre
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 64 || !(configured.load(std::memory_order_relaxed) >> dev & 1)) {
-        cudaError_t err = cudaFuncSetAttribute(k_kv4_prompt<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kp_smem<D>);
+        cudaError_t err = cudaFuncSetAttribute(k_kv4_prompt<D, NQ, CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kp_smem<D, NQ>);
         if (err != cudaSuccess) return (int)err;
         if (dev < 64) configured.fetch_or(1ull << dev);
     }
-    const int per_cta = KP_M / a.G * kp_nq<D>;
-    const long long most = (long long)a.rows / per_cta + a.batch;             // (a request's last tile may be short)
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(kp_items<D, NQ>(a) * CL), (unsigned)c.KV); cfg.blockDim = dim3(kp_threads<D, NQ>); cfg.dynamicSmemBytes = kp_smem<D, NQ>; cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (pdl) { attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[n++].val.programmaticStreamSerializationAllowed = 1; }
+    if (CL > 1) { attr[n].id = cudaLaunchAttributeClusterDimension; attr[n].val.clusterDim.x = CL; attr[n].val.clusterDim.y = 1; attr[n++].val.clusterDim.z = 1; }
+    cfg.attrs = attr; cfg.numAttrs = n;
     int rc = 0;
-    profile_launch("k_kv4_prompt", st, [&] { return rc = launch_pdl(pdl, k_kv4_prompt<D>, dim3((unsigned)most, (unsigned)c.KV), kp_threads<D>, kp_smem<D>, st, c, a, least, q_and, q_xor); });
+    profile_launch("k_kv4_prompt", st, [&] { return rc = (int)cudaLaunchKernelEx(&cfg, k_kv4_prompt<D, NQ, CL>, c, a, least, q_and, q_xor); });
     return rc;
 }
+template <int D, int NQ>
+static int launch_prompt_d(const Kv4Cache& c, const Kv4AttnArgs& a, int least, cudaStream_t st, bool pdl) {
+    const long long ctas = kp_items<D, NQ>(a) * c.KV, span = (long long)a.table_width * c.page_size;
+    const int sms = sm_count();
+    if (ctas * 8 <= sms * 7 / 8 && span >= KP_SPLIT * 8) return launch_prompt_t<D, NQ, 8>(c, a, least, st, pdl);
+    if (ctas * 4 <= sms && span >= KP_SPLIT * 4) return launch_prompt_t<D, NQ, 4>(c, a, least, st, pdl);
+    if (ctas * 2 <= sms && span >= KP_SPLIT * 2) return launch_prompt_t<D, NQ, 2>(c, a, least, st, pdl);
+    return launch_prompt_t<D, NQ, 1>(c, a, least, st, pdl);
+}
 int launch_kv4_prompt(const Kv4Cache& c, const Kv4AttnArgs& a, int least, cudaStream_t st, bool pdl) {
-    return c.D == 64 ? launch_prompt_t<64>(c, a, least, st, pdl) : c.D == 128 ? launch_prompt_t<128>(c, a, least, st, pdl) : launch_prompt_t<256>(c, a, least, st, pdl);
+    return c.D == 64 ? launch_prompt_d<64, 2>(c, a, least, st, pdl) : c.D == 128 ? launch_prompt_d<128, 2>(c, a, least, st, pdl) : launch_prompt_d<256, 1>(c, a, least, st, pdl);
 }
 
 }  // namespace sl
