@@ -19,14 +19,16 @@ namespace sl {
 
 constexpr int KP_M = 128, KP_N = 64, KP_ST = 3;
 // (D, NQ): two tiles a CTA; D 256: one, whose outputs alone take half of tensor memory
+template <int D, int NQ> constexpr int kp_ctas = D == 64 && NQ == 1 ? 2 : 1;   // CTAs of a multiprocessor
 template <int D> constexpr int kp_exp = D == 256 ? 8 : 4;                     // expanding warps
 template <int D, int NQ> constexpr int kp_threads = (1 + kp_exp<D> + 4 * NQ) * 32;
 template <int D> constexpr int kp_tile = KP_N * D * 2;                        // bytes of a tile of keys or values
 template <int D> constexpr bool kp_qt = D != 128;                            // queries in tensor memory (128 dims: outputs and scores fill it)
 template <int D, int NQ> constexpr int kp_io = 4 * NQ * 4096;      // where a softmax warp turns 32 rows of 64 dims
 template <int D, int NQ> constexpr int kp_bytes = 2 * KP_ST * kp_tile<D> + kp_io<D, NQ> + (kp_qt<D> ? 0 : NQ * KP_M * D * 2);
-// (more than half of a multiprocessor's: a second CTA would wait for the first one's tensor memory)
-template <int D, int NQ> constexpr int kp_smem = (kp_bytes<D, NQ> > 120 * 1024 ? kp_bytes<D, NQ> : 120 * 1024) + 1024;
+// (so much that no more CTAs come to a multiprocessor than there is tensor memory for: the next would wait for it)
+template <int D, int NQ> constexpr int kp_least = (kp_ctas<D, NQ> == 2 ? 80 : 120) * 1024;
+template <int D, int NQ> constexpr int kp_smem = (kp_bytes<D, NQ> > kp_least<D, NQ> ? kp_bytes<D, NQ> : kp_least<D, NQ>) + 1024;
 constexpr int KP_LIMIT = 1 << 22;                                            // polls of a wait (up to 4 us each)
 constexpr float KP_UP = 8.0f, KP_SLACK = 6.0f;
 
@@ -101,11 +103,11 @@ constexpr int KP_SPLIT = 256;                                                // 
 struct KpSeq { int q0, rows, n, keys; };
 
 template <int D, int NQ, int CL>
-__global__ void __launch_bounds__(kp_threads<D, NQ>, 1) k_kv4_prompt(Kv4Cache c, Kv4AttnArgs a, int least, uint32_t q_and, uint32_t q_xor) {
+__global__ void __launch_bounds__(kp_threads<D, NQ>, kp_ctas<D, NQ>) k_kv4_prompt(Kv4Cache c, Kv4AttnArgs a, int least, uint32_t q_and, uint32_t q_xor) {
     constexpr int TILE = kp_tile<D>, NT = kp_threads<D, NQ>, W = NT / 32, SW0 = 4;      // softmax warps start at SW0
     constexpr bool QT = kp_qt<D>;
-    constexpr uint32_t S0 = NQ * D, Q0 = S0 + NQ * 2 * KP_N;      // of tensor memory: outputs, scores (two of each tile), queries
-    static_assert(Q0 + (QT ? NQ * D / 2 : 0) <= 512, "tensor memory");
+    constexpr uint32_t S0 = NQ * D, Q0 = S0 + NQ * 2 * KP_N, COLUMNS = 512 / kp_ctas<D, NQ>;      // of tensor memory: outputs, scores (two of each tile), queries
+    static_assert(Q0 + (QT ? NQ * D / 2 : 0) <= COLUMNS, "tensor memory");
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ __align__(8) uint64_t full[KP_ST], empty[KP_ST], s_full[2 * NQ], p_full[2 * NQ], q_full, o_done[2 * NQ];
@@ -161,7 +163,7 @@ __global__ void __launch_bounds__(kp_threads<D, NQ>, 1) k_kv4_prompt(Kv4Cache c,
     }
     if (warp == 0) {
         __syncwarp();
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(COLUMNS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     kp_before();
@@ -369,22 +371,40 @@ __global__ void __launch_bounds__(kp_threads<D, NQ>, 1) k_kv4_prompt(Kv4Cache c,
                 if (!ok) break;
                 kp_after();
                 const uint32_t have = *reinterpret_cast<const uint32_t*>(s_have[j & 7]);
-                uint32_t r[64];
-                kp_ld32(tmem + lanes + S0 + slot * KP_N, r);
-                kp_ld32(tmem + lanes + S0 + slot * KP_N + 32, r + 32);
-                kp_wait_ld();
+                // (two CTAs a multiprocessor: half of the scores at a time, read twice, so that a thread's registers suffice)
+                constexpr int PART = kp_ctas<D, NQ> == 2 ? 32 : 64;
+                uint32_t r[PART];
                 float* s = reinterpret_cast<float*>(r);
-                if (k0 + KP_N > all || have != 0x01010101u) {
+                const bool edge = k0 + KP_N > all || have != 0x01010101u;
+                auto load = [&](int c0) {
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) if (k0 + i >= sees || !(have >> (i >> 4) * 8 & 1)) s[i] = -INFINITY;
+                    for (int i = 0; i < PART; i += 32) kp_ld32(tmem + lanes + S0 + slot * KP_N + c0 + i, r + i);
+                    kp_wait_ld();
+                    if (edge) {
+#pragma unroll
+                        for (int i = 0; i < PART; ++i) if (k0 + c0 + i >= sees || !(have >> ((c0 + i) >> 4) * 8 & 1)) s[i] = -INFINITY;
+                    }
+                };
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c0 = 0; c0 < KP_N; c0 += PART) {
+                    load(c0);
+                    if (PART == KP_N) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mx[k] = s[k];
+#pragma unroll
+                        for (int i = 4; i < PART - 4; i += 8)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) mx[k] = kv4_max3(mx[k], s[i + k], s[i + 4 + k]);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], s[PART - 4 + k]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < PART; i += 8)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) mx[k] = kv4_max3(mx[k], s[i + k], s[i + 4 + k]);
+                    }
                 }
-                float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                for (int i = 4; i < 60; i += 8)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) mx[k] = kv4_max3(mx[k], s[i + k], s[i + 4 + k]);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], s[60 + k]);
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale;
                 if (__any_sync(0xffffffffu, top > m + KP_SLACK)) {
                     const float nm = fmaxf(m, top), f = nm == -INFINITY ? 1.f : kv4_exp2(m - nm);
@@ -410,16 +430,20 @@ __global__ void __launch_bounds__(kp_threads<D, NQ>, 1) k_kv4_prompt(Kv4Cache c,
                 kv4_f2 sum[2] = {0, 0};
                 const kv4_f2 scale2 = kv4_pair(a.scale, a.scale), base2 = kv4_pair(base, base);
 #pragma unroll
-                for (int i0 = 0; i0 < 32; i0 += 16) {
-                    uint32_t p[16];
+                for (int c0 = 0; c0 < KP_N; c0 += PART) {
+                    if (PART < KP_N) load(c0);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float2 t = kv4_unpair(kv4_fma2(kv4_pair(s[2 * (i0 + i)], s[2 * (i0 + i) + 1]), scale2, base2));
-                        const float2 e = make_float2(kv4_exp2(t.x), kv4_exp2(t.y));
-                        sum[i & 1] = kv4_add2(sum[i & 1], kv4_pair(e.x, e.y));
-                        p[i] = kv4_pack(e.x, e.y);
+                    for (int i0 = 0; i0 < PART / 2; i0 += 16) {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float2 t = kv4_unpair(kv4_fma2(kv4_pair(s[2 * (i0 + i)], s[2 * (i0 + i) + 1]), scale2, base2));
+                            const float2 e = make_float2(kv4_exp2(t.x), kv4_exp2(t.y));
+                            sum[i & 1] = kv4_add2(sum[i & 1], kv4_pair(e.x, e.y));
+                            p[i] = kv4_pack(e.x, e.y);
+                        }
+                        kp_st16(tmem + lanes + S0 + slot * KP_N + c0 / 2 + i0, p);
                     }
-                    kp_st16(tmem + lanes + S0 + slot * KP_N + i0, p);
                 }
                 const float2 sums = kv4_unpair(kv4_add2(sum[0], sum[1]));
                 l += sums.x + sums.y;
@@ -532,7 +556,7 @@ __global__ void __launch_bounds__(kp_threads<D, NQ>, 1) k_kv4_prompt(Kv4Cache c,
         kv4_cluster_sync();                                                   // (nobody leaves while its shared memory is read)
     }
     __syncwarp();
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLUMNS) : "memory");
     pdl_wait();
 }
 
@@ -567,6 +591,9 @@ static int launch_prompt_d(const Kv4Cache& c, const Kv4AttnArgs& a, int least, c
     if (ctas * 8 <= sms * 7 / 8 && span >= KP_SPLIT * 8) return launch_prompt_t<D, NQ, 8>(c, a, least, st, pdl);
     if (ctas * 4 <= sms && span >= KP_SPLIT * 4) return launch_prompt_t<D, NQ, 4>(c, a, least, st, pdl);
     if (ctas * 2 <= sms && span >= KP_SPLIT * 2) return launch_prompt_t<D, NQ, 2>(c, a, least, st, pdl);
+    // requests of one tile and more CTAs than multiprocessors: two at once each.  16 x 77 rows, 12 heads, up to 1500 keys: 37 -> 34 us, all of 1500: 46 -> 36,
+    // 40 x 77: 76 -> 64; but 30 x 9, 32/8 heads, up to 809: 28.7 -> 31.4, and where a wave of CTAs is enough, 20 x 50, 8/4 heads, up to 3050: 41 -> 44
+    if constexpr (D == 64) { if (a.max_q * a.G <= KP_M && kp_items<64, 1>(a) * c.KV > sms) return launch_prompt_t<64, 1, 1>(c, a, least, st, pdl); }
     return launch_prompt_t<D, NQ, 1>(c, a, least, st, pdl);
 }
 int launch_kv4_prompt(const Kv4Cache& c, const Kv4AttnArgs& a, int least, cudaStream_t st, bool pdl) {
