@@ -8,6 +8,7 @@
 // a NaN gets a NaN scale: all of it reads back as NaN.
 // k_kv4_read: fp16(code * scale + bias) of K and V at given slots.
 #include "kv4.cuh"
+#include "kv4_mma.cuh"
 
 namespace sl {
 
@@ -219,10 +220,10 @@ __global__ void __launch_bounds__(256) k_kv4_read(Kv4Cache c, Kv4ReadArgs a) {
         const unsigned char* blk = base + head * head_bytes;
         const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(blk + region * 8 * D + kv4_swz((uint32_t)(at * (D / 2) + hl * 4))));
         const __half* sb = reinterpret_cast<const __half*>(blk + (16 + region) * D) + (hl >> 3) * 2 * KV4_B + at;
-        const float s = h2f(__ldg(sb)), b = h2f(__ldg(sb + KV4_B));
-        uint4 o; __half* oh = reinterpret_cast<__half*>(&o);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) oh[j] = f2h(fmaf((float)(w >> (4 * j) & 15u), s, b));
+        const __half2 s = __half2half2(__ldg(sb)), b = __half2half2(__ldg(sb + KV4_B));
+        uint32_t x[4];
+        kv4_expand(w, s, b, x);                                               // (dims 0 4, 1 5, 2 6, 3 7)
+        const uint4 o = make_uint4(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410), __byte_perm(x[0], x[1], 0x7632), __byte_perm(x[2], x[3], 0x7632));
         __half* dst = region ? a.v + row * a.v_row + head * a.v_head : a.k + row * a.k_row + head * a.k_head;
         reinterpret_cast<uint4*>(dst)[hl] = o;
     }
