@@ -323,7 +323,7 @@ typedef struct sl_kv4_cache {
     int64_t page_stride;     /* bytes from a page to the next: sl_kv4_page_bytes() or more (several layers in one page), a multiple of 16 */
     int32_t pages;
     int32_t page_size;       /* positions, a multiple of 16 */
-    int32_t kv_heads;
+    int32_t kv_heads;        /* up to 65535, like the query heads of sl_kv4_append */
     int32_t head_dim;        /* 64, 128 or 256 */
 } sl_kv4_cache;
 /* Bytes of one page of one layer, or SL_ERR_INVALID. */
@@ -376,7 +376,8 @@ int32_t sl_op_kv4_read_device(const sl_kv4_cache* cache, const sl_kv4_read* rows
 /* out = softmax(scale * q K^T) V [* sigmoid(gate)] for the rows q_start[b] .. q_start[b + 1] - 1 of every request b over its positions
  * 0 .. kv_len[b] - 1; query head h reads kv head h / (q_heads / kv_heads), at most 128 of them one kv head; at most 4096 requests.  causal: row i of a request's n
  * sees the first kv_len - n + i + 1 positions.  A row that sees none is zero; table entries that are no page of the cache hold no keys; rows of
- * no request, and rows of a request behind its first max_q, are left as they were.
+ * no request, and rows of a request behind its first max_q, are left as they were.  The requests' rows do not overlap.  Infinities and NaN in places
+ * that a row does not see do not count, unless another row of its request sees them: then this row may be NaN too.
  * workspace: 16-byte aligned, sl_kv4_attention_workspace() bytes (the same arguments), any contents; calls that may run at the same
  * time need one each. */
 typedef struct sl_kv4_attention {

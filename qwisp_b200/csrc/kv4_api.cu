@@ -7,10 +7,11 @@
 using namespace sl;
 
 namespace {
+constexpr int KV4_HEADS = 65535;                             // (a grid's second axis)
 bool aligned(const void* p, int64_t row, int64_t head) { return ((uintptr_t)p & 15) == 0 && row % 8 == 0 && head % 8 == 0; }
 // a cache that the kernels can address; its geometry as they take it
 bool cache_of(const sl_kv4_cache* c, Kv4Cache& o) {
-    if (!c || !c->data || ((uintptr_t)c->data & 15) || c->pages <= 0 || c->kv_heads <= 0 || c->page_size <= 0 || c->page_size % KV4_B) return false;
+    if (!c || !c->data || ((uintptr_t)c->data & 15) || c->pages <= 0 || c->kv_heads <= 0 || c->kv_heads > KV4_HEADS || c->page_size <= 0 || c->page_size % KV4_B) return false;
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return false;
     if (c->page_stride % 16 || c->page_stride < sl_kv4_page_bytes(c->kv_heads, c->head_dim, c->page_size)) return false;
     o = Kv4Cache{(unsigned char*)c->data, c->page_stride, c->pages, c->page_size, c->kv_heads, c->head_dim};
@@ -45,7 +46,7 @@ int32_t sl_op_kv_plan_device(const sl_kv_plan* p, void* cuda_stream) try {
 }
 int32_t sl_op_kv4_append_device(const sl_kv4_cache* cache, const sl_kv4_append* p, void* cuda_stream) try {
     Kv4Cache c{};
-    if (!p || !cache_of(cache, c) || p->rows < 0 || p->q_heads < 0 || (!p->q && !p->k) || !p->k != !p->v) return SL_ERR_INVALID;
+    if (!p || !cache_of(cache, c) || p->rows < 0 || p->q_heads < 0 || p->q_heads > KV4_HEADS || (!p->q && !p->k) || !p->k != !p->v) return SL_ERR_INVALID;
     if (p->q && (!p->q_out || p->q_heads == 0 || !aligned(p->q, p->q_row, p->q_head) || !aligned(p->q_out, p->q_out_row, p->q_out_head))) return SL_ERR_INVALID;
     if (p->k && (!p->slots || !aligned(p->k, p->k_row, p->k_head) || !aligned(p->v, p->v_row, p->v_head))) return SL_ERR_INVALID;
     if (!aligned(p->q_norm, 0, 0) || !aligned(p->k_norm, 0, 0) || !(p->eps >= 0.f)) return SL_ERR_INVALID;

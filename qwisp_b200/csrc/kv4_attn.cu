@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv
         const int* table = a.table + (int64_t)b * a.table_stride;
         auto look = [&](int it) {                                             // the page of the lane's block of the 32 from step `it` on
             const int j = j0 + (warp + (it + lane / U) * KD_WARPS) * U + lane % U;
-            return j < j1 ? table[j / page_blocks] : -1;
+            return j < j1 && j * KV4_B < sq.keys ? table[j / page_blocks] : -1;      // (an item without keys has a block that is none)
         };
         unsigned long long addr = 0;
         int ahead = look(0);

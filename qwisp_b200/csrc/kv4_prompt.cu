@@ -593,7 +593,7 @@ static int launch_prompt_d(const Kv4Cache& c, const Kv4AttnArgs& a, int least, c
     if (ctas * 2 <= sms && span >= KP_SPLIT * 2) return launch_prompt_t<D, NQ, 2>(c, a, least, st, pdl);
     // requests of one tile and more CTAs than multiprocessors: two at once each.  16 x 77 rows, 12 heads, up to 1500 keys: 37 -> 34 us, all of 1500: 46 -> 36,
     // 40 x 77: 76 -> 64; but 30 x 9, 32/8 heads, up to 809: 28.7 -> 31.4, and where a wave of CTAs is enough, 20 x 50, 8/4 heads, up to 3050: 41 -> 44
-    if constexpr (D == 64) { if (a.max_q * a.G <= KP_M && kp_items<64, 1>(a) * c.KV > sms) return launch_prompt_t<64, 1, 1>(c, a, least, st, pdl); }
+    if constexpr (D == 64) { if (a.max_q <= KP_M / a.G && kp_items<64, 1>(a) * c.KV > sms) return launch_prompt_t<64, 1, 1>(c, a, least, st, pdl); }
     return launch_prompt_t<D, NQ, 1>(c, a, least, st, pdl);
 }
 int launch_kv4_prompt(const Kv4Cache& c, const Kv4AttnArgs& a, int least, cudaStream_t st, bool pdl) {

@@ -425,6 +425,21 @@ def test_what_lies_behind_the_keys_does_not_count(D, news, keys):
     near(got, *attention_reference(cache, holes, keys, q, starts, True, D ** -0.5))
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 3, 70])
+@pytest.mark.parametrize("width", [0, 1, 5000])
+def test_requests_without_positions(D, n, width):
+    """No keys at all, in tables of no columns too: zeros, whatever the tables hold."""
+    cache = random_cache(2, 16, 2, D, 3)
+    table = torch.full((3, width), 1 << 30, dtype=I32, device="cuda")
+    q = torch.randn((3 * n, 8, D), generator=gen(4), device="cuda").to(F16)
+    for causal in (False, True):
+        for lens in ([0, 0, 0], [-5, 0, 0]):
+            out = torch.full_like(q, 7.0)
+            ops().kv4_attention(cache, table, ints(lens), q, ints([0, n, 2 * n, 3 * n]), n, causal=causal, out=out)
+            assert (out == 0).all()
+
+
 @pytest.mark.parametrize("n", [1, 70])
 def test_rows_that_belong_to_nobody_stay_as_they_were(n):
     cache, table, q, starts = attention_case(128, 8, 2, 64, [n, n + 4, n], [100, 200, 50])

@@ -44,7 +44,7 @@ def call(name, *structs):
 
 
 @pytest.mark.parametrize("kw", [dict(data=None), dict(data=P + 8), dict(pages=0), dict(pages=-1), dict(page_size=0), dict(page_size=24), dict(kv_heads=0),
-                                dict(head_dim=96), dict(page_stride=2 * 4 * 18 * 128 - 16), dict(page_stride=2 * 4 * 18 * 128 + 8)])
+                                dict(head_dim=96), dict(kv_heads=65536, page_stride=65536 * 4 * 18 * 128), dict(page_stride=2 * 4 * 18 * 128 - 16), dict(page_stride=2 * 4 * 18 * 128 + 8)])
 def test_caches_that_cannot_be_addressed_are_refused(kw):
     c = cache(**kw)
     assert call("sl_op_kv4_append_device", c, append()) == INVALID
@@ -59,7 +59,7 @@ def test_plan_refusals(kw):
     assert call("sl_op_kv_plan_device", plan(**kw)) == INVALID
 
 
-@pytest.mark.parametrize("kw", [dict(q=None, k=None, v=None), dict(v=None), dict(k=None), dict(q_out=None), dict(q_heads=0), dict(q_heads=-1), dict(rows=-1), dict(q=P + 2),
+@pytest.mark.parametrize("kw", [dict(q=None, k=None, v=None), dict(v=None), dict(k=None), dict(q_out=None), dict(q_heads=0), dict(q_heads=-1), dict(q_heads=65536), dict(rows=-1), dict(q=P + 2),
                                 dict(q_row=2044), dict(k_head=100), dict(v_row=12), dict(q_out_head=4), dict(q_norm=P + 8), dict(eps=-1.0), dict(eps=float("nan")),
                                 dict(slots=None), dict(pos=None), dict(rope_dims=24), dict(rope_dims=144), dict(rope_dims=-16), dict(axes=0),
                                 dict(rope_theta=0.5), dict(rope_theta=float("inf")), dict(rope_theta=float("nan")), dict(axis_of=bytes([1] * 32))])
