@@ -20,8 +20,15 @@ namespace sl {
 // the queries' (the outputs') to follow.  The running maximum is raised only when a score exceeds it by 2^6; the weights are
 // carried times 2^8, so that fp16 holds them from 2^-32 of the largest on.
 //
-// CL: for few (request, kv head) pairs of short caches a cluster of eight CTAs takes each, an eighth of its blocks a CTA, and adds the sums up
-// through one another's shared memory: no look at the other requests, no second kernel.
+// CL: a cluster of 8, 4, 2 or 1 CTAs takes a (request, kv head), a share of its blocks a CTA, and adds the sums up through one another's shared
+// memory: no look at the other requests, no second kernel; for tables so narrow that no CTA's share gets long (KD_CL_SPAN).
+//
+// What bounds it, 64 requests of up to 8192 positions, 32/8 heads of 128: 102 us, 3.8 TB/s = 0.58 of the measured copy rate (floor 60 us).  The memory
+// alone, expansion left out, took 74 us; the expansion alone 100: a word of eight codes is 4 LOP3, 4 subtractions and 4 multiply-adds in half
+// precision, all pipes of half rate, about 25 cycles of a scheduler with the scores' and weights' share.  Requests of up to 30000: 308 us, 0.71.
+// 16 warps a multiprocessor (registers), two blocks a step, so that one block's MMAs cover the other one's expansion; more warps, deeper rings and
+// expansion by integer shifts alone were no faster.  One request of 513 positions, 16/2 heads of 256: 8.2 us, latency: the launch, five dependent loads
+// (lengths, table, codes), 5 key blocks a warp, two meetings of the cluster.
 constexpr int KD_WARPS = 4, KD_MAX_BATCH = 4096;
 template <int D, int NT> constexpr int kd_step = D == 256 || NT == 2 ? 1 : 2;                              // blocks a warp takes at a time
 template <int D> constexpr int kd_stages = D == 256 ? 3 : D == 128 ? 4 : 6;                               // blocks of a warp's ring
@@ -462,9 +469,10 @@ __global__ void __launch_bounds__(KD_WARPS * 32) k_kv4_join(Kv4Cache c, Kv4AttnA
     kd_finish(a, sq.q0 + r / a.G, head * a.G + r % a.G, d, o, sum);
 }
 constexpr int KD_LEAST = 8;              // units a CTA takes at least
-// Positions x dims of a table's row up to which clusters are taken.  GPU time of a call by clusters | evenly dealt out, us (the call as a program
-// waits for it, launches and all, in brackets): 1 request, 32/8 heads of 128, 1001 positions: 8.2 | 12.3; 4001: 10.3 | 13.3; 8101: 14.4 | 16.4; 16/2
-// of 256, 513: 8.2 | 14.3; 2048: 10.3 | 11.3; 4096: 14.4 | 12.3 [14.7 | 17.5]; 8101: 20.5 | 16.4 [20.6 | 17.3]; 8/1 of 64, 16001: 16.4 | 13.6 [16.5 | 18.9].
+// Positions x dims of a table's row for each CTA of a cluster, at most: 1024 positions of 128.  GPU time of a call by clusters | evenly dealt out, us
+// (the call as a program waits for it, launches and all, in brackets).  Heads of 128, 32/8: 1 x 1001 positions 8.2 | 12.3, 1 x 4001 10.3 | 13.3, 1 x 8101
+// 14.4 | 16.4, 7 x (2000 + 4) 14.4 | 20.3, 16 x 1001 12.2 | 16.4, 64 x up to 1001 22.9 | 32.2.  16/2 of 256: 1 x 513 8.2 | 14.3, 1 x 2048 10.3 | 11.3, 1 x 4096
+// 14.4 | 12.3 [14.7 | 17.5], 1 x 8101 20.5 | 16.4.  8/1 of 64: 1 x 16001 16.4 | 13.6 [16.5 | 18.9].  Four CTAs for 16 x up to 8101 of 128: 36.9 | 35.4.
 constexpr long long KD_CL_SPAN = 1024 * 128;
 template <int D, int NT, int CL>
 static int decode_ready(int smem) {      // shared memory, once for each device

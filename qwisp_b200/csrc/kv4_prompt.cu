@@ -11,7 +11,16 @@
 //   softmax   4 warps a tile, a thread a row: scores in, running maximum and sum in registers, weights out.  The maximum is raised (and the
 //             outputs rescaled) only when a score exceeds it by 2^6; the weights are carried times 2^8, so that fp16 holds them from 2^-32 of the
 //             largest on.
-// NQ = 2 (D 64, 128): the expansion serves two tiles.  NQ = 1 (D 256): the outputs of one take half of tensor memory.
+// NQ = 2 (D 64, 128): the expansion serves two tiles.  NQ = 1 (D 256): the outputs of one take half of tensor memory; (D 64) requests of one tile.
+// CL > 1: where there are fewer tiles than multiprocessors a cluster of CTAs takes each, a run of the keys a CTA, and adds up its sums through shared
+// memory.  17 rows over 4017 positions, 32/8 heads of 128: 55 us with one CTA, 18.5 with eight.
+//
+// What bounds it: 1024 rows over 8192 positions, 16/2 heads of 256: 136 us, 0.95 PFLOP/s = 0.56 of the measured cuBLAS rate; four prompts of up to
+// 2900, 32/8 heads of 128: 238 us, 0.72 PFLOP/s = 0.43.  No unit is full (tensor pipe 39 %, MUFU 40 %, ALU 33 %, issue slots 43 % of the second): each tile of
+// 64 keys is a chain scores -> exponents -> weights -> outputs over barriers, which two tiles of rows overlap only in part, and every CTA begins
+// and ends alone (about 10 of 31 us there).  Leaving out the exponentials gave 12 %, the expansion 5 %, half of the MMAs nothing.  Tried, and no faster:
+// tiles of 128 keys with one score buffer (238 -> 254), two CTAs of one tile each (430: twice the expansion, 96 registers), more expanding
+// warps with registers moved between the roles, a polynomial in place of some MUFU exponentials.
 #include "kv4.cuh"
 #include "kv4_mma.cuh"
 
@@ -114,6 +123,7 @@ __global__ void __launch_bounds__(kp_threads<D, NQ>, kp_ctas<D, NQ>) k_kv4_promp
     __shared__ uint32_t s_tmem;
     __shared__ float2 s_ml[CL > 1 ? NQ * KP_M : 1];                           // CL > 1: the rows' (maximum, sum)
     static_assert(CL == 1 || NQ * KP_M * D * 4 <= kp_smem<D, NQ> - 1024, "");
+    __shared__ KpSeq s_seq;
     __shared__ int s_abort, s_b, s_tile, s_sum[W];
     __shared__ __align__(4) uint8_t s_have[8][4];                             // whether a tile's blocks of 16 keys exist (softmax is up to four tiles behind)
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -124,9 +134,11 @@ __global__ void __launch_bounds__(kp_threads<D, NQ>, kp_ctas<D, NQ>) k_kv4_promp
     for (int b0 = 0, base = 0; b0 < a.batch; b0 += NT) {
         const int b = b0 + tid;
         int x = 0;
+        KpSeq one{0, 0, 0, 0};
         if (b < a.batch) {
-            const int q0 = a.q_start[b], rows = min(min(a.q_start[b + 1] - q0, a.max_q), a.rows - q0);
-            if (q0 >= 0 && rows > least / a.G) x = (rows + per_cta - 1) / per_cta;
+            one.q0 = a.q_start[b]; one.n = a.q_start[b + 1] - one.q0; one.rows = min(min(one.n, a.max_q), a.rows - one.q0);
+            one.keys = min(max(a.kv_len[b], 0), a.table_width * c.page_size);
+            if (one.q0 >= 0 && one.rows > least / a.G) x = (one.rows + per_cta - 1) / per_cta;
         }
         const int own = x;
 #pragma unroll
@@ -136,7 +148,7 @@ __global__ void __launch_bounds__(kp_threads<D, NQ>, kp_ctas<D, NQ>) k_kv4_promp
         int all = 0;
         x += base;
         for (int w = 0; w < W; ++w) { if (w < warp) x += s_sum[w]; all += s_sum[w]; }
-        if (item < x && item >= x - own) { s_b = b; s_tile = x - 1 - item; }
+        if (item < x && item >= x - own) { s_b = b; s_tile = x - 1 - item; s_seq = one; }
         base += all;
         __syncthreads();
         if (s_b >= 0) break;
@@ -145,9 +157,7 @@ __global__ void __launch_bounds__(kp_threads<D, NQ>, kp_ctas<D, NQ>) k_kv4_promp
     // leaves, so that what follows this kernel in the stream follows those too.)
     const int b = s_b;
     if (b < 0) { pdl_wait(); return; }
-    KpSeq sq;
-    sq.q0 = a.q_start[b]; sq.n = a.q_start[b + 1] - sq.q0; sq.rows = min(min(sq.n, a.max_q), a.rows - sq.q0);
-    sq.keys = min(max(a.kv_len[b], 0), a.table_width * c.page_size);
+    const KpSeq sq = s_seq;
     const int t0 = s_tile * per_cta;                                          // first token
     const int nq = NQ == 1 || t0 + tokens >= sq.rows ? 1 : 2;                 // tiles that have rows
     const int last = min(t0 + per_cta, sq.rows) - 1;
@@ -591,8 +601,12 @@ static int launch_prompt_d(const Kv4Cache& c, const Kv4AttnArgs& a, int least, c
     if (ctas * 8 <= sms * 7 / 8 && span >= KP_SPLIT * 8) return launch_prompt_t<D, NQ, 8>(c, a, least, st, pdl);
     if (ctas * 4 <= sms && span >= KP_SPLIT * 4) return launch_prompt_t<D, NQ, 4>(c, a, least, st, pdl);
     if (ctas * 2 <= sms && span >= KP_SPLIT * 2) return launch_prompt_t<D, NQ, 2>(c, a, least, st, pdl);
+    if constexpr (D == 64) {                                                  // (two CTAs a multiprocessor) 20 x 50 rows, 8/4 heads, up to 3050 keys: 41 -> 35 us
+        if (a.max_q <= KP_M / a.G && kp_items<64, 1>(a) * c.KV <= sms && span >= KP_SPLIT * 2) return launch_prompt_t<64, 1, 2>(c, a, least, st, pdl);
+    }
     // requests of one tile and more CTAs than multiprocessors: two at once each.  16 x 77 rows, 12 heads, up to 1500 keys: 37 -> 34 us, all of 1500: 46 -> 36,
-    // 40 x 77: 76 -> 64; but 30 x 9, 32/8 heads, up to 809: 28.7 -> 31.4, and where a wave of CTAs is enough, 20 x 50, 8/4 heads, up to 3050: 41 -> 44
+    // 40 x 77: 76 -> 64; 20 x 50, 8/8, up to 350: 18.5 -> 16.6;
+    // but 30 x 9, 32/8 heads, up to 809: 28.7 -> 31.4
     if constexpr (D == 64) { if (a.max_q <= KP_M / a.G && kp_items<64, 1>(a) * c.KV > sms) return launch_prompt_t<64, 1, 1>(c, a, least, st, pdl); }
     return launch_prompt_t<D, NQ, 1>(c, a, least, st, pdl);
 }

@@ -8,6 +8,8 @@
 //
 // A few hundred requests are bound by latency alone (three dependent loads and the launch), so one CTA does everything: sums, pages and,
 // up to PLAN_ROWS of them, the rows.  More rows get a kernel of their own over the whole device.
+// 64 requests of a row each: 6.2 us (256 threads; 1024 take longer to start and to meet).  700 requests of up to 4001 positions and 509 rows in pages of
+// 16: 18.5 us, two kernels that take 14.5 and 8.7 by themselves; the first is the chain lengths -> sums -> pages -> offsets, with a bisection for each page.
 #include "kv4.cuh"
 
 namespace sl {
