@@ -392,6 +392,8 @@ typedef struct sl_kv4_attention {
     void* workspace; uint64_t workspace_bytes;
 } sl_kv4_attention;
 int64_t sl_kv4_attention_workspace(int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t batch, int32_t max_q, int32_t rows);
+/* The same for tables of `span` positions a row (table_width * page_size): 0 where such a call uses none (workspace is then any aligned place). */
+int64_t sl_kv4_attention_workspace_span(int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t batch, int32_t max_q, int64_t span);
 int32_t sl_op_kv4_attention_device(const sl_kv4_cache* cache, const sl_kv4_attention* call, void* cuda_stream);
 
 /* ---- synthetic data helpers (same generator as the engine's weights) ---- */

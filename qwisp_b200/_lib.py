@@ -145,6 +145,7 @@ SYMBOLS = {
     "sl_op_kv4_append_device": (_I32, [_VP, _VP, _VP]),
     "sl_op_kv4_read_device": (_I32, [_VP, _VP, _VP]),
     "sl_kv4_attention_workspace": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32]),
+    "sl_kv4_attention_workspace_span": (_I64, [_I32, _I32, _I32, _I32, _I32, _I64]),
     "sl_op_kv4_attention_device": (_I32, [_VP, _VP, _VP]),
     "sl_synth_tokens": (_I32, [_U64, C.c_char_p, _I64, _I32, _VP]),
     "sl_synth_f16": (_I32, [_U64, C.c_char_p, _I64, _F, _F, _VP]),

@@ -65,7 +65,7 @@ struct Kv4AttnArgs {
 int launch_kv_plan(const KvPlanArgs& a, cudaStream_t st);
 int launch_kv4_append(const Kv4Cache& c, const Kv4AppendArgs& a, cudaStream_t st);
 int launch_kv4_read(const Kv4Cache& c, const Kv4ReadArgs& a, cudaStream_t st);
-size_t kv4_attn_workspace(int D, int G, int KV, int batch, int max_q, int rows);
+size_t kv4_attn_workspace(int D, int G, int KV, int batch, int max_q, long long span);      // span: positions of a table's row, -1: any
 // requests of more than `least` rows a kv head; pdl: the kernel before it in the stream is one of this call's
 int launch_kv4_prompt(const Kv4Cache& c, const Kv4AttnArgs& a, int least, cudaStream_t st, bool pdl);
 int launch_kv4_attn(const Kv4Cache& c, const Kv4AttnArgs& a, cudaStream_t st);

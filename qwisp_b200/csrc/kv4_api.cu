@@ -1,6 +1,7 @@
 // kv4_api.cu -- C entry points of the operators around the cache held in 4 bits: arguments checked, then the kernel enqueued.
 #include "../../include/seedless_b200.h"
 #include "kv4.cuh"
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 
@@ -87,7 +88,11 @@ int32_t sl_op_kv4_read_device(const sl_kv4_cache* cache, const sl_kv4_read* p, v
 int64_t sl_kv4_attention_workspace(int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t batch, int32_t max_q, int32_t rows) {
     if (kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || batch < 0 || max_q < 1 || rows < 0 || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return SL_ERR_INVALID;
     if (q_heads / kv_heads > 128) return SL_ERR_CAPACITY;
-    return (int64_t)kv4_attn_workspace(head_dim, q_heads / kv_heads, kv_heads, batch, max_q, rows);
+    return (int64_t)kv4_attn_workspace(head_dim, q_heads / kv_heads, kv_heads, batch, max_q, -1);
+}
+int64_t sl_kv4_attention_workspace_span(int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t batch, int32_t max_q, int64_t span) {
+    const int64_t most = sl_kv4_attention_workspace(q_heads, kv_heads, head_dim, batch, max_q, 0);
+    return most < 0 ? most : span < 0 ? SL_ERR_INVALID : (int64_t)kv4_attn_workspace(head_dim, q_heads / kv_heads, kv_heads, batch, max_q, std::min<int64_t>(span, 0x7fffffff));
 }
 int32_t sl_op_kv4_attention_device(const sl_kv4_cache* cache, const sl_kv4_attention* p, void* cuda_stream) try {
     Kv4Cache c{};
@@ -101,7 +106,7 @@ int32_t sl_op_kv4_attention_device(const sl_kv4_cache* cache, const sl_kv4_atten
     if (p->q_heads / c.KV > 128 || p->batch > 4096 || span > 0x7fffffffll - 65536 || (span / KV4_B + 1) * p->batch * c.KV > 0x7fffffffll - 65536) return SL_ERR_CAPACITY;
     if (!device_ok()) return SL_ERR_NO_DEVICE;
     if (p->rows == 0 || p->batch == 0) return SL_OK;
-    if (p->workspace_bytes < kv4_attn_workspace(c.D, p->q_heads / c.KV, c.KV, p->batch, p->max_q, p->rows)) return SL_ERR_CAPACITY;
+    if (p->workspace_bytes < kv4_attn_workspace(c.D, p->q_heads / c.KV, c.KV, p->batch, p->max_q, span)) return SL_ERR_CAPACITY;
     Kv4AttnArgs a{(const __half*)p->q, p->q_row, p->q_head, (const __half*)p->gate, p->gate_row, p->gate_head, (__half*)p->out, p->out_row, p->out_head,
                   p->rows, p->q_heads, p->q_heads / c.KV, p->q_start, p->kv_len, p->batch, p->max_q, p->table, p->table_stride, p->table_width,
                   p->causal ? 1 : 0, p->scale, p->workspace, (size_t)p->workspace_bytes};

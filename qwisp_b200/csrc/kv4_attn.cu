@@ -474,6 +474,12 @@ constexpr int KD_LEAST = 8;              // units a CTA takes at least
 // 14.4 | 16.4, 7 x (2000 + 4) 14.4 | 20.3, 16 x 1001 12.2 | 16.4, 64 x up to 1001 22.9 | 32.2.  16/2 of 256: 1 x 513 8.2 | 14.3, 1 x 2048 10.3 | 11.3, 1 x 4096
 // 14.4 | 12.3 [14.7 | 17.5], 1 x 8101 20.5 | 16.4.  8/1 of 64: 1 x 16001 16.4 | 13.6 [16.5 | 18.9].  Four CTAs for 16 x up to 8101 of 128: 36.9 | 35.4.
 constexpr long long KD_CL_SPAN = 1024 * 128;
+// CTAs of a cluster for that many (request, kv head) pairs with tables of `span` positions; 0: the work is dealt out evenly
+template <int D, int NT>
+static int decode_cluster(long long pairs, long long span) {
+    for (int cl = 8; cl; cl >>= 1) if (pairs * cl <= sm_count() * kd_ctas<D, NT> && span * D <= cl * KD_CL_SPAN) return cl;
+    return 0;
+}
 template <int D, int NT, int CL>
 static int decode_ready(int smem) {      // shared memory, once for each device
     static std::atomic<unsigned long long> configured{0};
@@ -500,13 +506,14 @@ static int launch_cluster(const Kv4Cache& c, const Kv4AttnArgs& a, int most, cud
 template <int D, int NT>
 static int launch_decode(const Kv4Cache& c, Kv4AttnArgs a, int most, cudaStream_t st) {
     a.scale *= 1.4426950408889634f;
+    switch (decode_cluster<D, NT>((long long)a.batch * c.KV, (long long)a.table_width * c.page_size)) {
+        case 8: return launch_cluster<D, NT, 8>(c, a, most, st);
+        case 4: return launch_cluster<D, NT, 4>(c, a, most, st);
+        case 2: return launch_cluster<D, NT, 2>(c, a, most, st);
+        case 1: return launch_cluster<D, NT, 1>(c, a, most, st);
+    }
     const int ctas = sm_count() * kd_ctas<D, NT>;
     int rc = 0;
-    const long long pairs = (long long)a.batch * c.KV, span = (long long)a.table_width * c.page_size * D;
-    if (pairs * 8 <= ctas && span <= 8 * KD_CL_SPAN) return launch_cluster<D, NT, 8>(c, a, most, st);
-    if (pairs * 4 <= ctas && span <= 4 * KD_CL_SPAN) return launch_cluster<D, NT, 4>(c, a, most, st);
-    if (pairs * 2 <= ctas && span <= 2 * KD_CL_SPAN) return launch_cluster<D, NT, 2>(c, a, most, st);
-    if (pairs <= ctas && span <= KD_CL_SPAN) return launch_cluster<D, NT, 1>(c, a, most, st);
     if ((rc = decode_ready<D, NT, 0>((int)kd_smem<D>(KD_MAX_BATCH)))) return rc;
     profile_launch("k_kv4_decode", st, [&] { return rc = launch_pdl(false, k_kv4_decode<D, NT, 0>, dim3((unsigned)ctas), KD_WARPS * 32, kd_smem<D>(a.batch), st, c, a, most, KD_LEAST); });
     if (rc) return rc;
@@ -514,19 +521,24 @@ static int launch_decode(const Kv4Cache& c, Kv4AttnArgs a, int most, cudaStream_
     return rc;
 }
 
+template <int D, int NT>
+static size_t decode_workspace(int KV, int batch, long long span) {
+    if (span >= 0 && decode_cluster<D, NT>((long long)batch * KV, span)) return 0;
+    return (size_t)(batch + 4) / 4 * 16 + (size_t)sm_count() * kd_ctas<D, NT> * 2 * 8 * NT * (D + 2) * 4;
+}
 template <int D>
-static size_t decode_workspace(int rows) { return rows > 8 ? (size_t)sm_count() * kd_ctas<D, 2> * 2 * 16 * (D + 2) * 4 : (size_t)sm_count() * kd_ctas<D, 1> * 2 * 8 * (D + 2) * 4; }
-size_t kv4_attn_workspace(int D, int G, int KV, int batch, int max_q, int rows) {
-    (void)KV; (void)rows;
-    const int tile = max_q > 16 / G ? 16 : max_q * G;
-    return (size_t)(batch + 4) / 4 * 16 + (D == 64 ? decode_workspace<64>(tile) : D == 128 ? decode_workspace<128>(tile) : decode_workspace<256>(tile));
+static size_t attn_workspace(int G, int KV, int batch, int max_q, long long span) {
+    if (G > 16 && span >= 0) return 0;                                        // (all requests are k_kv4_prompt's)
+    return max_q > 8 / G ? decode_workspace<D, 2>(KV, batch, span) : decode_workspace<D, 1>(KV, batch, span);
+}
+size_t kv4_attn_workspace(int D, int G, int KV, int batch, int max_q, long long span) {
+    return D == 64 ? attn_workspace<64>(G, KV, batch, max_q, span) : D == 128 ? attn_workspace<128>(G, KV, batch, max_q, span) : attn_workspace<256>(G, KV, batch, max_q, span);
 }
 template <int D>
 static int launch_attn(const Kv4Cache& c, const Kv4AttnArgs& a, cudaStream_t st) {
     int rc = 0;
     const bool many = a.max_q > 16 / a.G;
-    const int tile = many ? 16 : a.max_q * a.G;
-    if (a.G <= 16) rc = tile > 8 ? launch_decode<D, 2>(c, a, 16, st) : launch_decode<D, 1>(c, a, 8, st);
+    if (a.G <= 16) rc = a.max_q > 8 / a.G ? launch_decode<D, 2>(c, a, 16, st) : launch_decode<D, 1>(c, a, 8, st);
     if (rc || !many) return rc;
     return launch_kv4_prompt(c, a, a.G <= 16 ? 16 : 0, st, a.G <= 16);
 }

@@ -211,7 +211,7 @@ def kv_plan(lens, new_rows, table, free_pages, free_count, page_size, max_rows, 
           _flat(where, "free_count", free_count, i32, 1, index)]
     if out is None:                                                        # one allocation
         buf = torch.empty(3 * max_rows + 2 * B + 5, dtype=i32, device=lens.device)
-        slots, kv_len, q_start, pos, count, status = buf.split((2 * max_rows, B, B + 1, max_rows, 1, 3))
+        slots, kv_len, q_start, pos, count, status = torch.split_with_sizes(buf, (2 * max_rows, B, B + 1, max_rows, 1, 3))
         out, p, n = KvPlan(kv_len, q_start, slots.view(torch.int64), pos, count, status), buf.data_ptr(), 8 * max_rows
         to = (p + n, p + n + 4 * B, p, p + n + 8 * B + 4, p + n + 8 * B + 4 + 4 * max_rows, p + n + 8 * B + 8 + 4 * max_rows)
     else:
@@ -237,8 +237,10 @@ def kv4_append(cache, slots, q=None, k=None, v=None, *, q_norm=None, k_norm=None
         heads = q.shape[1] if q.dim() == 3 else 0
         qa = _heads(where, "q", q, (rows, heads, dim), index)
         if q_out is None:
-            q_out = torch.empty((rows, heads, dim), dtype=torch.float16, device=q.device)
-        oa = _heads(where, "q_out", q_out, (rows, heads, dim), index)
+            q_out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((rows, heads, dim))
+            oa = (q_out.data_ptr(), heads * dim, dim)
+        else:
+            oa = _heads(where, "q_out", q_out, (rows, heads, dim), index)
     if k is not None:
         ka, va = _heads(where, "k", k, (rows, kv, dim), index), _heads(where, "v", v, (rows, kv, dim), index)
         if slots is None:
@@ -278,12 +280,17 @@ def kv4_read(cache, slots, k=None, v=None):
     sa = _flat(where, "slots", slots, torch.int64, rows, index)
     shape = (rows, kv, dim)
     if k is None:
-        k = torch.empty(shape, dtype=torch.float16, device=cache.device)
+        k = cache.new_empty(shape, dtype=torch.float16)
+        kp, kr, kh = k.data_ptr(), kv * dim, dim
+    else:
+        kp, kr, kh = _heads(where, "k", k, shape, index)
     if v is None:
-        v = torch.empty_like(k) if k.is_contiguous() else torch.empty(shape, dtype=torch.float16, device=cache.device)
-    (kp, *kb), (vp, *vb) = _heads(where, "k", k, shape, index), _heads(where, "v", v, shape, index)
+        v = torch.empty_like(k) if k.is_contiguous() else cache.new_empty(shape, dtype=torch.float16)
+        vp, vr, vh = v.data_ptr(), kv * dim, dim
+    else:
+        vp, vr, vh = _heads(where, "v", v, shape, index)
     if rows:
-        _call(lib().sl_op_kv4_read_device, index, where, block, _READ.pack(sa, rows, kp, vp, *kb, *vb))
+        _call(lib().sl_op_kv4_read_device, index, where, block, _READ.pack(sa, rows, kp, vp, kr, kh, vr, vh))
     return k, v
 
 
@@ -296,6 +303,14 @@ def kv4_attention_workspace(q_heads, kv_heads, head_dim, batch, max_q, rows):
     return n
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_span(q_heads, kv_heads, head_dim, batch, max_q, span):
+    n = lib().sl_kv4_attention_workspace_span(q_heads, kv_heads, head_dim, batch, max_q, span)
+    if n < 0:
+        raise SeedlessError(n, "sl_kv4_attention_workspace_span")
+    return n
+
+
 def kv4_attention(cache, table, kv_len, q, q_start, max_q, *, causal=True, scale=None, gate=None, out=None, workspace=None):
     """softmax(scale q K^T) V [* sigmoid(gate)] over the cache: q [rows, heads, dim] fp16, request b's rows q_start[b] .. q_start[b + 1] - 1 (at most
     max_q) over its positions 0 .. kv_len[b] - 1 in the pages table[b]; causal: its rows are its last positions.  scale: dim ** -0.5 if
@@ -303,7 +318,7 @@ def kv4_attention(cache, table, kv_len, q, q_start, max_q, *, causal=True, scale
     if None; calls that may run at the same time need one each."""
     import torch
     where, i32 = "sl_op_kv4_attention_device", torch.int32
-    block, _, kv, dim, index = _cache(where, cache)
+    block, page, kv, dim, index = _cache(where, cache)
     if q.dim() != 3 or table.dim() != 2 or kv_len.dim() != 1 or max_q < 1:
         raise _no(where, "q is [rows, heads, dim], table int32 [B, pages], kv_len int32 [B], q_start int32 [B + 1]")
     shape, B, by = q.shape, kv_len.shape[0], table.stride()
@@ -313,18 +328,24 @@ def kv4_attention(cache, table, kv_len, q, q_start, max_q, *, causal=True, scale
         raise _no(where, f"table has to be int32 [{B}, pages] on the call's device")
     qa = _heads(where, "q", q, (rows, heads, dim), index)
     if out is None:
-        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=torch.float16, device=q.device)
-    oa = _heads(where, "out", out, shape, index)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
+        oa = (out.data_ptr(), heads * dim, dim)
+    else:
+        oa = _heads(where, "out", out, shape, index)
     ga = (0, 0, 0) if gate is None else _heads(where, "gate", gate, shape, index)
     la, ra = _flat(where, "kv_len", kv_len, i32, B, index), _flat(where, "q_start", q_start, i32, B + 1, index)
-    need = kv4_attention_workspace(heads, kv, dim, B, max_q, rows)
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    elif workspace.numel() < need:
-        raise _no(where, f"workspace has to have {need} bytes")
-    wa = _flat(where, "workspace", workspace, torch.uint8, None, index)
+        size = _workspace_span(heads, kv, dim, B, max_q, width * page)
+        if size:
+            workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+        wa = workspace.data_ptr() if size else qa[0]
+    else:
+        need, size = kv4_attention_workspace(heads, kv, dim, B, max_q, rows), workspace.numel()
+        if size < need:
+            raise _no(where, f"workspace has to have {need} bytes")
+        wa = _flat(where, "workspace", workspace, torch.uint8, None, index)
     if rows:
         _call(lib().sl_op_kv4_attention_device, index, where, block,
               _ATTENTION.pack(*qa, *ga, *oa, rows, heads, ra, la, B, max_q, table.data_ptr(), max(by[0], width), width, 1 if causal else 0,
-                              dim ** -0.5 if scale is None else scale, wa, workspace.numel()))
+                              dim ** -0.5 if scale is None else scale, wa, size))
     return out

@@ -90,6 +90,20 @@ def test_sizes_beyond_the_kernels_are_refused():
         assert _lib.lib().sl_kv4_attention_workspace(*args) == INVALID
 
 
+def test_workspace_of_a_span():
+    """Never more than for tables of any width, nothing where the kernels take the work whole, refusals as there."""
+    any_width, of = _lib.lib().sl_kv4_attention_workspace, _lib.lib().sl_kv4_attention_workspace_span
+    for heads, kv, dim, batch, max_q in ((8, 2, 128, 1, 1), (16, 2, 256, 64, 1), (64, 2, 64, 3, 5), (32, 8, 128, 4096, 4), (16, 1, 256, 2, 900)):
+        most = any_width(heads, kv, dim, batch, max_q, 7)
+        assert most > 0
+        assert all(of(heads, kv, dim, batch, max_q, span) in (0, most) for span in (0, 1, 512, 8192, 1 << 30, 1 << 40))
+        assert of(heads, kv, dim, batch, max_q, 1 << 40) == (0 if heads // kv > 16 else most)
+    assert of(8, 2, 128, 1, 1, 512) == 0
+    for args in ((7, 2, 128, 1, 1, 1), (8, 2, 96, 1, 1, 1), (8, 2, 128, -1, 1, 1), (8, 2, 128, 1, 0, 1), (8, 2, 128, 1, 1, -1)):
+        assert of(*args) == INVALID
+    assert of(2 * 129, 2, 128, 1, 1, 1) == CAPACITY
+
+
 def test_page_bytes():
     f = _lib.lib().sl_kv4_page_bytes
     assert f(2, 256, 64) == 2 * 64 * 256 * 9 // 8 and f(8, 128, 16) == 8 * 16 * 144
