@@ -106,8 +106,9 @@ __device__ __forceinline__ bool kp_wait(uint64_t* b, uint32_t parity, volatile i
     return __all_sync(0xffffffffu, kp_wait_one(b, parity, abort_word));
 }
 
-// CTAs (clusters) of a kv head at most: a request's last tile may be short
-template <int D, int NQ> static long long kp_items(const Kv4AttnArgs& a) { return (long long)a.rows / (KP_M / a.G * NQ) + a.batch; }
+// CTAs (clusters) of a kv head at most: one a request where its rows are one CTA's, else its last tile may be short
+template <int D, int NQ> static bool kp_one(const Kv4AttnArgs& a) { return a.max_q <= KP_M / a.G * NQ; }
+template <int D, int NQ> static long long kp_items(const Kv4AttnArgs& a) { return kp_one<D, NQ>(a) ? a.batch : (long long)a.rows / (KP_M / a.G * NQ) + a.batch; }
 constexpr int KP_SPLIT = 256;                                                // keys a CTA of a cluster has at least, of a table's span
 struct KpSeq { int q0, rows, n, keys; };
 
@@ -127,8 +128,9 @@ __global__ void __launch_bounds__(kp_threads<D, NQ>, kp_ctas<D, NQ>) k_kv4_promp
     __shared__ int s_abort, s_b, s_tile, s_sum[W];
     __shared__ __align__(4) uint8_t s_have[8][4];                             // whether a tile's blocks of 16 keys exist (softmax is up to four tiles behind)
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    const int tokens = KP_M / a.G, per_cta = tokens * NQ, head = blockIdx.y, item = (int)blockIdx.x / CL;
-    // ---- which request, and which of its tiles: the longest of a request first
+    const int tokens = KP_M / a.G, per_cta = tokens * NQ, head = (int)blockIdx.x / CL % c.KV, item = (int)blockIdx.x / CL / c.KV;
+    // ---- which request, and which of its tiles: the longest of a request first, of all kv heads (head by head, each head's shortest before the next
+    // one's longest: 4 prompts of up to 2900, 238 us for 218; one of 4096: 177 for 148)
     if (tid == 0) { s_b = -1; s_abort = 0; }
     __syncthreads();
     for (int b0 = 0, base = 0; b0 < a.batch; b0 += NT) {
@@ -584,7 +586,7 @@ static int launch_prompt_t(const Kv4Cache& c, Kv4AttnArgs a, int least, cudaStre
         if (dev < 64) configured.fetch_or(1ull << dev);
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(kp_items<D, NQ>(a) * CL), (unsigned)c.KV); cfg.blockDim = dim3(kp_threads<D, NQ>); cfg.dynamicSmemBytes = kp_smem<D, NQ>; cfg.stream = st;
+    cfg.gridDim = dim3((unsigned)(kp_items<D, NQ>(a) * c.KV * CL)); cfg.blockDim = dim3(kp_threads<D, NQ>); cfg.dynamicSmemBytes = kp_smem<D, NQ>; cfg.stream = st;
     cudaLaunchAttribute attr[2];
     int n = 0;
     if (pdl) { attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[n++].val.programmaticStreamSerializationAllowed = 1; }
@@ -594,21 +596,35 @@ static int launch_prompt_t(const Kv4Cache& c, Kv4AttnArgs a, int least, cudaStre
     profile_launch("k_kv4_prompt", st, [&] { return rc = (int)cudaLaunchKernelEx(&cfg, k_kv4_prompt<D, NQ, CL>, c, a, least, q_and, q_xor); });
     return rc;
 }
+// CTAs of a cluster.  So many that all run at once; of requests of one CTA each, half as many again, as they are seldom alike (12 x 9 rows, 32/8 heads of 128,
+// up to 2809 keys: 51 -> 39 us for two CTAs; 20 x 50, 8/8 of 64, up to 4350: 69 -> 57; but 24 x 9, 32/8 of 128: 64 -> 65.5, 40 x 77, 12 of 64, up to 1500: 63 -> 67).
+template <int D, int NQ>
+static int prompt_cluster(const Kv4Cache& c, const Kv4AttnArgs& a) {
+    const long long ctas = kp_items<D, NQ>(a) * c.KV, span = (long long)a.table_width * c.page_size, room = (long long)sm_count() * kp_ctas<D, NQ>;
+    if (ctas * 8 <= room * 7 / 8 && span >= KP_SPLIT * 8) return 8;           // (clusters of eight do not fill every part of the device)
+    if (ctas * 4 <= room && span >= KP_SPLIT * 4) return 4;
+    if (ctas * 2 <= room && span >= KP_SPLIT * 2) return 2;
+    return kp_one<D, NQ>(a) && ctas * 4 <= room * 3 && span >= KP_SPLIT * 8 ? 2 : 1;
+}
 template <int D, int NQ>
 static int launch_prompt_d(const Kv4Cache& c, const Kv4AttnArgs& a, int least, cudaStream_t st, bool pdl) {
-    const long long ctas = kp_items<D, NQ>(a) * c.KV, span = (long long)a.table_width * c.page_size;
-    const int sms = sm_count();
-    if (ctas * 8 <= sms * 7 / 8 && span >= KP_SPLIT * 8) return launch_prompt_t<D, NQ, 8>(c, a, least, st, pdl);
-    if (ctas * 4 <= sms && span >= KP_SPLIT * 4) return launch_prompt_t<D, NQ, 4>(c, a, least, st, pdl);
-    if (ctas * 2 <= sms && span >= KP_SPLIT * 2) return launch_prompt_t<D, NQ, 2>(c, a, least, st, pdl);
-    if constexpr (D == 64) {                                                  // (two CTAs a multiprocessor) 20 x 50 rows, 8/4 heads, up to 3050 keys: 41 -> 35 us
-        if (a.max_q <= KP_M / a.G && kp_items<64, 1>(a) * c.KV <= sms && span >= KP_SPLIT * 2) return launch_prompt_t<64, 1, 2>(c, a, least, st, pdl);
+    const int cl = prompt_cluster<D, NQ>(c, a);
+    // 64 dims, requests of one tile: two CTAs a multiprocessor where there are more of them than multiprocessors.  16 x 77 rows, 12 heads, up to 1500 keys:
+    // 37 -> 34 us, all of 1500: 46 -> 35, 40 x 77: 74 -> 63; 30 x 9, 32/8 heads, up to 809: 28.7 -> 24.2; 20 x 50, 8/4 heads, up to 3050, a
+    // cluster of two each: 41 -> 34
+    if constexpr (D == 64 && NQ == 2) {
+        if (cl <= 2 && kp_one<64, 1>(a) && (long long)a.batch * c.KV * cl > sm_count()) {
+            if (prompt_cluster<64, 1>(c, a) >= 2) return launch_prompt_t<64, 1, 2>(c, a, least, st, pdl);
+            return launch_prompt_t<64, 1, 1>(c, a, least, st, pdl);
+        }
+        if (cl == 1 && kp_one<64, 1>(a) && prompt_cluster<64, 1>(c, a) >= 2) return launch_prompt_t<64, 1, 2>(c, a, least, st, pdl);
     }
-    // requests of one tile and more CTAs than multiprocessors: two at once each.  16 x 77 rows, 12 heads, up to 1500 keys: 37 -> 34 us, all of 1500: 46 -> 36,
-    // 40 x 77: 76 -> 64; 20 x 50, 8/8, up to 350: 18.5 -> 16.6;
-    // but 30 x 9, 32/8 heads, up to 809: 28.7 -> 31.4
-    if constexpr (D == 64) { if (a.max_q <= KP_M / a.G && kp_items<64, 1>(a) * c.KV > sms) return launch_prompt_t<64, 1, 1>(c, a, least, st, pdl); }
-    return launch_prompt_t<D, NQ, 1>(c, a, least, st, pdl);
+    switch (cl) {
+        case 8: return launch_prompt_t<D, NQ, 8>(c, a, least, st, pdl);
+        case 4: return launch_prompt_t<D, NQ, 4>(c, a, least, st, pdl);
+        case 2: return launch_prompt_t<D, NQ, 2>(c, a, least, st, pdl);
+        default: return launch_prompt_t<D, NQ, 1>(c, a, least, st, pdl);
+    }
 }
 int launch_kv4_prompt(const Kv4Cache& c, const Kv4AttnArgs& a, int least, cudaStream_t st, bool pdl) {
     return c.D == 64 ? launch_prompt_d<64, 2>(c, a, least, st, pdl) : c.D == 128 ? launch_prompt_d<128, 2>(c, a, least, st, pdl) : launch_prompt_d<256, 1>(c, a, least, st, pdl);

@@ -425,6 +425,23 @@ def test_what_lies_behind_the_keys_does_not_count(D, news, keys):
     near(got, *attention_reference(cache, holes, keys, q, starts, True, D ** -0.5))
 
 
+@pytest.mark.parametrize("D,NH,KV,batch,new,gated", [(64, 12, 12, 16, 77, False), (64, 32, 8, 30, 9, True), (64, 8, 8, 20, 50, False), (128, 32, 8, 12, 9, True),
+                                                     (128, 16, 4, 40, 33, False), (256, 8, 8, 12, 60, True), (64, 8, 4, 30, 90, False)])
+@pytest.mark.parametrize("width", [40, 400])
+def test_many_requests_of_a_tile_of_rows(D, NH, KV, batch, new, gated, width):
+    """More tiles than multiprocessors, or nearly; requests of one row, of none and without keys among them; tables of 640 and of 6400 positions."""
+    keys = [(i * 389) % 601 for i in range(batch)]
+    news = [[new, 1, new - 3, 0][i % 4] if i else new for i in range(batch)]
+    cache, table, q, starts = attention_case(D, NH, KV, 16, news, keys)
+    table = torch.nn.functional.pad(table, (0, width - table.shape[1]), value=-1)
+    gate = torch.randn(q.shape, generator=gen(9), device="cuda").to(F16) if gated else None
+    for causal in (True, False):
+        got = ops().kv4_attention(cache, table, ints(keys), q, ints(starts), new, causal=causal, gate=gate)
+        near(got, *attention_reference(cache, table, keys, q, starts, causal, D ** -0.5, gate))
+        for _ in range(5):
+            assert torch.equal(ops().kv4_attention(cache, table, ints(keys), q, ints(starts), new, causal=causal, gate=gate), got)
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("n", [1, 3, 70])
 @pytest.mark.parametrize("width", [0, 1, 5000])
