@@ -474,11 +474,15 @@ constexpr int KD_LEAST = 8;              // units a CTA takes at least
 // 14.4 | 16.4, 7 x (2000 + 4) 14.4 | 20.3, 16 x 1001 12.2 | 16.4, 64 x up to 1001 22.9 | 32.2.  16/2 of 256: 1 x 513 8.2 | 14.3, 1 x 2048 10.3 | 11.3, 1 x 4096
 // 14.4 | 12.3 [14.7 | 17.5], 1 x 8101 20.5 | 16.4.  8/1 of 64: 1 x 16001 16.4 | 13.6 [16.5 | 18.9].  Four CTAs for 16 x up to 8101 of 128: 36.9 | 35.4.
 constexpr long long KD_CL_SPAN = 1024 * 128;
-// CTAs of a cluster for that many (request, kv head) pairs with tables of `span` positions; 0: the work is dealt out evenly
+// CTAs of a cluster for that many (request, kv head) pairs with tables of `span` positions; 0: the work is dealt out evenly.  One CTA a pair may have the
+// longer spans the more pairs there are, beside which a long one does not show.  By single CTAs | dealt out, us, heads of 128, 32/8: 128 x up to 301 18.7 | 30.8,
+// 128 x up to 2001 60 | 70, 300 x up to 3001 160 | 184, 40 x (up to 1500 + 4) 33 | 39; 300 x up to 1501, 16/2 of 256: 61 | 80; 64 x up to 2001 (span of
+// 2 x 1024): 39 | 41, of 256, 16/2 (span of 4 x): 35 | 29.
 template <int D, int NT>
 static int decode_cluster(long long pairs, long long span) {
-    for (int cl = 8; cl; cl >>= 1) if (pairs * cl <= sm_count() * kd_ctas<D, NT> && span * D <= cl * KD_CL_SPAN) return cl;
-    return 0;
+    const long long room = (long long)sm_count() * kd_ctas<D, NT>;
+    for (int cl = 8; cl > 1; cl >>= 1) if (pairs * cl <= room && span * D <= cl * KD_CL_SPAN) return cl;
+    return span * D <= KD_CL_SPAN * (1 + 2 * pairs / room) ? 1 : 0;
 }
 template <int D, int NT, int CL>
 static int decode_ready(int smem) {      // shared memory, once for each device

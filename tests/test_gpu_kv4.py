@@ -425,6 +425,18 @@ def test_what_lies_behind_the_keys_does_not_count(D, news, keys):
     near(got, *attention_reference(cache, holes, keys, q, starts, True, D ** -0.5))
 
 
+@pytest.mark.parametrize("D,NH,KV,batch,new", [(64, 8, 8, 150, 1), (128, 24, 8, 90, 2), (256, 8, 4, 200, 1), (128, 12, 4, 301, 4)])
+def test_more_requests_than_the_device_holds(D, NH, KV, batch, new):
+    """Few rows a request, each (request, kv head) whole in one place."""
+    keys = [(i * 389) % 601 if i % 7 else i % 3 for i in range(batch)]
+    news = [new if i % 5 else 0 for i in range(batch)]
+    cache, table, q, starts = attention_case(D, NH, KV, 32, news, keys)
+    got = ops().kv4_attention(cache, table, ints(keys), q, ints(starts), new)
+    near(got, *attention_reference(cache, table, keys, q, starts, True, D ** -0.5))
+    for _ in range(5):
+        assert torch.equal(ops().kv4_attention(cache, table, ints(keys), q, ints(starts), new), got)
+
+
 @pytest.mark.parametrize("D,NH,KV,batch,new,gated", [(64, 12, 12, 16, 77, False), (64, 32, 8, 30, 9, True), (64, 8, 8, 20, 50, False), (128, 32, 8, 12, 9, True),
                                                      (128, 16, 4, 40, 33, False), (256, 8, 8, 12, 60, True), (64, 8, 4, 30, 90, False)])
 @pytest.mark.parametrize("width", [40, 400])
