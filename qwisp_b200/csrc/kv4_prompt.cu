@@ -12,14 +12,14 @@
 //             outputs rescaled) only when a score exceeds it by 2^6; the weights are carried times 2^8, so that fp16 holds them from 2^-32 of the
 //             largest on.
 // NQ = 2 (D 64, 128): the expansion serves two tiles.  NQ = 1 (D 256): the outputs of one take half of tensor memory; (D 64) requests of one tile.
-// CL > 1: where there are fewer tiles than multiprocessors a cluster of CTAs takes each, a run of the keys a CTA, and adds up its sums through shared
+// SPLIT: where there are fewer tiles than multiprocessors a cluster of up to eight CTAs takes each, a run of the keys a CTA, and adds up its sums through shared
 // memory.  17 rows over 4017 positions, 32/8 heads of 128: 55 us with one CTA, 18.5 with eight.
 //
 // What bounds it: 1024 rows over 8192 positions, 16/2 heads of 256: 136 us, 0.95 PFLOP/s = 0.56 of the measured cuBLAS rate; four prompts of up to
-// 2900, 32/8 heads of 128: 238 us, 0.72 PFLOP/s = 0.43.  No unit is full (tensor pipe 39 %, MUFU 40 %, ALU 33 %, issue slots 43 % of the second): each tile of
+// 2900, 32/8 heads of 128: 220 us, 0.78 PFLOP/s = 0.46.  No unit is full (tensor pipe 39 %, MUFU 40 %, ALU 33 %, issue slots 43 % of the second): each tile of
 // 64 keys is a chain scores -> exponents -> weights -> outputs over barriers, which two tiles of rows overlap only in part, and every CTA begins
-// and ends alone (about 10 of 31 us there).  Leaving out the exponentials gave 12 %, the expansion 5 %, half of the MMAs nothing.  Tried, and no faster:
-// tiles of 128 keys with one score buffer (238 -> 254), two CTAs of one tile each (430: twice the expansion, 96 registers), more expanding
+// and ends alone (about 10 of 29 us there).  Leaving out the exponentials gave 12 %, the expansion 5 %, half of the MMAs nothing.  Tried, and no faster:
+// tiles of 128 keys with one score buffer (7 % slower), two CTAs of one tile each (1.8 times the time: twice the expansion, 96 registers), more expanding
 // warps with registers moved between the roles, a polynomial in place of some MUFU exponentials.
 #include "kv4.cuh"
 #include "kv4_mma.cuh"
@@ -109,11 +109,12 @@ __device__ __forceinline__ bool kp_wait(uint64_t* b, uint32_t parity, volatile i
 // CTAs (clusters) of a kv head at most: one a request where its rows are one CTA's, else its last tile may be short
 template <int D, int NQ> static bool kp_one(const Kv4AttnArgs& a) { return a.max_q <= KP_M / a.G * NQ; }
 template <int D, int NQ> static long long kp_items(const Kv4AttnArgs& a) { return kp_one<D, NQ>(a) ? a.batch : (long long)a.rows / (KP_M / a.G * NQ) + a.batch; }
+constexpr int KP_PARTS = 8;                                                   // CTAs of a cluster at most
 constexpr int KP_SPLIT = 256;                                                // keys a CTA of a cluster has at least, of a table's span
 struct KpSeq { int q0, rows, n, keys; };
 
-template <int D, int NQ, int CL>
-__global__ void __launch_bounds__(kp_threads<D, NQ>, kp_ctas<D, NQ>) k_kv4_prompt(Kv4Cache c, Kv4AttnArgs a, int least, uint32_t q_and, uint32_t q_xor) {
+template <int D, int NQ, bool SPLIT>
+__global__ void __launch_bounds__(kp_threads<D, NQ>, kp_ctas<D, NQ>) k_kv4_prompt(Kv4Cache c, Kv4AttnArgs a, int least, uint32_t q_and, uint32_t q_xor, int parts) {
     constexpr int TILE = kp_tile<D>, NT = kp_threads<D, NQ>, W = NT / 32, SW0 = 4;      // softmax warps start at SW0
     constexpr bool QT = kp_qt<D>;
     constexpr uint32_t S0 = NQ * D, Q0 = S0 + NQ * 2 * KP_N, COLUMNS = 512 / kp_ctas<D, NQ>;      // of tensor memory: outputs, scores (two of each tile), queries
@@ -122,13 +123,14 @@ __global__ void __launch_bounds__(kp_threads<D, NQ>, kp_ctas<D, NQ>) k_kv4_promp
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ __align__(8) uint64_t full[KP_ST], empty[KP_ST], s_full[2 * NQ], p_full[2 * NQ], q_full, o_done[2 * NQ];
     __shared__ uint32_t s_tmem;
-    __shared__ float2 s_ml[CL > 1 ? NQ * KP_M : 1];                           // CL > 1: the rows' (maximum, sum)
-    static_assert(CL == 1 || NQ * KP_M * D * 4 <= kp_smem<D, NQ> - 1024, "");
+    __shared__ float2 s_ml[SPLIT ? NQ * KP_M : 1];                            // SPLIT: the rows' (maximum, sum)
+    static_assert(!SPLIT || NQ * KP_M * D * 4 <= kp_smem<D, NQ> - 1024, "");
     __shared__ KpSeq s_seq;
     __shared__ int s_abort, s_b, s_tile, s_sum[W];
     __shared__ __align__(4) uint8_t s_have[8][4];                             // whether a tile's blocks of 16 keys exist (softmax is up to four tiles behind)
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    const int tokens = KP_M / a.G, per_cta = tokens * NQ, head = (int)blockIdx.x / CL % c.KV, item = (int)blockIdx.x / CL / c.KV;
+    const int tokens = KP_M / a.G, per_cta = tokens * NQ, CL = SPLIT ? parts : 1, rank = SPLIT ? (int)blockIdx.x % CL : 0;
+    const int head = (int)blockIdx.x / CL % c.KV, item = (int)blockIdx.x / CL / c.KV;
     // ---- which request, and which of its tiles: the longest of a request first, of all kv heads (head by head, each head's shortest before the next
     // one's longest: 4 prompts of up to 2900, 238 us for 218; one of 4096: 177 for 148)
     if (tid == 0) { s_b = -1; s_abort = 0; }
@@ -165,8 +167,8 @@ __global__ void __launch_bounds__(kp_threads<D, NQ>, kp_ctas<D, NQ>) k_kv4_promp
     const int last = min(t0 + per_cta, sq.rows) - 1;
     const int span = a.causal ? min(sq.keys, max(0, sq.keys - sq.n + last + 1)) : sq.keys;
     // keys KP_N j0 .. : all of them, or the cluster's CTAs share them out
-    const int all_tiles = (span + KP_N - 1) / KP_N, per = (all_tiles + CL - 1) / CL, j0 = CL == 1 ? 0 : min((int)(blockIdx.x % CL) * per, all_tiles);
-    const int tiles = CL == 1 ? all_tiles : min(per, all_tiles - j0);
+    const int all_tiles = (span + KP_N - 1) / KP_N, per = (all_tiles + CL - 1) / CL, j0 = min(rank * per, all_tiles);
+    const int tiles = min(per, all_tiles - j0);
     if (tid == 0) {
         for (int i = 0; i < KP_ST; ++i) { mbar_init(&full[i], kp_exp<D>); mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2 * NQ; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
@@ -464,7 +466,7 @@ __global__ void __launch_bounds__(kp_threads<D, NQ>, kp_ctas<D, NQ>) k_kv4_promp
                 __syncwarp();
                 if (lane == 0) kp_arrive(&p_full[slot]);
             }
-            if constexpr (CL > 1) {
+            if constexpr (SPLIT) {
                 // ---- the sums as they are, 16-byte pieces XORed with the row, over the ring and the queries (whose last readers were these MMAs)
                 for (int i = 0; i < nq; ++i) if (tiles > 0 && ok) ok = kp_wait(&o_done[2 * i + ((tiles - 1) & 1)], (uint32_t)((tiles - 1) >> 1) & 1u, &s_abort);
                 kp_after();
@@ -530,28 +532,42 @@ __global__ void __launch_bounds__(kp_threads<D, NQ>, kp_ctas<D, NQ>) k_kv4_promp
     }
     kp_before();
     __syncthreads();
-    if constexpr (CL > 1) {
+    if constexpr (SPLIT) {
         // ---- each CTA adds up every CL-th row, eight columns a thread
         __syncwarp();
         kv4_cluster_sync();
-        for (int x = tid; x < NQ * KP_M / CL * (D / 8); x += NT) {
-            const int r = x / (D / 8) * CL + (int)(blockIdx.x % CL), d = x % (D / 8) * 8, q = r / KP_M, row = r % KP_M, tok = t0 + q * tokens + row / a.G, h = head * a.G + row % a.G;
+        for (int x = tid; x < (NQ * KP_M + CL - 1) / CL * (D / 8); x += NT) {
+            const int r = x / (D / 8) * CL + rank, d = x % (D / 8) * 8, q = r / KP_M, row = r % KP_M, tok = t0 + q * tokens + row / a.G, h = head * a.G + row % a.G;
             if (q >= nq || row >= tokens * a.G || tok >= sq.rows) continue;
             const int64_t at_row = sq.q0 + tok;
             uint4 g = make_uint4(0, 0, 0, 0);
             if (a.gate) g = __ldcg(reinterpret_cast<const uint4*>(a.gate + at_row * a.g_row + h * a.g_head + d));
             const uint32_t p0 = smem0 + r * (D * 4) + (((d / 4) ^ (r & 7)) << 4), p1 = smem0 + r * (D * 4) + (((d / 4 + 1) ^ (r & 7)) << 4);
-            float2 ml[CL];
+            float2 ml[KP_PARTS];
             float top = -INFINITY, l = 0.f, v[8] = {};
+            // (ranks from CL on: the last one's place, for nothing, so that no load is behind a branch)
 #pragma unroll
-            for (int i = 0; i < CL; ++i) { ml[i] = kv4_peer2(kv4_peer(smem_u32(&s_ml[CL > 1 ? r : 0]), i)); top = fmaxf(top, ml[i].x); }
+            for (int i0 = 0; i0 < KP_PARTS; i0 += 4) {
+                if (i0 >= CL) break;
 #pragma unroll
-            for (int i = 0; i < CL; ++i) {
-                const float4 y0 = kv4_peer4(kv4_peer(p0, i)), y1 = kv4_peer4(kv4_peer(p1, i));
-                const float f = ml[i].x == -INFINITY ? 0.f : kv4_exp2(ml[i].x - top);
-                l = fmaf(ml[i].y, f, l);
-                v[0] = fmaf(y0.x, f, v[0]); v[1] = fmaf(y0.y, f, v[1]); v[2] = fmaf(y0.z, f, v[2]); v[3] = fmaf(y0.w, f, v[3]);
-                v[4] = fmaf(y1.x, f, v[4]); v[5] = fmaf(y1.y, f, v[5]); v[6] = fmaf(y1.z, f, v[6]); v[7] = fmaf(y1.w, f, v[7]);
+                for (int i = i0; i < i0 + 4; ++i) ml[i] = kv4_peer2(kv4_peer(smem_u32(&s_ml[SPLIT ? r : 0]), min(i, CL - 1)));
+#pragma unroll
+                for (int i = i0; i < i0 + 4; ++i) top = fmaxf(top, ml[i].x);
+            }
+#pragma unroll
+            for (int i0 = 0; i0 < KP_PARTS; i0 += 4) {
+                if (i0 >= CL) break;
+                float4 y0[4], y1[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { y0[i] = kv4_peer4(kv4_peer(p0, min(i0 + i, CL - 1))); y1[i] = kv4_peer4(kv4_peer(p1, min(i0 + i, CL - 1))); }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 x = ml[i0 + i];
+                    const float f = i0 + i >= CL || x.x == -INFINITY ? 0.f : kv4_exp2(x.x - top);
+                    l = fmaf(x.y, f, l);
+                    v[0] = fmaf(y0[i].x, f, v[0]); v[1] = fmaf(y0[i].y, f, v[1]); v[2] = fmaf(y0[i].z, f, v[2]); v[3] = fmaf(y0[i].w, f, v[3]);
+                    v[4] = fmaf(y1[i].x, f, v[4]); v[5] = fmaf(y1[i].y, f, v[5]); v[6] = fmaf(y1[i].z, f, v[6]); v[7] = fmaf(y1[i].w, f, v[7]);
+                }
             }
             const float inv = l == 0.f ? 0.f : 1.0f / l;
             float y[8];
@@ -572,38 +588,64 @@ __global__ void __launch_bounds__(kp_threads<D, NQ>, kp_ctas<D, NQ>) k_kv4_promp
     pdl_wait();
 }
 
-template <int D, int NQ, int CL>
-static int launch_prompt_t(const Kv4Cache& c, Kv4AttnArgs a, int least, cudaStream_t st, bool pdl) {
-    // a scale below zero, or zero, goes into the queries: the maximum of the scores is that of the scaled ones then
-    const uint32_t q_and = a.scale == 0.f ? 0u : 0xffffffffu, q_xor = a.scale < 0.f ? 0x80008000u : 0u;
-    a.scale = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
+// shared memory, once for each device
+template <int D, int NQ, bool SPLIT>
+static int prompt_ready() {
     static std::atomic<unsigned long long> configured{0};                     // devices
     int dev = 0;
     cudaGetDevice(&dev);
-    if (dev >= 64 || !(configured.load(std::memory_order_relaxed) >> dev & 1)) {
-        cudaError_t err = cudaFuncSetAttribute(k_kv4_prompt<D, NQ, CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kp_smem<D, NQ>);
-        if (err != cudaSuccess) return (int)err;
-        if (dev < 64) configured.fetch_or(1ull << dev);
-    }
+    if (dev < 64 && (configured.load(std::memory_order_relaxed) >> dev & 1)) return 0;
+    const cudaError_t err = cudaFuncSetAttribute(k_kv4_prompt<D, NQ, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kp_smem<D, NQ>);
+    if (err == cudaSuccess && dev < 64) configured.fetch_or(1ull << dev);
+    return (int)err;
+}
+// a launch of clusters of cl CTAs; attr: room for two attributes
+template <int D, int NQ>
+static cudaLaunchConfig_t prompt_config(long long ctas, int cl, bool pdl, cudaStream_t st, cudaLaunchAttribute* attr) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(kp_items<D, NQ>(a) * c.KV * CL)); cfg.blockDim = dim3(kp_threads<D, NQ>); cfg.dynamicSmemBytes = kp_smem<D, NQ>; cfg.stream = st;
+    cfg.gridDim = dim3((unsigned)ctas); cfg.blockDim = dim3(kp_threads<D, NQ>); cfg.dynamicSmemBytes = kp_smem<D, NQ>; cfg.stream = st; cfg.attrs = attr;
+    if (pdl) { attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1; }
+    if (cl > 1) { attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension; attr[cfg.numAttrs].val.clusterDim.x = (unsigned)cl; attr[cfg.numAttrs].val.clusterDim.y = 1; attr[cfg.numAttrs++].val.clusterDim.z = 1; }
+    return cfg;
+}
+template <int D, int NQ>
+static int launch_prompt_t(const Kv4Cache& c, Kv4AttnArgs a, int least, cudaStream_t st, bool pdl, int cl) {
+    // a scale below zero, or zero, goes into the queries: the maximum of the scores is that of the scaled ones then
+    const uint32_t q_and = a.scale == 0.f ? 0u : 0xffffffffu, q_xor = a.scale < 0.f ? 0x80008000u : 0u;
+    a.scale = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
+    int rc = cl > 1 ? prompt_ready<D, NQ, true>() : prompt_ready<D, NQ, false>();
+    if (rc) return rc;
     cudaLaunchAttribute attr[2];
-    int n = 0;
-    if (pdl) { attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[n++].val.programmaticStreamSerializationAllowed = 1; }
-    if (CL > 1) { attr[n].id = cudaLaunchAttributeClusterDimension; attr[n].val.clusterDim.x = CL; attr[n].val.clusterDim.y = 1; attr[n++].val.clusterDim.z = 1; }
-    cfg.attrs = attr; cfg.numAttrs = n;
-    int rc = 0;
-    profile_launch("k_kv4_prompt", st, [&] { return rc = (int)cudaLaunchKernelEx(&cfg, k_kv4_prompt<D, NQ, CL>, c, a, least, q_and, q_xor); });
+    const cudaLaunchConfig_t cfg = prompt_config<D, NQ>(kp_items<D, NQ>(a) * c.KV * cl, cl, pdl, st, attr);
+    profile_launch("k_kv4_prompt", st, [&] {
+        return rc = (int)(cl > 1 ? cudaLaunchKernelEx(&cfg, k_kv4_prompt<D, NQ, true>, c, a, least, q_and, q_xor, cl) : cudaLaunchKernelEx(&cfg, k_kv4_prompt<D, NQ, false>, c, a, least, q_and, q_xor, 1));
+    });
     return rc;
+}
+// clusters of cl CTAs that the device holds at once (they do not fill every part of it)
+template <int D, int NQ>
+static int prompt_room(int cl) {
+    static std::atomic<int> known[64][KP_PARTS + 1] = {};                     // (+ 1)
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    if ((n = known[dev][cl].load(std::memory_order_relaxed))) return n - 1;
+    cudaLaunchAttribute attr[2];
+    const cudaLaunchConfig_t cfg = prompt_config<D, NQ>(cl * 1024, cl, false, nullptr, attr);
+    if (prompt_ready<D, NQ, true>() || cudaOccupancyMaxActiveClusters(&n, k_kv4_prompt<D, NQ, true>, &cfg) != cudaSuccess || n < 0) { n = 0; cudaGetLastError(); }
+    known[dev][cl].store(n + 1, std::memory_order_relaxed);
+    return n;
 }
 // CTAs of a cluster.  So many that all run at once; of requests of one CTA each, half as many again, as they are seldom alike (12 x 9 rows, 32/8 heads of 128,
 // up to 2809 keys: 51 -> 39 us for two CTAs; 20 x 50, 8/8 of 64, up to 4350: 69 -> 57; but 24 x 9, 32/8 of 128: 64 -> 65.5, 40 x 77, 12 of 64, up to 1500: 63 -> 67).
 template <int D, int NQ>
 static int prompt_cluster(const Kv4Cache& c, const Kv4AttnArgs& a) {
     const long long ctas = kp_items<D, NQ>(a) * c.KV, span = (long long)a.table_width * c.page_size, room = (long long)sm_count() * kp_ctas<D, NQ>;
-    if (ctas * 8 <= room * 7 / 8 && span >= KP_SPLIT * 8) return 8;           // (clusters of eight do not fill every part of the device)
-    if (ctas * 4 <= room && span >= KP_SPLIT * 4) return 4;
-    if (ctas * 2 <= room && span >= KP_SPLIT * 2) return 2;
+    auto keys = [&](int cl) { return span >= KP_SPLIT * cl; };
+    if (keys(8) && ctas * 8 <= room * 7 / 8 && ctas <= prompt_room<D, NQ>(8)) return 8;
+    if (keys(6) && ctas * 6 <= room && ctas <= prompt_room<D, NQ>(6) * 7 / 8) return 6;      // (three in a part of the device: where the kernels before still leave room)
+    if (keys(4) && ctas * 4 <= room) return 4;
+    if (keys(3) && ctas * 3 <= room && ctas <= prompt_room<D, NQ>(3)) return 3;      // 300 rows over 30300, 32/8 heads of 128: 260 -> 183 us against two, over 9300, 16/2 of 256: 83 -> 67
+    if (keys(2) && ctas * 2 <= room) return 2;
     return kp_one<D, NQ>(a) && ctas * 4 <= room * 3 && span >= KP_SPLIT * 8 ? 2 : 1;
 }
 template <int D, int NQ>
@@ -612,19 +654,13 @@ static int launch_prompt_d(const Kv4Cache& c, const Kv4AttnArgs& a, int least, c
     // 64 dims, requests of one tile: two CTAs a multiprocessor where there are more of them than multiprocessors.  16 x 77 rows, 12 heads, up to 1500 keys:
     // 37 -> 34 us, all of 1500: 46 -> 35, 40 x 77: 74 -> 63; 30 x 9, 32/8 heads, up to 809: 28.7 -> 24.2; 20 x 50, 8/4 heads, up to 3050, a
     // cluster of two each: 41 -> 34
-    if constexpr (D == 64 && NQ == 2) {
-        if (cl <= 2 && kp_one<64, 1>(a) && (long long)a.batch * c.KV * cl > sm_count()) {
-            if (prompt_cluster<64, 1>(c, a) >= 2) return launch_prompt_t<64, 1, 2>(c, a, least, st, pdl);
-            return launch_prompt_t<64, 1, 1>(c, a, least, st, pdl);
+    if constexpr (D == 64) {
+        if (cl <= 2 && kp_one<64, 1>(a)) {
+            const int pairs = prompt_cluster<64, 1>(c, a);
+            if (cl < pairs || (long long)a.batch * c.KV * cl > sm_count()) return launch_prompt_t<64, 1>(c, a, least, st, pdl, pairs);
         }
-        if (cl == 1 && kp_one<64, 1>(a) && prompt_cluster<64, 1>(c, a) >= 2) return launch_prompt_t<64, 1, 2>(c, a, least, st, pdl);
     }
-    switch (cl) {
-        case 8: return launch_prompt_t<D, NQ, 8>(c, a, least, st, pdl);
-        case 4: return launch_prompt_t<D, NQ, 4>(c, a, least, st, pdl);
-        case 2: return launch_prompt_t<D, NQ, 2>(c, a, least, st, pdl);
-        default: return launch_prompt_t<D, NQ, 1>(c, a, least, st, pdl);
-    }
+    return launch_prompt_t<D, NQ>(c, a, least, st, pdl, cl);
 }
 int launch_kv4_prompt(const Kv4Cache& c, const Kv4AttnArgs& a, int least, cudaStream_t st, bool pdl) {
     return c.D == 64 ? launch_prompt_d<64, 2>(c, a, least, st, pdl) : c.D == 128 ? launch_prompt_d<128, 2>(c, a, least, st, pdl) : launch_prompt_d<256, 1>(c, a, least, st, pdl);

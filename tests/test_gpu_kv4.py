@@ -425,6 +425,19 @@ def test_what_lies_behind_the_keys_does_not_count(D, news, keys):
     near(got, *attention_reference(cache, holes, keys, q, starts, True, D ** -0.5))
 
 
+@pytest.mark.parametrize("D,NH,KV,new,past", [(128, 32, 8, 300, 1800), (128, 16, 4, 90, 2500), (64, 16, 8, 200, 1900), (256, 16, 2, 140, 1700), (256, 16, 2, 300, 1000), (64, 8, 8, 600, 700),
+                                              (128, 8, 8, 65, 3000), (256, 8, 8, 33, 2000)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_keys_shared_out(D, NH, KV, new, past, causal):
+    """Few tiles of rows over many keys: shares of every size, some of them without keys for a tile."""
+    news, keys = [new, 20], [new + past, 21]
+    cache, table, q, starts = attention_case(D, NH, KV, 16, news, keys)
+    got = ops().kv4_attention(cache, table, ints(keys), q, ints(starts), new, causal=causal)
+    near(got, *attention_reference(cache, table, keys, q, starts, causal, D ** -0.5))
+    for _ in range(10):
+        assert torch.equal(ops().kv4_attention(cache, table, ints(keys), q, ints(starts), new, causal=causal), got)
+
+
 @pytest.mark.parametrize("D,NH,KV,batch,new", [(64, 8, 8, 150, 1), (128, 24, 8, 90, 2), (256, 8, 4, 200, 1), (128, 12, 4, 301, 4)])
 def test_more_requests_than_the_device_holds(D, NH, KV, batch, new):
     """Few rows a request, each (request, kv head) whole in one place."""
