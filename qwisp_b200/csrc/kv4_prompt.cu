@@ -627,7 +627,7 @@ template <int D, int NQ>
 static int prompt_room(int cl) {
     static std::atomic<int> known[64][KP_PARTS + 1] = {};                     // (+ 1)
     int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return 0; }
     if ((n = known[dev][cl].load(std::memory_order_relaxed))) return n - 1;
     cudaLaunchAttribute attr[2];
     const cudaLaunchConfig_t cfg = prompt_config<D, NQ>(cl * 1024, cl, false, nullptr, attr);
