@@ -378,6 +378,7 @@ int32_t sl_op_kv4_read_device(const sl_kv4_cache* cache, const sl_kv4_read* rows
  * sees the first kv_len - n + i + 1 positions.  A row that sees none is zero; table entries that are no page of the cache hold no keys; rows of
  * no request, and rows of a request behind its first max_q, are left as they were.  The requests' rows do not overlap.  Infinities and NaN in places
  * that a row does not see do not count, unless another row of its request sees them: then this row may be NaN too.
+ * Waits inside the kernels are bounded; the rows of one that ran out are NaN.
  * workspace: 16-byte aligned, sl_kv4_attention_workspace() bytes (the same arguments), any contents; calls that may run at the same
  * time need one each. */
 typedef struct sl_kv4_attention {
