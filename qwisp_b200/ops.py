@@ -210,7 +210,7 @@ def kv_plan(lens, new_rows, table, free_pages, free_count, page_size, max_rows, 
     at = [_flat(where, "lens", lens, i32, B, index), _flat(where, "new_rows", new_rows, i32, B, index), _flat(where, "free_pages", free_pages, i32, None, index),
           _flat(where, "free_count", free_count, i32, 1, index)]
     if out is None:                                                        # one allocation
-        buf = torch.empty(3 * max_rows + 2 * B + 5, dtype=i32, device=lens.device)
+        buf = lens.new_empty(3 * max_rows + 2 * B + 5)
         slots, kv_len, q_start, pos, count, status = torch.split_with_sizes(buf, (2 * max_rows, B, B + 1, max_rows, 1, 3))
         out, p, n = KvPlan(kv_len, q_start, slots.view(torch.int64), pos, count, status), buf.data_ptr(), 8 * max_rows
         to = (p + n, p + n + 4 * B, p, p + n + 8 * B + 4, p + n + 8 * B + 4 + 4 * max_rows, p + n + 8 * B + 8 + 4 * max_rows)
