@@ -388,7 +388,7 @@ typedef struct sl_kv4_attention {
     int32_t rows, q_heads;                                   /* rows of q, gate and out */
     const int32_t *q_start, *kv_len; int32_t batch;
     int32_t max_q;                                           /* most rows of a request */
-    const int32_t* table; int64_t table_stride; int32_t table_width;
+    const int32_t* table; int64_t table_stride; int32_t table_width;   /* rows table_stride apart; 0: all requests have the first */
     int32_t causal; float scale;
     void* workspace; uint64_t workspace_bytes;
 } sl_kv4_attention;

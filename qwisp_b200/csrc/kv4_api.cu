@@ -99,7 +99,7 @@ int32_t sl_op_kv4_attention_device(const sl_kv4_cache* cache, const sl_kv4_atten
     if (!p || !cache_of(cache, c) || p->rows < 0 || p->batch < 0 || p->max_q < 1 || p->table_width < 0) return SL_ERR_INVALID;
     if (p->q_heads <= 0 || p->q_heads % c.KV || !std::isfinite(p->scale)) return SL_ERR_INVALID;
     if (!p->q || !p->out || !p->q_start || !p->workspace || ((uintptr_t)p->workspace & 15)) return SL_ERR_INVALID;
-    if (p->batch && (!p->kv_len || (!p->table && p->table_width) || p->table_stride < p->table_width)) return SL_ERR_INVALID;
+    if (p->batch && (!p->kv_len || (!p->table && p->table_width) || (p->table_stride && p->table_stride < p->table_width))) return SL_ERR_INVALID;
     if (!aligned(p->q, p->q_row, p->q_head) || !aligned(p->out, p->out_row, p->out_head) || (p->gate && !aligned(p->gate, p->gate_row, p->gate_head))) return SL_ERR_INVALID;
     // (positions and key blocks are counted in 31 bits)
     const int64_t span = (int64_t)p->table_width * c.page_size;

@@ -207,6 +207,8 @@ def kv_plan(lens, new_rows, table, free_pages, free_count, page_size, max_rows, 
     B, (rows, width), by = lens.shape[0], table.shape, table.stride()
     if rows != B or table.dtype is not i32 or (by[1] != 1 and width > 1) or table.get_device() != index:
         raise _no(where, f"table has to be int32 [{B}, pages] on the call's device")
+    if B > 1 and by[0] < width:                                            # (an expanded one: its requests would write each other's pages)
+        raise _no(where, "the table's rows must not overlap")
     at = [_flat(where, "lens", lens, i32, B, index), _flat(where, "new_rows", new_rows, i32, B, index), _flat(where, "free_pages", free_pages, i32, None, index),
           _flat(where, "free_count", free_count, i32, 1, index)]
     if out is None:                                                        # one allocation
@@ -216,7 +218,7 @@ def kv_plan(lens, new_rows, table, free_pages, free_count, page_size, max_rows, 
         to = (p + n, p + n + 4 * B, p, p + n + 8 * B + 4, p + n + 8 * B + 4 + 4 * max_rows, p + n + 8 * B + 8 + 4 * max_rows)
     else:
         to = [_flat(where, name + " out", t, torch.int64 if name == "slots" else i32, n, index) for name, t, n in zip(KvPlan._fields, out, (B, B + 1, max_rows, max_rows, 1, 3))]
-    _call(lib().sl_op_kv_plan_device, index, where, _PLAN.pack(at[0], at[1], B, page_size, table.data_ptr(), max(by[0], width), width, at[2], free_pages.shape[0], at[3], *to[:4], max_rows, *to[4:]))
+    _call(lib().sl_op_kv_plan_device, index, where, _PLAN.pack(at[0], at[1], B, page_size, table.data_ptr(), by[0] if B > 1 else width, width, at[2], free_pages.shape[0], at[3], *to[:4], max_rows, *to[4:]))
     return out
 
 
@@ -313,8 +315,8 @@ def _workspace_span(q_heads, kv_heads, head_dim, batch, max_q, span):
 
 def kv4_attention(cache, table, kv_len, q, q_start, max_q, *, causal=True, scale=None, gate=None, out=None, workspace=None):
     """softmax(scale q K^T) V [* sigmoid(gate)] over the cache: q [rows, heads, dim] fp16, request b's rows q_start[b] .. q_start[b + 1] - 1 (at most
-    max_q) over its positions 0 .. kv_len[b] - 1 in the pages table[b]; causal: its rows are its last positions.  scale: dim ** -0.5 if
-    None.  A row that sees no position is zero.  workspace: a uint8 tensor of kv4_attention_workspace() bytes, allocated for the call
+    max_q) over its positions 0 .. kv_len[b] - 1 in the pages table[b] (one row expanded to all requests will do where they share them);
+    causal: its rows are its last positions.  scale: dim ** -0.5 if None.  A row that sees no position is zero.  workspace: a uint8 tensor of kv4_attention_workspace() bytes, allocated for the call
     if None; calls that may run at the same time need one each."""
     import torch
     where, i32 = "sl_op_kv4_attention_device", torch.int32
@@ -346,6 +348,6 @@ def kv4_attention(cache, table, kv_len, q, q_start, max_q, *, causal=True, scale
         wa = _flat(where, "workspace", workspace, torch.uint8, None, index)
     if rows:
         _call(lib().sl_op_kv4_attention_device, index, where, block,
-              _ATTENTION.pack(*qa, *ga, *oa, rows, heads, ra, la, B, max_q, table.data_ptr(), max(by[0], width), width, 1 if causal else 0,
+              _ATTENTION.pack(*qa, *ga, *oa, rows, heads, ra, la, B, max_q, table.data_ptr(), by[0] if B > 1 else width, width, 1 if causal else 0,
                               dim ** -0.5 if scale is None else scale, wa, size))
     return out
