@@ -34,8 +34,9 @@ __device__ __forceinline__ float2 kv4_unpair(kv4_f2 v) { float2 r; asm("mov.b64 
 __device__ __forceinline__ kv4_f2 kv4_fma2(kv4_f2 a, kv4_f2 b, kv4_f2 c) { kv4_f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
 __device__ __forceinline__ kv4_f2 kv4_add2(kv4_f2 a, kv4_f2 b) { kv4_f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ float kv4_max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
-// 1 / (1 + e^-x), some 2^-21 of itself off: an infinite power makes it 0
-__device__ __forceinline__ float kv4_sigmoid(float x) { return __fdividef(1.0f, 1.0f + fminf(kv4_exp2(x * -1.4426950408889634f), 0x1p126f)); }
+__device__ __forceinline__ float kv4_min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }      // (fminf drops a NaN)
+// 1 / (1 + e^-x), some 2^-21 of itself off: an infinite power makes it 0, a NaN stays one
+__device__ __forceinline__ float kv4_sigmoid(float x) { return __fdividef(1.0f, 1.0f + kv4_min_nan(kv4_exp2(x * -1.4426950408889634f), 0x1p126f)); }
 __device__ __forceinline__ uint32_t kv4_pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ __half2 kv4_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
 __device__ __forceinline__ uint32_t kv4_u(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }

@@ -1,0 +1,52 @@
+"""Values at the edges of the attention over the 4-bit KV cache: gates that are no numbers.  The
+kernels' tolerances are those of test_gpu_kv4.py, whose references these tests use."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_kv4 import F16, attention_case, attention_reference, gen, ints, near, ops
+
+pytestmark = pytest.mark.gpu
+
+ENDS = [  # D, heads, kv heads, rows of the requests, their keys, columns that the table has more: each of the kernels' ends
+    (128, 8, 2, [1, 1], [37, 5], 0),               # decode, clusters
+    (256, 16, 2, [1, 1], [40, 2100], 3000),        # decode, dealt out: whole in a CTA, and joined
+    (64, 8, 2, [3, 2], [50, 700], 5000),           # the same, two tiles of rows
+    (128, 16, 2, [40, 3], [90, 3], 0),             # prompt, a tile of rows and two
+    (256, 8, 2, [40], [30], 0),                    # prompt, rows that see nothing
+    (64, 4, 4, [20] * 9, [100] * 9, 0),            # prompt, tiles of 64 dims by themselves
+    (128, 8, 2, [70], [2100], 0),                  # prompt, keys shared out by a cluster
+    (64, 4, 4, [33], [1500], 0),
+]
+each_end = pytest.mark.parametrize("case", ENDS, ids=lambda c: "-".join(str(v) if not isinstance(v, list) else f"{len(v)}x{max(v)}" for v in c))
+
+
+def inputs(case):
+    D, NH, KV, news, keys, more = case
+    cache, table, q, starts = attention_case(D, NH, KV, 32, news, keys)
+    return cache, torch.nn.functional.pad(table, (0, more), value=-1), q, starts
+
+
+def alike(got, want, size, live):
+    """NaN where it has to be and nowhere else, the rest near."""
+    assert torch.equal(got.isnan()[live], want.isnan()[live])
+    near(got.nan_to_num(0.0), want.nan_to_num(0.0), size.nan_to_num(0.0), live)
+
+
+@each_end
+@pytest.mark.parametrize("causal", [True, False])
+def test_gates_that_are_no_numbers(case, causal):
+    """A gate of NaN gives NaN, one of minus infinity zero, one of infinity the attention itself, each in its own place."""
+    D, news, keys = case[0], case[3], case[4]
+    cache, table, q, starts = inputs(case)
+    gate = torch.randn(q.shape, generator=gen(3), device="cuda").mul_(2).to(F16)
+    odd = torch.rand(q.shape, generator=gen(4), device="cuda")
+    for lo, v in enumerate((math.nan, -math.nan, math.inf, -math.inf, 65504.0, -65504.0)):
+        gate[(odd >= lo * 0.02) & (odd < lo * 0.02 + 0.02)] = v
+    gate[0, 0, :9] = math.nan
+    got = ops().kv4_attention(cache, table, ints(keys), q, ints(starts), max(news), causal=causal, gate=gate)
+    want = attention_reference(cache, table, keys, q, starts, causal, D ** -0.5, gate)
+    assert want[0].isnan().any()
+    alike(got, *want)
