@@ -356,8 +356,10 @@ __global__ void __launch_bounds__(kp_threads<D, NQ>, kp_ctas<D, NQ>) k_kv4_promp
                         const int d = d0 + 64 * k;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            const uint4 y = v[k][i], x = make_uint4((__byte_perm(y.x, y.z, 0x5410) & q_and) ^ q_xor, (__byte_perm(y.x, y.z, 0x7632) & q_and) ^ q_xor,
-                                                                    (__byte_perm(y.y, y.w, 0x5410) & q_and) ^ q_xor, (__byte_perm(y.y, y.w, 0x7632) & q_and) ^ q_xor);
+                            // (x * 0 + x: an infinity, whose scores are infinities or NaN for every key, makes the row NaN whatever their signs, also where
+                            // the scale is zero; anything finite is itself)
+                            auto put = [&](uint32_t h) { return kv4_u(__hfma2(kv4_h2(h), kv4_h2(0u), kv4_h2(h & q_and))) ^ q_xor; };
+                            const uint4 y = v[k][i], x = make_uint4(put(__byte_perm(y.x, y.z, 0x5410)), put(__byte_perm(y.x, y.z, 0x7632)), put(__byte_perm(y.y, y.w, 0x5410)), put(__byte_perm(y.y, y.w, 0x7632)));
                             kp_sts(QT ? io + turn(i) : qs0 + q * (KP_M * D * 2) + (d >> 6) * (KP_M * 128) + (warp & 3) * 4096 + turn(i), x);
                         }
                         if (QT) {

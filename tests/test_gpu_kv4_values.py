@@ -1,5 +1,5 @@
-"""Values at the edges of the attention over the 4-bit KV cache: gates that are no numbers.  The
-kernels' tolerances are those of test_gpu_kv4.py, whose references these tests use."""
+"""Values at the edges of the attention over the 4-bit KV cache: gates and queries that are no numbers.
+The kernels' tolerances are those of test_gpu_kv4.py, whose references these tests use."""
 import math
 
 import pytest
@@ -50,3 +50,27 @@ def test_gates_that_are_no_numbers(case, causal):
     want = attention_reference(cache, table, keys, q, starts, causal, D ** -0.5, gate)
     assert want[0].isnan().any()
     alike(got, *want)
+
+
+@each_end
+@pytest.mark.parametrize("scale", [None, -0.05, 0.0])
+def test_queries_that_are_no_numbers(case, scale):
+    """An infinity or a NaN among a row's queries makes its scores infinities and NaN, and so, whatever their signs, its outputs NaN: with
+    one key as with many.  Heads and rows beside it keep their values; a row that sees nothing stays zero."""
+    D, NH, _, news, keys, _ = case
+    cache, table, q, starts = inputs(case)
+    g, rows = gen(5), q.shape[0]
+    clean = q.clone()
+    bad = torch.rand((rows, NH), generator=g, device="cuda") < 0.3
+    bad[0, 0] = True
+    at = torch.randint(0, D, (rows, NH, 1), generator=g, device="cuda")
+    what = torch.tensor([math.nan, math.inf, -math.inf], dtype=F16, device="cuda")[torch.randint(0, 3, (rows, NH, 1), generator=g, device="cuda")]
+    q.scatter_(2, at, torch.where(bad[..., None], what, q.gather(2, at)))
+    for causal in (True, False):
+        want, size, live = attention_reference(cache, table, keys, clean, starts, causal, D ** -0.5 if scale is None else scale)
+        sees = torch.zeros(rows, dtype=torch.bool, device="cuda")
+        for b, n in enumerate(keys):
+            lo, hi = starts[b], starts[b + 1]
+            sees[lo:hi] = (n - (hi - lo) + torch.arange(hi - lo, device="cuda") + 1 if causal else torch.full((hi - lo,), n, device="cuda")) > 0
+        want[bad & sees[:, None]] = math.nan
+        alike(ops().kv4_attention(cache, table, ints(keys), q, ints(starts), max(news), causal=causal, scale=scale), want, size, live)
