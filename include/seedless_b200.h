@@ -376,7 +376,7 @@ int32_t sl_op_kv4_read_device(const sl_kv4_cache* cache, const sl_kv4_read* rows
 /* out = softmax(scale * q K^T) V [* sigmoid(gate)] for the rows q_start[b] .. q_start[b + 1] - 1 of every request b over its positions
  * 0 .. kv_len[b] - 1; query head h reads kv head h / (q_heads / kv_heads), at most 128 of them one kv head; at most 4096 requests.  causal: row i of a request's n
  * sees the first kv_len - n + i + 1 positions.  A row that sees none is zero before its gate (a gate of NaN makes NaN
- * of anything); an infinity or a NaN in the query of a row that sees some makes it NaN; table entries that are no page of the cache hold no keys; rows of
+ * of anything); an infinity or a NaN in the query of a row that sees some makes it NaN; table entries that are no page of the cache, and positions past the table's columns, hold no keys; rows of
  * no request, and rows of a request behind its first max_q, are left as they were.  The requests' rows do not overlap.  Infinities and NaN in places
  * that a row does not see do not count, unless another row of its request sees them: then this row may be NaN too.
  * Waits inside the kernels are bounded; the rows of one that ran out are NaN.

@@ -1,7 +1,7 @@
 // kv4_attn.cu -- attention of a ragged batch of query rows over the cache held in 4 bits (kv4.cuh):
 //   out = softmax(scale * q K^T) V, optionally times sigmoid(gate), K and V the fp16 values that the codes stand for.
 // Request b's rows are q_start[b] .. q_start[b + 1] - 1, its keys positions 0 .. kv_len[b] - 1; causal: its row i of n sees
-// kv_len - n + i + 1 keys.  A row that sees none is zero.  A page that the cache does not have holds no keys.
+// kv_len - n + i + 1 keys.  A row that sees none is zero.  A page that the cache does not have, or the table no column for, holds no keys.
 //
 // Requests of up to 16 rows a kv head (tokens x query heads of the head) take k_kv4_decode, the others k_kv4_prompt.
 #include "kv4.cuh"
@@ -37,16 +37,19 @@ template <int D> constexpr size_t kd_ring = (size_t)KD_WARPS * kd_stages<D> * kv
 template <int D> constexpr size_t kd_smem(int batch) { return kd_ring<D> + (size_t)(batch + 1) * 4; }
 constexpr float KD_UP = 8.0f, KD_SLACK = 6.0f;
 
-// rows of request b (0: none, or more than `most` rows a kv head), and the units of one of its kv heads
-struct KdSeq { int q0, rows, keys, units; };
+// rows of request b (0: none, or more than `most` rows a kv head), its keys in the table, keys before the first row's own (as many as the
+// table's, if more), and the units of one of its kv heads
+struct KdSeq { int q0, rows, keys, past, units; };
 __device__ __forceinline__ KdSeq kd_seq(const Kv4Cache& c, const Kv4AttnArgs& a, int b, int most) {
     KdSeq s;
     s.q0 = a.q_start[b];
     const int n = a.q_start[b + 1] - s.q0;
     s.rows = min(min(n, a.max_q), a.rows - s.q0);
-    s.keys = min(max(a.kv_len[b], 0), a.table_width * c.page_size);
+    const int len = max(a.kv_len[b], 0);
+    s.keys = min(len, a.table_width * c.page_size);
+    s.past = min(len - n, s.keys);
     if (s.q0 < 0 || s.rows <= 0 || s.rows > most / a.G) { s.rows = 0; s.units = 0; return s; }
-    const int sees = a.causal ? min(s.keys, max(0, s.keys - n + s.rows)) : s.keys;                        // (rows behind max_q see more)
+    const int sees = a.causal ? min(s.keys, max(0, s.past + s.rows)) : s.keys;                            // (rows behind max_q see more)
     s.units = max(1, (sees + KV4_B - 1) / KV4_B);
     return s;
 }
@@ -146,7 +149,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv
             head = rel / sq.units; j0 = rel % sq.units; j1 = min(sq.units, j0 + (u1 - u));
         }
         const bool whole = j0 == 0 && j1 == sq.units;
-        const int n = a.q_start[b + 1] - sq.q0, live = sq.rows * a.G;        // rows of the tile that exist
+        const int live = sq.rows * a.G;                                       // rows of the tile that exist
         // ---- the warp's steps of U blocks: warp, + 4, .. of the item's; 32 blocks looked up at a time, a lane each
         const int mine = max(0, ((j1 - j0 + U - 1) / U - warp + KD_WARPS - 1) / KD_WARPS);
         const int* table = a.table + (int64_t)b * a.table_stride;
@@ -193,8 +196,8 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_ctas<D, NT>) k_kv4_decode(Kv
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) sees[nt][e] = a.causal ? sq.keys - n + (nt * 8 + 2 * t + e) / a.G + 1 : sq.keys;
-        if (a.causal) all = min(all, sq.keys - n + 1);
+            for (int e = 0; e < 2; ++e) sees[nt][e] = a.causal ? sq.past + (nt * 8 + 2 * t + e) / a.G + 1 : sq.keys;
+        if (a.causal) all = min(all, sq.past + 1);
         float o[NT][CH][2][4], base[NT][2], l[NT][2];                        // base: KD_UP - the maximum
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {

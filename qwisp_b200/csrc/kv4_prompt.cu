@@ -111,7 +111,7 @@ template <int D, int NQ> static bool kp_one(const Kv4AttnArgs& a) { return a.max
 template <int D, int NQ> static long long kp_items(const Kv4AttnArgs& a) { return kp_one<D, NQ>(a) ? a.batch : (long long)a.rows / (KP_M / a.G * NQ) + a.batch; }
 constexpr int KP_PARTS = 8;                                                   // CTAs of a cluster at most
 constexpr int KP_SPLIT = 256;                                                // keys a CTA of a cluster has at least, of a table's span
-struct KpSeq { int q0, rows, n, keys; };
+struct KpSeq { int q0, rows, keys, past; };                                   // past: keys before the first row's own (as many as the table's, if more)
 
 template <int D, int NQ, bool SPLIT>
 __global__ void __launch_bounds__(kp_threads<D, NQ>, kp_ctas<D, NQ>) k_kv4_prompt(Kv4Cache c, Kv4AttnArgs a, int least, uint32_t q_and, uint32_t q_xor, int parts) {
@@ -140,8 +140,11 @@ __global__ void __launch_bounds__(kp_threads<D, NQ>, kp_ctas<D, NQ>) k_kv4_promp
         int x = 0;
         KpSeq one{0, 0, 0, 0};
         if (b < a.batch) {
-            one.q0 = a.q_start[b]; one.n = a.q_start[b + 1] - one.q0; one.rows = min(min(one.n, a.max_q), a.rows - one.q0);
-            one.keys = min(max(a.kv_len[b], 0), a.table_width * c.page_size);
+            one.q0 = a.q_start[b];
+            const int n = a.q_start[b + 1] - one.q0, len = max(a.kv_len[b], 0);
+            one.rows = min(min(n, a.max_q), a.rows - one.q0);
+            one.keys = min(len, a.table_width * c.page_size);
+            one.past = min(len - n, one.keys);
             if (one.q0 >= 0 && one.rows > least / a.G) x = (one.rows + per_cta - 1) / per_cta;
         }
         const int own = x;
@@ -165,7 +168,7 @@ __global__ void __launch_bounds__(kp_threads<D, NQ>, kp_ctas<D, NQ>) k_kv4_promp
     const int t0 = s_tile * per_cta;                                          // first token
     const int nq = NQ == 1 || t0 + tokens >= sq.rows ? 1 : 2;                 // tiles that have rows
     const int last = min(t0 + per_cta, sq.rows) - 1;
-    const int span = a.causal ? min(sq.keys, max(0, sq.keys - sq.n + last + 1)) : sq.keys;
+    const int span = a.causal ? min(sq.keys, max(0, sq.past + last + 1)) : sq.keys;
     // keys KP_N j0 .. : all of them, or the cluster's CTAs share them out
     const int all_tiles = (span + KP_N - 1) / KP_N, per = (all_tiles + CL - 1) / CL, j0 = min(rank * per, all_tiles);
     const int tiles = min(per, all_tiles - j0);
@@ -377,9 +380,9 @@ __global__ void __launch_bounds__(kp_threads<D, NQ>, kp_ctas<D, NQ>) k_kv4_promp
                 __syncwarp();
                 if (lane == 0) kp_arrive(&q_full);
             }
-            const int sees = !live ? 0 : a.causal ? sq.keys - sq.n + tok + 1 : sq.keys;
+            const int sees = !live ? 0 : a.causal ? sq.past + tok + 1 : sq.keys;
             // keys that all of the tile's rows see
-            const int all = a.causal ? min(sq.keys, sq.keys - sq.n + t0 + q * tokens + 1) : sq.keys;
+            const int all = a.causal ? min(sq.keys, sq.past + t0 + q * tokens + 1) : sq.keys;
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < tiles && ok; ++j) {
                 const int slot = 2 * q + (j & 1), k0 = (j0 + j) * KP_N;

@@ -1,5 +1,5 @@
-"""Values at the edges of the attention over the 4-bit KV cache: gates and queries that are no numbers.
-The kernels' tolerances are those of test_gpu_kv4.py, whose references these tests use."""
+"""Values at the edges of the attention over the 4-bit KV cache: gates and queries that are no numbers, lengths past
+the table.  The kernels' tolerances are those of test_gpu_kv4.py, whose references these tests use."""
 import math
 
 import pytest
@@ -74,3 +74,22 @@ def test_queries_that_are_no_numbers(case, scale):
             sees[lo:hi] = (n - (hi - lo) + torch.arange(hi - lo, device="cuda") + 1 if causal else torch.full((hi - lo,), n, device="cuda")) > 0
         want[bad & sees[:, None]] = math.nan
         alike(ops().kv4_attention(cache, table, ints(keys), q, ints(starts), max(news), causal=causal, scale=scale), want, size, live)
+
+
+@pytest.mark.parametrize("D,NH,KV,news,keys,pages", [(128, 8, 2, [1, 1, 1], [1000, 64, 129], 2), (64, 8, 2, [3, 5], [140, 131], 2), (256, 16, 2, [2], [900], 9), (128, 16, 4, [40, 70], [140, 150], 2),
+                                                     (64, 4, 4, [30] * 5, [70, 64, 80, 94, 93], 1), (128, 8, 2, [65, 3], [2100, 70], 30), (256, 8, 8, [33], [100], 1)])
+@pytest.mark.parametrize("more", [0, 3000])
+def test_lengths_past_the_table(D, NH, KV, news, keys, pages, more):
+    """Positions that the table has no page for hold no keys, like those of entries of no page: a causal row's place goes by the
+    request's length all the same."""
+    cache, table, q, starts = attention_case(D, NH, KV, 64, news, keys)
+    cut = table[:, :pages].contiguous()
+    gone = table.clone()
+    gone[:, pages:] = -1
+    for causal in (True, False):
+        want = attention_reference(cache, gone, keys, q, starts, causal, D ** -0.5)
+        near(ops().kv4_attention(cache, cut, ints(keys), q, ints(starts), max(news), causal=causal), *want)
+        near(ops().kv4_attention(cache, torch.nn.functional.pad(gone, (0, more), value=-1), ints(keys), q, ints(starts), max(news), causal=causal), *want)
+    # the longest length that there is
+    far = ops().kv4_attention(cache, cut, ints([2 ** 31 - 1] * len(keys)), q, ints(starts), max(news))
+    assert torch.equal(far, ops().kv4_attention(cache, cut, ints([pages * 64] * len(keys)), q, ints(starts), max(news), causal=False))
