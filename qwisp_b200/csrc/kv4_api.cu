@@ -18,10 +18,10 @@ bool cache_of(const sl_kv4_cache* c, Kv4Cache& o) {
     o = Kv4Cache{(unsigned char*)c->data, c->page_stride, c->pages, c->page_size, c->kv_heads, c->head_dim};
     return true;
 }
-// the status of an enqueued launch
+// The status of a call's launches, which report their own errors: one that another call has left behind is not looked at, and none is left.
 int32_t launched(int err, const char* what) {
-    if (err == 0) err = (int)cudaGetLastError();
     if (err == 0) return SL_OK;
+    cudaGetLastError();
     fprintf(stderr, "%s: CUDA error %d (%s)\n", what, err, cudaGetErrorString((cudaError_t)err));
     return SL_ERR_CUDA;
 }

@@ -249,3 +249,42 @@ if gathered > 24:                                          # (shorter plain call
     s.forward([1] * gathered)
     assert [b - a for a, b in zip(before, blocks())] == one
 """)
+
+
+def test_a_failed_launch_of_the_4_bit_cache_is_that_calls_alone(fake):
+    """Each operator around the 4-bit KV cache reports a launch of its own that fails, at whichever it is, and leaves no error for the next call;
+    an error that somebody else has left is neither reported nor taken away."""
+    fake("""
+L, P = Q._lib, 1 << 20
+lib = L.lib()
+cache = L.SlKv4Cache(data=P, page_stride=2 * 4 * 18 * 128, pages=8, page_size=64, kv_heads=2, head_dim=128)
+plan = L.SlKvPlan(lens=P, new_rows=P, batch=4, page_size=64, table=P, table_stride=8, table_width=8, free_pages=P, free_capacity=32, free_count=P,
+                  kv_len=P, q_start=P, slots=P, pos=P, max_rows=10000, free_count_out=P, status=P)
+append = L.SlKv4Append(q=P, k=P, v=P, q_row=1024, q_head=128, k_row=256, k_head=128, v_row=256, v_head=128, q_out=P, q_out_row=1024, q_out_head=128, rows=3, q_heads=8, slots=P)
+read = L.SlKv4Read(slots=P, rows=3, k=P, v=P, k_row=256, k_head=128, v_row=256, v_head=128)
+
+def attention(max_q, width, scale=0.1):
+    return L.SlKv4Attention(q=P, q_row=1024, q_head=128, out=P, out_row=1024, out_head=128, rows=300, q_heads=8, q_start=P, kv_len=P, batch=2, max_q=max_q,
+                            table=P, table_stride=width, table_width=width, causal=1, scale=scale, workspace=P, workspace_bytes=1 << 40)
+
+calls = [(lib.sl_op_kv_plan_device, plan, None), (lib.sl_op_kv4_append_device, cache, append), (lib.sl_op_kv4_read_device, cache, read),
+         (lib.sl_op_kv4_attention_device, cache, attention(1, 8)), (lib.sl_op_kv4_attention_device, cache, attention(1, 4096)),
+         (lib.sl_op_kv4_attention_device, cache, attention(150, 8)), (lib.sl_op_kv4_attention_device, cache, attention(150, 4096))]
+kernels = []
+for fn, a, b in calls:
+    args = [C.byref(x) for x in (a, b) if x is not None] + [None]
+    before = count("launches")
+    assert fn(*args) == 0
+    n = count("launches") - before
+    kernels.append(n)
+    for k in range(n):
+        F.fake_fail_launches(k)
+        assert fn(*args) == -3
+        F.fake_fail_launches(-1)
+        assert F.cudaGetLastError() == 0
+        assert fn(*args) == 0
+    assert F.cudaStreamBeginCapture(None, 0) != 0                # (of another's call)
+    assert fn(*args) == 0
+    assert F.cudaGetLastError() != 0 and F.cudaGetLastError() == 0
+assert kernels == [2, 1, 1, 1, 2, 2, 3], kernels
+""")
