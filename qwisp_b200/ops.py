@@ -146,15 +146,18 @@ def _cuda():
             getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream))
 
 
+def _on(index, fn, *args):
+    """fn's result with that device current."""
+    if _cuda()[0]() == index:
+        return fn(*args)
+    import torch
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
 def _call(fn, index, where, *blocks):
     """The call on the device's current stream."""
-    device, stream = _cuda()
-    if device() == index:
-        rc = fn(*blocks, stream(index))
-    else:
-        import torch
-        with torch.cuda.device(index):
-            rc = fn(*blocks, stream(index))
+    rc = _on(index, fn, *blocks, _cuda()[1](index))
     if rc != 0:
         raise SeedlessError(rc, where)
 
@@ -297,20 +300,23 @@ def kv4_read(cache, slots, k=None, v=None):
 
 
 @functools.lru_cache(maxsize=256)
+def _workspace(index, q_heads, kv_heads, head_dim, batch, max_q, span):
+    """Bytes of workspace of such a call on that device (-1: whichever is current), by its number of multiprocessors; span None: tables of any width."""
+    call = (q_heads, kv_heads, head_dim, batch, max_q)
+    fn, where, more = (lib().sl_kv4_attention_workspace, "sl_kv4_attention_workspace", 0) if span is None else \
+        (lib().sl_kv4_attention_workspace_span, "sl_kv4_attention_workspace_span", span)
+    n = fn(*call, more) if index < 0 else _on(index, fn, *call, more)
+    if n < 0:
+        raise SeedlessError(n, where)
+    return n
+
+
 def kv4_attention_workspace(q_heads, kv_heads, head_dim, batch, max_q, rows):
-    """Bytes of workspace of such a call of kv4_attention."""
-    n = lib().sl_kv4_attention_workspace(q_heads, kv_heads, head_dim, batch, max_q, rows)
-    if n < 0:
-        raise SeedlessError(n, "sl_kv4_attention_workspace")
-    return n
-
-
-@functools.lru_cache(maxsize=256)
-def _workspace_span(q_heads, kv_heads, head_dim, batch, max_q, span):
-    n = lib().sl_kv4_attention_workspace_span(q_heads, kv_heads, head_dim, batch, max_q, span)
-    if n < 0:
-        raise SeedlessError(n, "sl_kv4_attention_workspace_span")
-    return n
+    """Bytes of workspace of such a call of kv4_attention on the current device."""
+    import torch
+    if rows < 0:
+        raise _no("sl_kv4_attention_workspace", "rows is not negative")
+    return _workspace(torch.cuda.current_device() if torch.cuda.is_available() else -1, q_heads, kv_heads, head_dim, batch, max_q, None)
 
 
 def kv4_attention(cache, table, kv_len, q, q_start, max_q, *, causal=True, scale=None, gate=None, out=None, workspace=None):
@@ -337,12 +343,12 @@ def kv4_attention(cache, table, kv_len, q, q_start, max_q, *, causal=True, scale
     ga = (0, 0, 0) if gate is None else _heads(where, "gate", gate, shape, index)
     la, ra = _flat(where, "kv_len", kv_len, i32, B, index), _flat(where, "q_start", q_start, i32, B + 1, index)
     if workspace is None:
-        size = _workspace_span(heads, kv, dim, B, max_q, width * page)
+        size = _workspace(index, heads, kv, dim, B, max_q, width * page)
         if size:
             workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
         wa = workspace.data_ptr() if size else qa[0]
     else:
-        need, size = kv4_attention_workspace(heads, kv, dim, B, max_q, rows), workspace.numel()
+        need, size = _workspace(index, heads, kv, dim, B, max_q, None), workspace.numel()
         if size < need:
             raise _no(where, f"workspace has to have {need} bytes")
         wa = _flat(where, "workspace", workspace, torch.uint8, None, index)

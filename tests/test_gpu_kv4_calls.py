@@ -20,3 +20,13 @@ def test_requests_that_share_a_row_of_the_table(D, NH, KV, new, keys, more):
         got = ops().kv4_attention(cache, shared, ints(keys), q, ints(starts), new, causal=causal)
         assert torch.equal(got, ops().kv4_attention(cache, row.repeat(len(keys), 1), ints(keys), q, ints(starts), new, causal=causal))
         near(got, *attention_reference(cache, shared, keys, q, starts, causal, D ** -0.5))
+
+
+def test_workspace_of_the_current_device():
+    cache, table, q, starts = attention_case(128, 8, 2, 64, [1, 1], [100, 40])
+    size = ops().kv4_attention_workspace(8, 2, 128, 2, 1, 2)
+    assert size > 0 and size == ops().kv4_attention_workspace(8, 2, 128, 2, 1, 500)
+    want = ops().kv4_attention(cache, table, ints([100, 40]), q, ints(starts), 1)
+    assert torch.equal(want, ops().kv4_attention(cache, table, ints([100, 40]), q, ints(starts), 1, workspace=torch.empty(size, dtype=torch.uint8, device="cuda")))
+    with pytest.raises(Exception):
+        ops().kv4_attention_workspace(8, 2, 128, 2, 1, -1)

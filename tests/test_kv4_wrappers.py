@@ -13,12 +13,18 @@ F16, I32, I64 = torch.float16, torch.int32, torch.int64
 
 
 class OnDevice(torch.Tensor):
+    index = 0
+
     def get_device(self):
-        return 0
+        return self.index
 
 
-def on(t):
-    return t.as_subclass(OnDevice)
+class OnAnother(OnDevice):
+    index = 1
+
+
+def on(t, device=OnDevice):
+    return t.as_subclass(device)
 
 
 def ints(*v):
@@ -29,6 +35,7 @@ def ints(*v):
 def blocks(monkeypatch):
     """The argument blocks of the calls that would have been made."""
     made = []
+    monkeypatch.setattr(ops, "_cuda", lambda: (lambda: 0, lambda index: 0))
     monkeypatch.setattr(ops, "_call", lambda fn, index, where, *b: made.append((where, b)))
     return made
 
@@ -78,3 +85,48 @@ def test_the_library_refuses_rows_that_overlap_in_part():
         call = _lib.SlKv4Attention(q=P, q_row=1024, q_head=128, out=P, out_row=1024, out_head=128, rows=0, q_heads=8, q_start=P, kv_len=P, batch=2, max_q=2, table=P,
                                    table_stride=stride, table_width=width, causal=1, scale=0.1, workspace=P, workspace_bytes=1 << 40)
         assert _lib.lib().sl_op_kv4_attention_device(C.byref(cache), C.byref(call), None) in want
+
+
+def test_the_workspace_is_that_of_the_tensors_device(monkeypatch):
+    """Devices of different numbers of multiprocessors: the size is asked for with the call's device current, and kept for each."""
+    import contextlib
+    current, calls = [0], []
+
+    class Lib:
+        sl_kv4_attention_workspace = staticmethod(lambda *a: 1000 * (current[0] + 1))
+        sl_kv4_attention_workspace_span = staticmethod(lambda *a: 10 * (current[0] + 1))
+
+        @staticmethod
+        def sl_op_kv4_attention_device(cache, block, stream):
+            calls.append((current[0], _lib.SlKv4Attention.from_buffer_copy(block).workspace_bytes))
+            return 0
+
+    @contextlib.contextmanager
+    def device(index):
+        before, current[0] = current[0], index
+        yield
+        current[0] = before
+
+    monkeypatch.setattr(ops, "lib", Lib)
+    monkeypatch.setattr(ops, "_cuda", lambda: (lambda: current[0], lambda index: 0))
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    ops._workspace.cache_clear()
+
+    def attend(kind, **kw):
+        z = lambda *shape, dtype=I32: on(torch.zeros(shape, dtype=dtype), kind)  # noqa: E731
+        ops.kv4_attention(z(4, 1, 4, 18 * 64, dtype=torch.uint8), z(3, 5), z(3), z(3, 2, 64, dtype=F16), z(4), 1, **{k: on(v, kind) for k, v in kw.items()})
+
+    try:
+        for now in (0, 1, 0):
+            current[0] = now
+            for kind in (OnDevice, OnAnother, OnDevice):
+                attend(kind)
+                assert calls.pop() == (kind.index, 10 * (kind.index + 1)) and current[0] == now
+                attend(kind, workspace=torch.zeros(1000 * (kind.index + 1), dtype=torch.uint8))
+                assert calls.pop() == (kind.index, 1000 * (kind.index + 1))
+                refused(lambda: attend(kind, workspace=torch.zeros(1000 * (kind.index + 1) - 1, dtype=torch.uint8)))  # noqa: B023
+            assert ops.kv4_attention_workspace(2, 1, 64, 3, 1, 3) == 1000 * (now + 1)
+    finally:
+        ops._workspace.cache_clear()
