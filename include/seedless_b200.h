@@ -379,7 +379,8 @@ int32_t sl_op_kv4_read_device(const sl_kv4_cache* cache, const sl_kv4_read* rows
  * of anything); an infinity or a NaN in the query of a row that sees some makes it NaN; table entries that are no page of the cache, and positions past the table's columns, hold no keys; rows of
  * no request, and rows of a request behind its first max_q, are left as they were.  The requests' rows do not overlap.  Infinities and NaN in places
  * that a row does not see do not count, unless another row of its request sees them: then this row may be NaN too.
- * Waits inside the kernels are bounded; the rows of one that ran out are NaN.
+ * The polls of barriers inside the kernels are bounded; the rows of one that ran out are NaN.  Waits for tensor memory and for the other CTAs of a cluster
+ * have no limit of their own: they are for CTAs that run, and no two of these kernels hold what the other waits for.
  * workspace: 16-byte aligned, sl_kv4_attention_workspace() bytes (the same arguments), any contents; calls that may run at the same
  * time need one each. */
 typedef struct sl_kv4_attention {

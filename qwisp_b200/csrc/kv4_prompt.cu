@@ -35,9 +35,16 @@ template <int D> constexpr int kp_tile = KP_N * D * 2;                        //
 template <int D> constexpr bool kp_qt = D != 128;                            // queries in tensor memory (128 dims: outputs and scores fill it)
 template <int D, int NQ> constexpr int kp_io = 4 * NQ * 4096;      // where a softmax warp turns 32 rows of 64 dims
 template <int D, int NQ> constexpr int kp_bytes = 2 * KP_ST * kp_tile<D> + kp_io<D, NQ> + (kp_qt<D> ? 0 : NQ * KP_M * D * 2);
-// (so much that no more CTAs come to a multiprocessor than there is tensor memory for: the next would wait for it)
-template <int D, int NQ> constexpr int kp_least = (kp_ctas<D, NQ> == 2 ? 80 : 120) * 1024;
+// So much that no more of these kernels' CTAs, calls on other streams included, come to a multiprocessor than there is tensor memory for.
+// tcgen05.alloc and the meetings of a cluster wait without a limit: two clusters, each with a CTA that has its tensor memory and one that waits
+// for the other cluster's, would wait for ever.
+template <int D, int NQ> constexpr int kp_least = (kp_ctas<D, NQ> == 2 ? 80 : 148) * 1024;
 template <int D, int NQ> constexpr int kp_smem = (kp_bytes<D, NQ> > kp_least<D, NQ> ? kp_bytes<D, NQ> : kp_least<D, NQ>) + 1024;
+constexpr int KP_SM = 228 * 1024;                                            // of a multiprocessor; a CTA takes 1 KB more than it asks for
+static_assert(3 * (kp_smem<64, 1> + 1024) > KP_SM && kp_smem<64, 1> + kp_smem<64, 2> + 2048 > KP_SM && kp_smem<64, 1> + kp_smem<128, 2> + 2048 > KP_SM &&
+              kp_smem<64, 1> + kp_smem<256, 1> + 2048 > KP_SM && 2 * (kp_smem<64, 2> + 1024) > KP_SM && kp_smem<64, 2> + kp_smem<128, 2> + 2048 > KP_SM &&
+              kp_smem<64, 2> + kp_smem<256, 1> + 2048 > KP_SM && 2 * (kp_smem<128, 2> + 1024) > KP_SM && kp_smem<128, 2> + kp_smem<256, 1> + 2048 > KP_SM &&
+              2 * (kp_smem<256, 1> + 1024) > KP_SM, "tensor memory of a multiprocessor");
 constexpr int KP_LIMIT = 1 << 22;                                            // polls of a wait (up to 4 us each)
 constexpr float KP_UP = 8.0f, KP_SLACK = 6.0f;
 
