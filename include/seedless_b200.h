@@ -375,12 +375,15 @@ int32_t sl_op_kv4_read_device(const sl_kv4_cache* cache, const sl_kv4_read* rows
 
 /* out = softmax(scale * q K^T) V [* sigmoid(gate)] for the rows q_start[b] .. q_start[b + 1] - 1 of every request b over its positions
  * 0 .. kv_len[b] - 1; query head h reads kv head h / (q_heads / kv_heads), at most 128 of them one kv head; at most 4096 requests.  causal: row i of a request's n
- * sees the first kv_len - n + i + 1 positions.  A row that sees none is zero before its gate (a gate of NaN makes NaN
- * of anything); an infinity or a NaN in the query of a row that sees some makes it NaN; table entries that are no page of the cache, and positions past the table's columns, hold no keys; rows of
- * no request, and rows of a request behind its first max_q, are left as they were.  The requests' rows do not overlap.  Infinities and NaN in places
- * that a row does not see do not count, unless another row of its request sees them: then this row may be NaN too.
+ * sees the first kv_len - n + i + 1 positions.  A row that sees none is zero before its gate (a gate of NaN makes NaN of anything); an infinity or a
+ * NaN in the query of a row that sees some makes it NaN.  Table entries that are no page of the cache, and positions past the table's columns, hold no
+ * keys; rows of no request, and rows of a request behind its first max_q, are left as they were.  The requests' rows do not overlap.  Infinities and NaN
+ * in places that a row does not see do not count, unless another row of its request sees them: then this row may be NaN too.
  * The polls of barriers inside the kernels are bounded; the rows of one that ran out are NaN.  Waits for tensor memory and for the other CTAs of a cluster
  * have no limit of their own: they are for CTAs that run, and no two of these kernels hold what the other waits for.
+ * A call repeated gives the same bits.  A row's bits may change with the table's width, max_q, the batch and its rows, and in wide tables with the
+ * other requests' lengths: kernels and the places where sums are split go by them.  The kernels take the table's width for the longest
+ * request's length: a table cut to the step's longest is faster for few or short requests.
  * workspace: 16-byte aligned, sl_kv4_attention_workspace() bytes (the same arguments), any contents; calls that may run at the same
  * time need one each. */
 typedef struct sl_kv4_attention {

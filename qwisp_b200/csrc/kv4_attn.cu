@@ -475,7 +475,8 @@ constexpr int KD_LEAST = 8;              // units a CTA takes at least
 // Positions x dims of a table's row for each CTA of a cluster, at most: 1024 positions of 128.  GPU time of a call by clusters | evenly dealt out, us
 // (the call as a program waits for it, launches and all, in brackets).  Heads of 128, 32/8: 1 x 1001 positions 8.2 | 12.3, 1 x 4001 10.3 | 13.3, 1 x 8101
 // 14.4 | 16.4, 7 x (2000 + 4) 14.4 | 20.3, 16 x 1001 12.2 | 16.4, 64 x up to 1001 22.9 | 32.2.  16/2 of 256: 1 x 513 8.2 | 14.3, 1 x 2048 10.3 | 11.3, 1 x 4096
-// 14.4 | 12.3 [14.7 | 17.5], 1 x 8101 20.5 | 16.4.  8/1 of 64: 1 x 16001 16.4 | 13.6 [16.5 | 18.9].  Four CTAs for 16 x up to 8101 of 128: 36.9 | 35.4.
+// 14.4 | 12.3 [14.7 | 17.5], 1 x 8101 20.5 | 16.4.  8/1 of 64: 1 x 16001 16.4 | 13.6 [16.5 | 18.9].  The bound is that of the call in brackets: the second
+// launch costs the host more there than it saves the GPU.  In a graph dealing out would be 2 to 3 us ahead at those two.  Four CTAs for 16 x up to 8101 of 128: 36.9 | 35.4.
 constexpr long long KD_CL_SPAN = 1024 * 128;
 // CTAs of a cluster for that many (request, kv head) pairs with tables of `span` positions; 0: the work is dealt out evenly.  One CTA a pair may have the
 // longer spans the more pairs there are, beside which a long one does not show.  By single CTAs | dealt out, us, heads of 128, 32/8: 128 x up to 301 18.7 | 30.8,

@@ -15,8 +15,8 @@
 // SPLIT: where there are fewer tiles than multiprocessors a cluster of up to eight CTAs takes each, a run of the keys a CTA, and adds up its sums through shared
 // memory.  17 rows over 4017 positions, 32/8 heads of 128: 55 us with one CTA, 18.5 with eight.
 //
-// What bounds it: 1024 rows over 8192 positions, 16/2 heads of 256: 136 us, 0.95 PFLOP/s = 0.56 of the measured cuBLAS rate; four prompts of up to
-// 2900, 32/8 heads of 128: 220 us, 0.78 PFLOP/s = 0.46.  No unit is full (tensor pipe 39 %, MUFU 40 %, ALU 33 %, issue slots 43 % of the second): each tile of
+// What bounds it: 1024 rows over 8192 positions, 16/2 heads of 256: 134 us, 0.96 PFLOP/s = 0.57 of the measured cuBLAS rate; four prompts of up to
+// 2900, 32/8 heads of 128: 227 us, 0.75 PFLOP/s = 0.45.  No unit is full (tensor pipe 39 %, MUFU 40 %, ALU 33 %, issue slots 43 % of the second): each tile of
 // 64 keys is a chain scores -> exponents -> weights -> outputs over barriers, which two tiles of rows overlap only in part, and every CTA begins
 // and ends alone (about 10 of 29 us there).  Leaving out the exponentials gave 12 %, the expansion 5 %, half of the MMAs nothing.  Tried, and no faster:
 // tiles of 128 keys with one score buffer (7 % slower), two CTAs of one tile each (1.8 times the time: twice the expansion, 96 registers), more expanding

@@ -8,10 +8,10 @@
 // a NaN gets a NaN scale: all of it reads back as NaN.
 // k_kv4_read: fp16(code * scale + bias) of K and V at given slots.
 //
-// What bounds them.  Append, 4093 rows of 32/8 heads of 128 with norms and three axes, at scattered slots: 34 us, 2.0 TB/s with what it reads
-// and writes, bound by issue: the quantiser (two divisions for a group, eight rounded quotients a word, exact) is some 200 instructions a lane's word, and
-// keys in 64 bits about 4 us of it.  One row: 4 us, latency.  Read, 30001 rows of 8 heads of 128: 45 us, 3.5 TB/s: 123 MB of writes, which a
-// fill alone needs 35 us for (floor at the copy rate: 24).  Larger CTAs, more CTAs a row, streaming stores, eight words in flight: no faster.
+// What bounds them.  Append, 4093 rows of 32/8 heads of 128 with norms and three axes, at scattered slots: 34 us, 2.6 TB/s with what it reads
+// and writes.  No unit is full: issue slots 64 %, 5.9 warps a scheduler, which wait for results in flight and for shared memory.  The quantiser (two divisions
+// for a group, eight rounded quotients a word, exact) is some 200 instructions a lane's word; keys in 64 bits are about 4 us.  One row: 4 us, latency.
+// Read, 30001 rows of 8 heads of 128: 45 us, 3.5 TB/s: 123 MB of writes, which a fill alone needs 35 us for (floor at the copy rate: 24).  Larger CTAs, more CTAs a row, streaming stores, eight words in flight: no faster.
 #include "kv4.cuh"
 #include "kv4_mma.cuh"
 
@@ -65,7 +65,7 @@ __device__ __forceinline__ void kv4_store(unsigned char* blk, int at, int region
 }
 
 // A row's angles once per CTA: turns = position * frequency as a 64-bit fraction of a turn, exact for every position, then cos and
-// sin in 64 bits.  Keys stay in 64 bits up to the one rounding to fp16 (a code next to a border then does not go by the order of a sum or
+// sin in 64 bits.  Keys stay in 64 bits up to their rounding, to fp32 and then fp16 (a code next to a border then does not go by the order of a sum or
 // by the shape of the launch); queries take 32.
 // RPC rows at a time, KA_WARPS / RPC warps each; grid (row groups, parts).  A warp's task: 32 / (D / 8) heads of one kind, eight dims a lane,
 // the next task's halves on their way.  Many rows: CTAs that stay, so that frequencies and weights are fetched once (from the parameters a
