@@ -171,6 +171,14 @@ def _heads(where, name, t, shape, index):
     return t.data_ptr(), by[0], by[1]
 
 
+def _heads_out(where, name, t, shape, index):
+    """The same of one that is written: an expanded one has one place for many results."""
+    at = _heads(where, name, t, shape, index)
+    if (at[1] == 0 and shape[0] > 1) or (at[2] == 0 and shape[1] > 1):
+        raise _no(where, f"{name} is written: its rows and heads must not overlap")
+    return at
+
+
 def _flat(where, name, t, dtype, n, index):
     """The pointer of a contiguous tensor of n values (None: any number) on that device."""
     if t.dtype is not dtype or (n is not None and t.shape != (n,)) or not t.is_contiguous() or t.get_device() != index:
@@ -246,7 +254,7 @@ def kv4_append(cache, slots, q=None, k=None, v=None, *, q_norm=None, k_norm=None
             q_out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((rows, heads, dim))
             oa = (q_out.data_ptr(), heads * dim, dim)
         else:
-            oa = _heads(where, "q_out", q_out, (rows, heads, dim), index)
+            oa = _heads_out(where, "q_out", q_out, (rows, heads, dim), index)
     if k is not None:
         ka, va = _heads(where, "k", k, (rows, kv, dim), index), _heads(where, "v", v, (rows, kv, dim), index)
         if slots is None:
@@ -289,12 +297,12 @@ def kv4_read(cache, slots, k=None, v=None):
         k = cache.new_empty(shape, dtype=torch.float16)
         kp, kr, kh = k.data_ptr(), kv * dim, dim
     else:
-        kp, kr, kh = _heads(where, "k", k, shape, index)
+        kp, kr, kh = _heads_out(where, "k", k, shape, index)
     if v is None:
         v = torch.empty_like(k) if k.is_contiguous() else cache.new_empty(shape, dtype=torch.float16)
         vp, vr, vh = v.data_ptr(), kv * dim, dim
     else:
-        vp, vr, vh = _heads(where, "v", v, shape, index)
+        vp, vr, vh = _heads_out(where, "v", v, shape, index)
     if rows:
         _call(lib().sl_op_kv4_read_device, index, where, block, _READ.pack(sa, rows, kp, vp, kr, kh, vr, vh))
     return k, v
@@ -342,7 +350,7 @@ def kv4_attention(cache, table, kv_len, q, q_start, max_q, *, causal=True, scale
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
         oa = (out.data_ptr(), heads * dim, dim)
     else:
-        oa = _heads(where, "out", out, shape, index)
+        oa = _heads_out(where, "out", out, shape, index)
     ga = (0, 0, 0) if gate is None else _heads(where, "gate", gate, shape, index)
     la, ra = _flat(where, "kv_len", kv_len, i32, B, index), _flat(where, "q_start", q_start, i32, B + 1, index)
     if workspace is None:

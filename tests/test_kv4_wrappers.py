@@ -75,6 +75,27 @@ def test_a_table_that_grows_in_place_has_rows_of_its_own(blocks):
     assert not blocks
 
 
+def test_results_have_places_of_their_own(blocks):
+    """Outputs that are one row, or one head, expanded are refused; expanded inputs are not, nor is a stride of zero where there is one row."""
+    cache = on(torch.zeros((4, 2, 4, 18 * 64), dtype=torch.uint8))
+    full, slots = on(torch.zeros((3, 2, 64), dtype=F16)), on(torch.zeros(3, dtype=I64))
+    rows, heads = full[:1].expand(3, -1, -1), full[:, :1].expand(-1, 2, -1)
+    table, lens, starts = on(torch.zeros((3, 5), dtype=I32)), ints(5, 5, 5), ints(0, 1, 2, 3)
+    for bad in (rows, heads):
+        refused(lambda: ops.kv4_append(cache, slots, full, q_out=bad))  # noqa: B023
+        refused(lambda: ops.kv4_read(cache, slots, k=bad, v=full))  # noqa: B023
+        refused(lambda: ops.kv4_read(cache, slots, k=full, v=bad))  # noqa: B023
+        refused(lambda: ops.kv4_attention(cache, table, lens, full, starts, 1, out=bad))  # noqa: B023
+        assert not blocks
+        ops.kv4_append(cache, slots, bad, bad, bad, q_out=full)
+        ops.kv4_attention(cache, table, lens, bad, starts, 1, gate=bad, out=full)
+        assert len(blocks) == 2
+        blocks.clear()
+    one = full.as_strided((1, 2, 64), (0, 64, 1))
+    ops.kv4_attention(cache, table[:1], ints(5), one, ints(0, 1), 1, out=one)
+    assert blocks
+
+
 def test_the_library_refuses_rows_that_overlap_in_part():
     """One row for all requests, but not rows that begin inside one another.  (Pointers that nothing follows: without a device the call
     that is in order ends there, with one it has no rows.)"""
